@@ -287,6 +287,107 @@ int mgpu_argmax_logits(const mgpu_device* dev, mgpu_buf* logits, int vocab_size)
  * result is argmax_logits' first maximum over the whole row.  One thread, one launch. */
 mgpu_event* mgpu_argmax_combine(const mgpu_device* dev, mgpu_buf* pairs, int n_ranks, int n_total, mgpu_buf* out);
 
+/* ---------------------------------------------------------------- paged KV cache --- */
+/* New (the reference keeps one contiguous cache per sequence of at most max_seq_len tokens,
+ * kv_cache_append, src/models/moondream2.cpp:302-314).  One layer's keys and values in pages of
+ * page_size tokens, shared by all sequences: K and V are [num_pages][kv_heads][page_size][head_dim]
+ * of fp16 or bf16.  page_size a multiple of 8, head_dim a multiple of 8 and at most 128.  k and v:
+ * NULL (allocated here, zeroed) or the caller's buffers (16-byte aligned, num_pages * kv_heads *
+ * page_size * head_dim elements each, which must outlive the cache).  mgpu_kv_cache_k / _v give
+ * the buffers the cache uses; they belong to it. */
+typedef struct mgpu_kv_cache mgpu_kv_cache;
+mgpu_kv_cache* mgpu_kv_cache_create(const mgpu_device* dev, int num_pages, int page_size, int kv_heads, int head_dim,
+                                    int type, mgpu_buf* k, mgpu_buf* v);
+mgpu_buf* mgpu_kv_cache_k(const mgpu_kv_cache* cache);
+mgpu_buf* mgpu_kv_cache_v(const mgpu_kv_cache* cache);
+void mgpu_kv_cache_release(mgpu_kv_cache* cache);
+/* The sequences of one step and where they stand in the cache.  Sequence b's new tokens are rows
+ * cu_q[b] .. cu_q[b+1]-1 of the step's activations, the last ones of its kv_lens[b] tokens (the
+ * new ones included): new token i has index kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i.  Its token at
+ * index x is in page page_table[b][x / page_size] at place x % page_size.  All three are int32
+ * device buffers that the kernels read when they run, so a captured graph follows their contents;
+ * the counts below are the host's: n_tokens activation rows (rows of no sequence are left alone),
+ * max_q_len the most new tokens of a sequence, max_pages the row pitch of page_table.  Contents
+ * that do not fit (pages outside the cache, more new tokens than max_q_len, lengths beyond
+ * max_pages * page_size, a new token before index 0) are skipped, and the next mgpu_finish or
+ * mgpu_buf_read reports MGPU_ERR_INVALID_ARG; no access leaves the buffers. */
+typedef struct mgpu_paged_batch {
+    mgpu_buf* cu_q;       /* int32 [n_seqs + 1] */
+    mgpu_buf* kv_lens;    /* int32 [n_seqs] */
+    mgpu_buf* page_table; /* int32 [n_seqs][max_pages] */
+    int n_seqs;
+    int n_tokens;
+    int max_q_len;
+    int max_pages;
+} mgpu_paged_batch;
+/* The position rotation of the first rot_dim dimensions of a head (the rest pass unchanged).
+ * Pair i of the rot_dim / 2 pairs is dimensions (i, i + rot_dim / 2), or (2i, 2i + 1) with
+ * `interleaved`; it turns by the angle whose {cos, sin} is table[position][i].  The pairs are
+ * dealt to n_axes axes (1 to 3, e.g. time, height, width) in runs of sections[a]; a token's
+ * position on axis a is positions[a][token].  positions NULL: its index in the sequence, on every
+ * axis.  A position outside [0, max_pos) is reported like the contents above. */
+typedef struct mgpu_rope {
+    mgpu_buf* table;     /* fp32 [max_pos][rot_dim / 2][2], e.g. from mgpu_rope_table */
+    mgpu_buf* positions; /* int32 [n_axes][n_tokens], or NULL */
+    int max_pos;
+    int rot_dim;
+    int interleaved;
+    int n_axes;
+    int sections[3]; /* pairs of each axis; sum rot_dim / 2 */
+} mgpu_rope;
+/* table[p][i] = {cos, sin}(p * theta^(-2i / rot_dim)), computed in fp64 and rounded once. */
+mgpu_event* mgpu_rope_table(const mgpu_device* dev, mgpu_buf* table, int max_pos, int rot_dim, double theta);
+/* One step's keys and values into the cache, keys rotated on the way, and the queries rotated
+ * into q_out: dispatch_rope_apply on q and k followed by kv_cache_append (moondream2.cpp:406-420)
+ * in one launch.  q [n_tokens][q_heads * head_dim], k and v [n_tokens][kv_heads * head_dim], f32 /
+ * f16 / bf16 each, rows at their tag's pitch (so they may be views into one qkv projection);
+ * q_out f32 / f16 / bf16, may be q itself.  q and q_out NULL: only the cache.  rope NULL: no
+ * rotation.  fp32 arithmetic, one rounding.  Two tokens of a step must not share a slot. */
+mgpu_event* mgpu_kv_append(const mgpu_kv_cache* cache, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* k,
+                           mgpu_buf* v, mgpu_buf* q_out, int q_heads, const mgpu_rope* rope);
+/* Attention of the step's tokens over the cache (their own keys and values appended before):
+ * out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j][h / (q_heads / kv_heads)]) V[j][..] over the
+ * indexes j < kv_lens[b] that the token at index p sees: j <= p if causal, and p - j < window if
+ * window > 0.  A token that sees nothing gets zeros; what cache places beyond a sequence's length
+ * hold, and the keys and values a token does not see, does not matter, whatever their bits.
+ * Replaces dispatch_attention_decode / _prefill (moondream2.cpp:424-430): any number of new tokens
+ * per sequence, mixed in one call.  q and out of the cache's type, [n_tokens][q_heads * head_dim]
+ * at their tag's pitch; q_heads a multiple of kv_heads, at most 128 to a key head.  scale 0 means
+ * 1 / sqrt(head_dim).  fp32 scores, softmax and sums; the weights are rounded to the cache's type
+ * for the tensor cores.  Uses the device's scratch (run once before a graph capture). */
+mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* cache, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* out,
+                                 int q_heads, float scale, int causal, int window);
+
+/* ---------------------------------------------------------------- logit rules ------ */
+/* What is done to each row of logits before a token is chosen, in this order, in fp32:
+ *   history      ids the row's sequence holds, the prompt's first (int32 [rows][history_ld], the
+ *                first history_lens[r] of them, prompt_lens[r] of these the prompt's);
+ *                ids outside [0, n) are skipped
+ *   penalties    {repetition, frequency, presence} of each row (fp32 [rows][3]): a token in the
+ *                history has x > 0 ? x / repetition : x * repetition; one that is c > 0 times in
+ *                the history after the prompt loses frequency * c, then presence
+ *   bias         row r's entries bias_offsets[r] .. bias_offsets[r+1]-1 of bias_tokens /
+ *                bias_values: x += value (of entries with one token, the last one's)
+ *   allowed      bit t % 32 of word t / 32 of row r (uint32 [rows][(n + 31) / 32]) clear: x = -inf
+ * Each group may be NULL: history (with its lens and penalties), prompt_lens alone (no prompt),
+ * bias_* together, allowed. */
+typedef struct mgpu_logit_rules {
+    mgpu_buf* history;
+    mgpu_buf* history_lens; /* int32 [rows] */
+    mgpu_buf* prompt_lens;  /* int32 [rows] */
+    mgpu_buf* penalties;
+    mgpu_buf* bias_offsets; /* int32 [rows + 1] */
+    mgpu_buf* bias_tokens;  /* int32 */
+    mgpu_buf* bias_values;  /* fp32 */
+    mgpu_buf* allowed;
+    int history_ld;
+} mgpu_logit_rules;
+/* out = rules(logits) for `rows` rows of n logits (f32 / f16 / bf16, each buffer's rows at its
+ * tag's pitch, default n); out of logits' type, may be logits itself, or NULL.  best (>= 8 bytes a
+ * row, or NULL) receives each row's {int32 index, fp32 value} as mgpu_argmax_rows(out) would. */
+mgpu_event* mgpu_logits_process(const mgpu_device* dev, mgpu_buf* logits, mgpu_buf* out, int rows, int n,
+                                const mgpu_logit_rules* rules, mgpu_buf* best);
+
 /* ---------------------------------------------------------------- peer groups ----- */
 /* New (the reference runs on one device): small exchanges between the GPUs of one node over
  * NVLink, without a collective library, for the column-sharded lm_head of a batched decode

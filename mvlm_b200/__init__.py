@@ -85,6 +85,14 @@ SIGNATURES = {
     "mgpu_argmax_logits": (_i, [_vp, _vp, _i]),
     "mgpu_argmax_rows": (_vp, [_vp, _vp, _i, _i, _i64, _vp]),
     "mgpu_argmax_combine": (_vp, [_vp, _vp, _i, _i, _vp]),
+    "mgpu_kv_cache_create": (_vp, [_vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "mgpu_kv_cache_k": (_vp, [_vp]),
+    "mgpu_kv_cache_v": (_vp, [_vp]),
+    "mgpu_kv_cache_release": (None, [_vp]),
+    "mgpu_rope_table": (_vp, [_vp, _vp, _i, _i, _d]),
+    "mgpu_kv_append": (_vp, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "mgpu_paged_attention": (_vp, [_vp, _vp, _vp, _vp, _i, _f, _i, _i]),
+    "mgpu_logits_process": (_vp, [_vp, _vp, _vp, _i, _i, _vp, _vp]),
     "mgpu_peer_group_create": (_vp, [_vp, _i, _i, _sz]),
     "mgpu_peer_group_handle": (_i, [_vp, _vp]),
     "mgpu_peer_group_connect": (_i, [_vp, _vp]),
@@ -130,6 +138,24 @@ class GemvLink(ctypes.Structure):
     """mgpu_gemv_link: one GEMV of a chain (x may be a view of an earlier link's y)."""
     _fields_ = [("x", ctypes.c_void_p), ("W", ctypes.c_void_p), ("y", ctypes.c_void_p), ("N", ctypes.c_int),
                 ("K", ctypes.c_int)]
+
+
+class _PagedBatch(ctypes.Structure):
+    _fields_ = [("cu_q", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("n_seqs", ctypes.c_int), ("n_tokens", ctypes.c_int), ("max_q_len", ctypes.c_int),
+                ("max_pages", ctypes.c_int)]
+
+
+class _Rope(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("max_pos", ctypes.c_int),
+                ("rot_dim", ctypes.c_int), ("interleaved", ctypes.c_int), ("n_axes", ctypes.c_int),
+                ("sections", ctypes.c_int * 3)]
+
+
+class _LogitRules(ctypes.Structure):
+    _fields_ = [("history", ctypes.c_void_p), ("history_lens", ctypes.c_void_p), ("prompt_lens", ctypes.c_void_p),
+                ("penalties", ctypes.c_void_p), ("bias_offsets", ctypes.c_void_p), ("bias_tokens", ctypes.c_void_p),
+                ("bias_values", ctypes.c_void_p), ("allowed", ctypes.c_void_p), ("history_ld", ctypes.c_int)]
 
 
 _lib = None
@@ -503,6 +529,115 @@ def argmax_combine(dev: Device, pairs: Buffer, n_ranks: int, n_total: int, out: 
     """out (8 bytes) <- the global {index, value} from the ranks' gathered mgpu_argmax pairs of a
     row column-sharded over n_ranks GPUs (the reference's first maximum over the whole row)."""
     return _ev(lib().mgpu_argmax_combine(dev.h, pairs.h, n_ranks, n_total, out.h), "argmax_combine")
+
+
+class KVCache:
+    """mgpu_kv_cache: one layer's keys and values in pages, [num_pages][kv_heads][page_size][head_dim]
+    (F16 or BF16).  k, v: buffers to use (kept referenced here), or None to allocate them."""
+
+    def __init__(self, dev: Device, num_pages: int, page_size: int, kv_heads: int, head_dim: int, type_: int,
+                 k: Buffer | None = None, v: Buffer | None = None):
+        h = lib().mgpu_kv_cache_create(dev.h, num_pages, page_size, kv_heads, head_dim, type_, _h(k), _h(v))
+        if not h:
+            _raise_last("kv_cache_create")
+        self.dev, self.h, self.type, self._keep = dev, h, type_, (k, v)
+        self.num_pages, self.page_size, self.kv_heads, self.head_dim = num_pages, page_size, kv_heads, head_dim
+
+    def _side(self, handle) -> Buffer:
+        n = lib().mgpu_buf_bytes(handle)
+        v = lib().mgpu_buf_view(handle, 0, n)
+        if not v:
+            _raise_last("kv_cache view")
+        b = Buffer(self.dev, v, n)
+        b._cache = self  # the memory is the cache's
+        return b
+
+    @property
+    def k(self) -> Buffer:
+        return self._side(lib().mgpu_kv_cache_k(self.h))
+
+    @property
+    def v(self) -> Buffer:
+        return self._side(lib().mgpu_kv_cache_v(self.h))
+
+    def release(self):
+        if getattr(self, "h", None) and _lib is not None:
+            _lib.mgpu_kv_cache_release(self.h)
+        self.h = None
+
+    def __del__(self):
+        self.release()
+
+
+class PagedBatch:
+    """mgpu_paged_batch: the sequences of one step.  cu_q [n_seqs + 1], kv_lens [n_seqs] (new tokens
+    included) and page_table [n_seqs][max_pages] are int32 buffers, read by the kernels when they
+    run; their contents may change between calls, the counts are fixed here."""
+
+    def __init__(self, cu_q: Buffer, kv_lens: Buffer, page_table: Buffer, n_seqs: int, n_tokens: int, max_q_len: int,
+                 max_pages: int):
+        self._keep = (cu_q, kv_lens, page_table)
+        self.n_seqs, self.n_tokens, self.max_q_len, self.max_pages = n_seqs, n_tokens, max_q_len, max_pages
+        self.c = _PagedBatch(_h(cu_q), _h(kv_lens), _h(page_table), n_seqs, n_tokens, max_q_len, max_pages)
+        self.ref = ctypes.addressof(self.c)
+
+
+class Rope:
+    """mgpu_rope: the rotation of a head's first rot_dim dimensions by table[position][pair] (fp32
+    {cos, sin}, see rope_table).  positions: int32 [axes][n_tokens], or None for each token's index
+    in its sequence; sections: pairs of each axis (default: one axis)."""
+
+    def __init__(self, table: Buffer, max_pos: int, rot_dim: int, interleaved: bool = False, sections=None,
+                 positions: Buffer | None = None):
+        sections = [rot_dim // 2] if sections is None else [int(x) for x in sections]
+        if not 1 <= len(sections) <= 3:
+            raise MgpuError(ERR_INVALID_ARG, f"rope: {len(sections)} axes (1 to 3)")
+        self._keep = (table, positions)
+        self.c = _Rope(_h(table), _h(positions), max_pos, rot_dim, int(interleaved), len(sections),
+                       (ctypes.c_int * 3)(*sections))
+        self.ref = ctypes.addressof(self.c)
+
+
+def rope_table(dev: Device, max_pos: int, rot_dim: int, theta: float = 10000.0) -> Buffer:
+    """A new fp32 [max_pos][rot_dim / 2][2] buffer of {cos, sin}(p * theta^(-2i / rot_dim))."""
+    if max_pos <= 0 or rot_dim <= 0:
+        raise MgpuError(ERR_INVALID_ARG, f"rope_table: max_pos={max_pos} rot_dim={rot_dim}")
+    b = dev.empty(max_pos * rot_dim, F32)
+    _ev(lib().mgpu_rope_table(dev.h, b.h, max_pos, rot_dim, theta), "rope_table")
+    return b
+
+
+def kv_append(cache: KVCache, batch: PagedBatch, q: Buffer | None, k: Buffer, v: Buffer, q_out: Buffer | None,
+              q_heads: int, rope: Rope | None = None) -> Event:
+    """A step's keys (rotated) and values into the cache, its queries rotated into q_out."""
+    return _ev(lib().mgpu_kv_append(cache.h, batch.ref, _h(q), _h(k), _h(v), _h(q_out), q_heads,
+                                    rope.ref if rope is not None else None), "kv_append")
+
+
+def paged_attention(cache: KVCache, batch: PagedBatch, q: Buffer, out: Buffer, q_heads: int, scale: float = 0.0,
+                    causal: bool = True, window: int = 0) -> Event:
+    """out = softmax(scale * q . K) . V over what each token sees of its sequence in the cache."""
+    return _ev(lib().mgpu_paged_attention(cache.h, batch.ref, _h(q), _h(out), q_heads, scale, int(causal), window),
+               "paged_attention")
+
+
+class LogitRules:
+    """mgpu_logit_rules: penalties for tokens in a row's history, biases and a mask of allowed tokens
+    (each group may be left out)."""
+
+    def __init__(self, history: Buffer | None = None, history_lens: Buffer | None = None,
+                 prompt_lens: Buffer | None = None, history_ld: int = 0, penalties: Buffer | None = None,
+                 bias_offsets: Buffer | None = None, bias_tokens: Buffer | None = None,
+                 bias_values: Buffer | None = None, allowed: Buffer | None = None):
+        self._keep = (history, history_lens, prompt_lens, penalties, bias_offsets, bias_tokens, bias_values, allowed)
+        self.c = _LogitRules(*[_h(b) for b in self._keep], history_ld)
+        self.ref = ctypes.addressof(self.c)
+
+
+def logits_process(dev: Device, logits: Buffer, out: Buffer | None, rows: int, n: int, rules: LogitRules,
+                   best: Buffer | None = None) -> Event:
+    """out = rules(logits), and / or best = its rows' {int32 index, fp32 value} first maxima."""
+    return _ev(lib().mgpu_logits_process(dev.h, _h(logits), _h(out), rows, n, rules.ref, _h(best)), "logits_process")
 
 
 class PeerGroup:

@@ -18,8 +18,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmgpu.so")
-SOURCES = ["runtime.cu", "gemv.cu", "chain.cu", "gemm_tc.cu", "skinny.cu", "misc.cu", "peer.cu"]
-HEADERS = ["common.cuh", "kernels.h", "qdot.cuh"]
+SOURCES = ["runtime.cu", "gemv.cu", "chain.cu", "gemm_tc.cu", "skinny.cu", "misc.cu", "peer.cu", "cache.cu",
+           "attention.cu", "logits.cu"]
+HEADERS = ["common.cuh", "kernels.h", "qdot.cuh", "paged.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",

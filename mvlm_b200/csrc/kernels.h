@@ -99,6 +99,60 @@ cudaError_t argmax_combine(const LaunchCtx& c, const int* pairs, int n_ranks, in
 cudaError_t im2col(const LaunchCtx& c, int type, const void* img, void* patches, int C, int H, int W, int ph,
                    int pw, int kpad);
 
+// ------------------------------------------------- paged cache (cache.cu, attention.cu) --
+// A step's sequences (device arrays; the kernels check their contents against the counts and
+// record MGPU_ERR_INVALID_ARG in the status word for what does not fit).
+struct PagedBatch {
+    const int* cu_q;        // [n_seqs + 1]
+    const int* kv_lens;     // [n_seqs]
+    const int* page_table;  // [n_seqs][max_pages]
+    int n_seqs, n_tokens, max_q_len, max_pages;
+};
+// table[p][i] = {cos, sin}(p * theta^(-2i / rot)), i < rot / 2.
+cudaError_t rope_table(const LaunchCtx& c, float* table, int max_pos, int rot, double theta);
+struct AppendArgs {
+    const void *q, *k, *v;  // q null: no queries
+    void *qo, *kc, *vc;
+    int qt, kt, vt, qot, ctype;
+    int64_t ldq, ldk, ldv, ldqo;
+    int hq, hkv, D, num_pages, page_size;
+    PagedBatch batch;
+    const float* table;  // null (with rot = 0): no rotation
+    const int* positions;
+    int max_pos, rot, interleaved, n_axes;
+    int end0, end1;  // first pair of the second and of the third axis
+    int* status;
+};
+cudaError_t kv_append(const LaunchCtx& c, const AppendArgs& a);
+struct AttendArgs {
+    const void *q, *kc, *vc;
+    void* out;
+    int64_t ldq, ldo;
+    int type, hq, hkv, D, num_pages, page_size;
+    PagedBatch batch;
+    float scale;
+    int causal, window;
+    int* status;
+};
+cudaError_t paged_attention(const LaunchCtx& c, const AttendArgs& a);
+
+// ------------------------------------------------------------- logit rules (logits.cu) --
+struct RulesArgs {
+    const void* x;
+    void* out;  // may be x, or null
+    int* best;  // may be null
+    int64_t ldx, ldo;
+    int type, rows, n;
+    const int *history, *history_lens, *prompt_lens;
+    int history_ld;
+    const float* penalties;
+    const int *bias_offsets, *bias_tokens;
+    const float* bias_values;
+    int bias_entries;
+    const uint32_t* allowed;
+};
+cudaError_t logits_process(const LaunchCtx& c, const RulesArgs& a);
+
 // ---------------------------------------------------------------- GEMM (gemm_tc.cu) --
 struct GemmOperand {
     const void* ptr;

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -183,7 +184,10 @@ bool check_status(mgpu_device* d) {
     if (!cuda_ok(cudaMemcpy(&st, d->d_status, sizeof(int), cudaMemcpyDeviceToHost), "read status")) return false;
     if (st != 0) {
         cudaMemsetAsync(d->d_status, 0, sizeof(int), d->stream);
-        set_error(st, "a kernel's bounded wait expired (device status %d); its output is invalid", st);
+        if (st == MGPU_ERR_INVALID_ARG)
+            set_error(st, "a kernel skipped sequences whose lengths, pages or positions do not fit their buffers");
+        else
+            set_error(st, "a kernel's bounded wait expired (device status %d); its output is invalid", st);
         return false;
     }
     return true;
@@ -1004,6 +1008,329 @@ void mgpu_gemv_chain_destroy(mgpu_gemv_chain* c) {
     DeviceGuard g(c->dev->ordinal);
     cudaStreamSynchronize(c->dev->stream);
     free_chain(c);
+}
+
+// ------------------------------------------------------------------ paged cache ------
+struct mgpu_kv_cache {
+    mgpu_device* dev;
+    mgpu_buf* k;
+    mgpu_buf* v;
+    int num_pages, page_size, kv_heads, head_dim, type;
+};
+
+namespace {
+
+constexpr int kMaxHeadDim = 128;
+constexpr int kMaxGroup = 128;  // query heads of one key head: one tile's rows
+
+bool aligned_to(const mgpu_buf* b, size_t n) { return ((uintptr_t)b->ptr % n) == 0; }
+
+// An int32 array of n entries (tags do not matter).
+bool holds_ints(const mgpu_buf* b, int64_t n) { return b && b->bytes / 4 >= (size_t)n && aligned_to(b, 4); }
+
+// Rows x width of a float type at the buffer's pitch; the error is set when they do not fit.
+bool rows_ok(const mgpu_buf* b, int64_t rows, int64_t width, const char* who, const char* what, int64_t* ld) {
+    *ld = ld_or(b, width);
+    if (!is_float_type(b->type)) {
+        set_error(MGPU_ERR_INVALID_ARG, "%s: %s must be f32 / f16 / bf16", who, what);
+        return false;
+    }
+    const size_t es = elem_size(b->type);
+    if (*ld < width || b->bytes / es < (size_t)(rows - 1) * *ld + width || !aligned_to(b, es)) {
+        set_error(MGPU_ERR_INVALID_ARG, "%s: %s does not hold %lld rows of %lld values (pitch %lld)", who, what,
+                  (long long)rows, (long long)width, (long long)*ld);
+        return false;
+    }
+    return true;
+}
+
+bool batch_ok(const mgpu_paged_batch* b, const char* who, mgpu_k::PagedBatch* out) {
+    if (!b || b->n_seqs <= 0 || b->n_tokens <= 0 || b->max_q_len <= 0 || b->max_pages <= 0) {
+        set_error(MGPU_ERR_INVALID_ARG, "%s: null batch or counts below 1", who);
+        return false;
+    }
+    if (!holds_ints(b->cu_q, (int64_t)b->n_seqs + 1) || !holds_ints(b->kv_lens, b->n_seqs) ||
+        !holds_ints(b->page_table, (int64_t)b->n_seqs * b->max_pages)) {
+        set_error(MGPU_ERR_INVALID_ARG, "%s: cu_q, kv_lens or page_table smaller than its n_seqs=%d / max_pages=%d", who,
+                  b->n_seqs, b->max_pages);
+        return false;
+    }
+    *out = mgpu_k::PagedBatch{(const int*)b->cu_q->ptr, (const int*)b->kv_lens->ptr, (const int*)b->page_table->ptr,
+                              b->n_seqs, b->n_tokens, b->max_q_len, b->max_pages};
+    return true;
+}
+
+Range rows_range(const mgpu_buf* b, int64_t rows, int64_t width, int64_t ld) {
+    return range_of(b, ((size_t)(rows - 1) * ld + width) * elem_size(b->type));
+}
+
+}  // namespace
+
+mgpu_kv_cache* mgpu_kv_cache_create(const mgpu_device* cd, int num_pages, int page_size, int kv_heads, int head_dim,
+                                    int type, mgpu_buf* k, mgpu_buf* v) {
+    API_ENTRY();
+    REQUIRE(cd, "kv_cache_create: null device");
+    REQUIRE(num_pages > 0 && kv_heads > 0, "kv_cache_create: num_pages=%d kv_heads=%d", num_pages, kv_heads);
+    REQUIRE(page_size > 0 && page_size % 8 == 0, "kv_cache_create: page_size=%d must be a multiple of 8", page_size);
+    REQUIRE(head_dim > 0 && head_dim % 8 == 0, "kv_cache_create: head_dim=%d must be a multiple of 8", head_dim);
+    REQUIRE(type == MGPU_F16 || type == MGPU_BF16, "kv_cache_create: type must be f16 or bf16");
+    REQUIRE((k == nullptr) == (v == nullptr), "kv_cache_create: both of k and v, or neither");
+    if (head_dim > kMaxHeadDim) {
+        set_error(MGPU_ERR_UNSUPPORTED, "kv_cache_create: head_dim=%d is above %d", head_dim, kMaxHeadDim);
+        return nullptr;
+    }
+    // rows of pages x heads are one coordinate of the tensor maps
+    REQUIRE((int64_t)num_pages * kv_heads <= INT32_MAX && (int64_t)page_size * head_dim <= INT32_MAX,
+            "kv_cache_create: num_pages x kv_heads or page_size x head_dim above 2^31");
+    const size_t bytes = (size_t)num_pages * kv_heads * page_size * head_dim * 2;
+    mgpu_device* d = const_cast<mgpu_device*>(cd);
+    if (k) {
+        REQUIRE(k->bytes >= bytes && v->bytes >= bytes, "kv_cache_create: k or v holds fewer than %zu bytes", bytes);
+        REQUIRE(aligned_to(k, 16) && aligned_to(v, 16), "kv_cache_create: k and v must be 16-byte aligned");
+        const Range rk = range_of(k, bytes), rv = range_of(v, bytes);
+        REQUIRE(!rk.overlaps(rv), "kv_cache_create: k and v overlap");
+    }
+    DeviceGuard g(d->ordinal);
+    mgpu_kv_cache* c = new mgpu_kv_cache{d, nullptr, nullptr, num_pages, page_size, kv_heads, head_dim, type};
+    c->k = k ? new_buf(d, k->ptr, bytes, false) : mgpu_create_buffer(d, bytes, nullptr);
+    c->v = v ? new_buf(d, v->ptr, bytes, false) : mgpu_create_buffer(d, bytes, nullptr);
+    if (!c->k || !c->v ||
+        (!k && (!cuda_ok(cudaMemsetAsync(c->k->ptr, 0, bytes, d->stream), "kv_cache_create: clear") ||
+                !cuda_ok(cudaMemsetAsync(c->v->ptr, 0, bytes, d->stream), "kv_cache_create: clear")))) {
+        mgpu_kv_cache_release(c);
+        return nullptr;
+    }
+    c->k->type = c->v->type = type;
+    return c;
+}
+
+mgpu_buf* mgpu_kv_cache_k(const mgpu_kv_cache* c) { return c ? c->k : nullptr; }
+mgpu_buf* mgpu_kv_cache_v(const mgpu_kv_cache* c) { return c ? c->v : nullptr; }
+
+void mgpu_kv_cache_release(mgpu_kv_cache* c) {
+    if (!c) return;
+    mgpu_release_buffer(c->k);
+    mgpu_release_buffer(c->v);
+    delete c;
+}
+
+mgpu_event* mgpu_rope_table(const mgpu_device* cd, mgpu_buf* table, int max_pos, int rot_dim, double theta) {
+    API_ENTRY();
+    REQUIRE(cd && table, "rope_table: null argument");
+    REQUIRE(max_pos > 0 && rot_dim > 0 && rot_dim % 2 == 0, "rope_table: max_pos=%d rot_dim=%d", max_pos, rot_dim);
+    REQUIRE(theta > 0.0, "rope_table: theta=%g must be positive", theta);
+    REQUIRE(table->bytes / 4 >= (size_t)max_pos * rot_dim && aligned_to(table, 8),
+            "rope_table: table must hold max_pos x rot_dim fp32 values, 8-byte aligned");
+    mgpu_device* d = const_cast<mgpu_device*>(cd);
+    DeviceGuard g(d->ordinal);
+    mgpu_event* ev = event_begin(d);
+    if (!cuda_ok(mgpu_k::rope_table(ctx_of(d), (float*)table->ptr, max_pos, rot_dim, theta), "rope_table")) {
+        if (ev) d->event_pool.push_back(ev);
+        return nullptr;
+    }
+    return event_end(d, ev);
+}
+
+mgpu_event* mgpu_kv_append(const mgpu_kv_cache* c, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* k, mgpu_buf* v,
+                           mgpu_buf* q_out, int q_heads, const mgpu_rope* rope) {
+    API_ENTRY();
+    REQUIRE(c && k && v, "kv_append: null argument");
+    REQUIRE((q == nullptr) == (q_out == nullptr), "kv_append: both of q and q_out, or neither");
+    mgpu_k::AppendArgs a = {};
+    if (!batch_ok(batch, "kv_append", &a.batch)) return nullptr;
+    const int64_t rows = batch->n_tokens, kw = (int64_t)c->kv_heads * c->head_dim;
+    if (!rows_ok(k, rows, kw, "kv_append", "k", &a.ldk) || !rows_ok(v, rows, kw, "kv_append", "v", &a.ldv)) return nullptr;
+    const size_t bytes = c->k->bytes;
+    Range caches[2] = {range_of(c->k, bytes), range_of(c->v, bytes)};
+    if (q) {
+        REQUIRE(q_heads > 0, "kv_append: q_heads=%d", q_heads);
+        const int64_t qw = (int64_t)q_heads * c->head_dim;
+        if (!rows_ok(q, rows, qw, "kv_append", "q", &a.ldq) || !rows_ok(q_out, rows, qw, "kv_append", "q_out", &a.ldqo))
+            return nullptr;
+        const Range out = rows_range(q_out, rows, qw, a.ldqo);
+        // interleaved rows (views into one projection) share a range without sharing a value: only
+        // q_out's own rows are checked against them, as whole views
+        if (q_out->ptr == q->ptr)
+            REQUIRE(q_out->type == q->type && a.ldqo == a.ldq, "kv_append: q_out in place must have q's type and pitch");
+        else
+            REQUIRE(!out.overlaps(rows_range(q, rows, qw, a.ldq)), "kv_append: q_out overlaps q without being q");
+        for (const Range& r : caches) REQUIRE(!out.overlaps(r), "kv_append: q_out overlaps the cache");
+        if (q_out->ptr != q->ptr)
+            REQUIRE(!out.overlaps(rows_range(k, rows, kw, a.ldk)) && !out.overlaps(rows_range(v, rows, kw, a.ldv)),
+                    "kv_append: q_out overlaps k or v");
+        a.q = q->ptr;
+        a.qo = q_out->ptr;
+        a.qt = q->type;
+        a.qot = q_out->type;
+        a.hq = q_heads;
+    }
+    for (const Range& r : caches)
+        REQUIRE(!r.overlaps(rows_range(k, rows, kw, a.ldk)) && !r.overlaps(rows_range(v, rows, kw, a.ldv)) &&
+                    (!q || !r.overlaps(rows_range(q, rows, (int64_t)q_heads * c->head_dim, a.ldq))),
+                "kv_append: q, k or v overlaps the cache");
+    if (rope) {
+        REQUIRE(rope->rot_dim > 0 && rope->rot_dim % 2 == 0 && rope->rot_dim <= c->head_dim,
+                "kv_append: rot_dim=%d of head_dim=%d", rope->rot_dim, c->head_dim);
+        REQUIRE(rope->max_pos > 0 && rope->table && aligned_to(rope->table, 8) &&
+                    rope->table->bytes / 4 >= (size_t)rope->max_pos * rope->rot_dim,
+                "kv_append: the rope table must hold max_pos=%d x rot_dim=%d fp32 values", rope->max_pos, rope->rot_dim);
+        REQUIRE(rope->n_axes >= 1 && rope->n_axes <= 3, "kv_append: %d rope axes (1 to 3)", rope->n_axes);
+        int64_t sum = 0;
+        for (int i = 0; i < rope->n_axes; ++i) {
+            REQUIRE(rope->sections[i] >= 0, "kv_append: rope section %d is negative", i);
+            sum += rope->sections[i];
+        }
+        REQUIRE(sum == rope->rot_dim / 2, "kv_append: rope sections sum to %lld of %d pairs", (long long)sum,
+                rope->rot_dim / 2);
+        if (rope->positions)
+            REQUIRE(holds_ints(rope->positions, (int64_t)rope->n_axes * rows), "kv_append: positions holds fewer than %d x %lld",
+                    rope->n_axes, (long long)rows);
+        a.table = (const float*)rope->table->ptr;
+        a.positions = rope->positions ? (const int*)rope->positions->ptr : nullptr;
+        a.max_pos = rope->max_pos;
+        a.rot = rope->rot_dim;
+        a.interleaved = rope->interleaved != 0;
+        a.n_axes = rope->n_axes;
+        a.end0 = rope->sections[0];
+        a.end1 = a.end0 + (rope->n_axes > 1 ? rope->sections[1] : 0);
+    }
+    mgpu_device* d = c->dev;
+    DeviceGuard g(d->ordinal);
+    a.k = k->ptr;
+    a.v = v->ptr;
+    a.kc = c->k->ptr;
+    a.vc = c->v->ptr;
+    a.kt = k->type;
+    a.vt = v->type;
+    a.ctype = c->type;
+    a.hkv = c->kv_heads;
+    a.D = c->head_dim;
+    a.num_pages = c->num_pages;
+    a.page_size = c->page_size;
+    a.status = d->d_status;
+    mgpu_event* ev = event_begin(d);
+    if (!cuda_ok(mgpu_k::kv_append(ctx_of(d), a), "kv_append")) {
+        if (ev) d->event_pool.push_back(ev);
+        return nullptr;
+    }
+    return event_end(d, ev);
+}
+
+mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* out,
+                                 int q_heads, float scale, int causal, int window) {
+    API_ENTRY();
+    REQUIRE(c && q && out, "paged_attention: null argument");
+    mgpu_k::AttendArgs a = {};
+    if (!batch_ok(batch, "paged_attention", &a.batch)) return nullptr;
+    REQUIRE(q_heads > 0 && q_heads % c->kv_heads == 0, "paged_attention: q_heads=%d is no multiple of kv_heads=%d", q_heads,
+            c->kv_heads);
+    if (q_heads / c->kv_heads > kMaxGroup) {
+        set_error(MGPU_ERR_UNSUPPORTED, "paged_attention: %d query heads to a key head (at most %d)", q_heads / c->kv_heads,
+                  kMaxGroup);
+        return nullptr;
+    }
+    REQUIRE(q->type == c->type && out->type == c->type, "paged_attention: q and out must have the cache's type");
+    REQUIRE(window >= 0, "paged_attention: window=%d", window);
+    REQUIRE(scale >= 0.0f && scale < INFINITY, "paged_attention: scale=%g", (double)scale);
+    const int64_t rows = batch->n_tokens, width = (int64_t)q_heads * c->head_dim;
+    if (!rows_ok(q, rows, width, "paged_attention", "q", &a.ldq) ||
+        !rows_ok(out, rows, width, "paged_attention", "out", &a.ldo))
+        return nullptr;
+    const Range ro = rows_range(out, rows, width, a.ldo);
+    REQUIRE(!ro.overlaps(rows_range(q, rows, width, a.ldq)), "paged_attention: out overlaps q");
+    REQUIRE(!ro.overlaps(range_of(c->k, c->k->bytes)) && !ro.overlaps(range_of(c->v, c->v->bytes)),
+            "paged_attention: out overlaps the cache");
+    mgpu_device* d = c->dev;
+    DeviceGuard g(d->ordinal);
+    a.q = q->ptr;
+    a.out = out->ptr;
+    a.kc = c->k->ptr;
+    a.vc = c->v->ptr;
+    a.type = c->type;
+    a.hq = q_heads;
+    a.hkv = c->kv_heads;
+    a.D = c->head_dim;
+    a.num_pages = c->num_pages;
+    a.page_size = c->page_size;
+    a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim);
+    a.causal = causal != 0;
+    a.window = window;
+    a.status = d->d_status;
+    mgpu_event* ev = event_begin(d);
+    if (!cuda_ok(mgpu_k::paged_attention(ctx_of(d), a), "paged_attention")) {
+        if (ev) d->event_pool.push_back(ev);
+        return nullptr;
+    }
+    return event_end(d, ev);
+}
+
+// ------------------------------------------------------------------ logit rules ------
+mgpu_event* mgpu_logits_process(const mgpu_device* cd, mgpu_buf* logits, mgpu_buf* out, int rows, int n,
+                                const mgpu_logit_rules* r, mgpu_buf* best) {
+    API_ENTRY();
+    REQUIRE(cd && logits && r, "logits_process: null argument");
+    REQUIRE(out || best, "logits_process: neither out nor best");
+    REQUIRE(rows > 0 && n > 0, "logits_process: rows=%d n=%d", rows, n);
+    REQUIRE((int64_t)rows * 8 <= INT32_MAX && n <= (1 << 30), "logits_process: rows=%d or n=%d too large", rows, n);
+    mgpu_k::RulesArgs a = {};
+    if (!rows_ok(logits, rows, n, "logits_process", "logits", &a.ldx)) return nullptr;
+    if (out) {
+        if (!rows_ok(out, rows, n, "logits_process", "out", &a.ldo)) return nullptr;
+        REQUIRE(out->type == logits->type, "logits_process: out must have the logits' type");
+        if (out->ptr == logits->ptr)
+            REQUIRE(a.ldo == a.ldx, "logits_process: in place needs one pitch");
+        else
+            REQUIRE(!rows_range(out, rows, n, a.ldo).overlaps(rows_range(logits, rows, n, a.ldx)),
+                    "logits_process: out overlaps logits without being logits");
+        a.out = out->ptr;
+    }
+    if (best) {
+        REQUIRE(best->bytes >= (size_t)rows * 8 && aligned_to(best, 4), "logits_process: best needs 8 bytes per row");
+        a.best = (int*)best->ptr;
+    }
+    if (r->history) {
+        REQUIRE(r->history_ld > 0 && holds_ints(r->history, (int64_t)rows * r->history_ld),
+                "logits_process: history holds fewer than %d x history_ld=%d ids", rows, r->history_ld);
+        REQUIRE(holds_ints(r->history_lens, rows), "logits_process: history without %d history_lens", rows);
+        REQUIRE(!r->prompt_lens || holds_ints(r->prompt_lens, rows), "logits_process: prompt_lens holds fewer than %d", rows);
+        REQUIRE(holds_ints(r->penalties, (int64_t)rows * 3), "logits_process: penalties must hold %d x 3 fp32 values", rows);
+        a.history = (const int*)r->history->ptr;
+        a.history_lens = (const int*)r->history_lens->ptr;
+        a.prompt_lens = r->prompt_lens ? (const int*)r->prompt_lens->ptr : nullptr;
+        a.history_ld = r->history_ld;
+        a.penalties = (const float*)r->penalties->ptr;
+    } else {
+        REQUIRE(!r->history_lens && !r->prompt_lens && !r->penalties, "logits_process: lens or penalties without a history");
+    }
+    if (r->bias_offsets) {
+        REQUIRE(holds_ints(r->bias_offsets, (int64_t)rows + 1), "logits_process: bias_offsets holds fewer than %d", rows + 1);
+        REQUIRE(holds_ints(r->bias_tokens, 1) && holds_ints(r->bias_values, 1), "logits_process: bias_offsets without "
+                "bias_tokens and bias_values");
+        const size_t entries = std::min(r->bias_tokens->bytes, r->bias_values->bytes) / 4;
+        a.bias_offsets = (const int*)r->bias_offsets->ptr;
+        a.bias_tokens = (const int*)r->bias_tokens->ptr;
+        a.bias_values = (const float*)r->bias_values->ptr;
+        a.bias_entries = (int)std::min<size_t>(entries, INT32_MAX);
+    } else {
+        REQUIRE(!r->bias_tokens && !r->bias_values, "logits_process: biases without bias_offsets");
+    }
+    if (r->allowed) {
+        REQUIRE(holds_ints(r->allowed, (int64_t)rows * ((n + 31) / 32)), "logits_process: allowed holds fewer than %d x %d "
+                "words", rows, (n + 31) / 32);
+        a.allowed = (const uint32_t*)r->allowed->ptr;
+    }
+    a.x = logits->ptr;
+    a.type = logits->type;
+    a.rows = rows;
+    a.n = n;
+    mgpu_device* d = const_cast<mgpu_device*>(cd);
+    DeviceGuard g(d->ordinal);
+    mgpu_event* ev = event_begin(d);
+    if (!cuda_ok(mgpu_k::logits_process(ctx_of(d), a), "logits_process")) {
+        if (ev) d->event_pool.push_back(ev);
+        return nullptr;
+    }
+    return event_end(d, ev);
 }
 
 mgpu_event* mgpu_dispatch_patch_embed(const mgpu_device* cd, mgpu_program, mgpu_buf* image, mgpu_buf* proj_weight,

@@ -130,11 +130,19 @@ struct AttendArgs {
     int64_t ldq, ldo;
     int type, hq, hkv, D, num_pages, page_size;
     PagedBatch batch;
-    float scale;
+    float scale_log2;  // scale * log2(e)
     int causal, window;
     int* status;
+    float* partials;        // attend_scratch_bytes
+    unsigned int* tickets;  // one per CTA, zero between calls (the kernel leaves them so)
+    // set by paged_attention
+    int box_rows, max_rows, q_pairs, out_pairs;
 };
-cudaError_t paged_attention(const LaunchCtx& c, const AttendArgs& a);
+size_t attend_scratch_bytes(int sm_count);
+// The TMA map of one side of a cache: [num_pages * kv_heads][page_size][head_dim], boxes of 64
+// dims x the most rows that divide both a page and a block of keys.
+bool make_cache_map(CUtensorMap* m, const void* side, int type, int num_pages, int page_size, int kv_heads, int head_dim);
+cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const AttendArgs& a);
 
 // ------------------------------------------------------------- logit rules (logits.cu) --
 struct RulesArgs {
@@ -184,10 +192,10 @@ cudaError_t gemm(const LaunchCtx& c, const GemmOperand& A, const GemmOperand& B,
 bool skinny_ok(const GemmOperand& A, const GemmOperand& B, int M, int N, int K);
 cudaError_t gemm_q4_skinny(const LaunchCtx& c, const GemmOperand& A, const GemmOperand& B, const GemmOperand& C,
                            const void* bias, int bias_type, int M, int N, int K, const Epilogue& epi = Epilogue());
-// A 3-D TMA map over 16-bit units without swizzle: extents dims[0] (contiguous), dims[1],
+// A 3-D TMA map over 16-bit units, without swizzle or with the 128-byte one: extents dims[0] (contiguous), dims[1],
 // dims[2]; byte strides of dims 1 and 2 (multiples of 16, in any order); box {box[0..2]}.
 bool make_tensor_map_u16_3d(CUtensorMap* m, const void* ptr, const int64_t dims[3], const int64_t strides[2],
-                            const int box[3]);
+                            const int box[3], bool swizzle128 = false);
 // Exchange over peer memory (peer.cu): this GPU's `bytes` (from src, or src + p * src_stride
 // for peer p) into slot `rank` of every peer's receive region, then one flag per peer, then a
 // bounded wait for every peer's flag of this exchange.

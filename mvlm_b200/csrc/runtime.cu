@@ -105,14 +105,16 @@ bool is_float_type(int t) { return t == MGPU_F32 || t == MGPU_F16 || t == MGPU_B
 bool is_quant_type(int t) { return t == MGPU_Q4_0 || t == MGPU_Q8_0; }
 size_t quant_row_bytes(int t, int64_t k) { return (size_t)((k + 31) / 32) * (t == MGPU_Q4_0 ? 18 : 34); }
 
-// Scratch arena layout: [0, 64 KB) holds the split-K tickets of gemv_kn and [64 KB, 128 KB)
-// those of the split-K GEMM; both must stay zero between launches (the kernels reset them).
+// Scratch arena layout: [0, 64 KB) holds the split-K tickets of gemv_kn, [64 KB, 128 KB) those of
+// the split-K GEMM and [128 KB, 132 KB) those of the paged attention's shares (one per CTA of a
+// one-wave grid); all must stay zero between launches (the kernels reset them).
 // Everything from kScratchOffset on is free for per-call use (split-K partials, im2col
 // patches, staged operands), in stream order.
 constexpr size_t kGemvTicketBytes = 64 * 1024;
 constexpr size_t kGemmTicketOffset = 64 * 1024;
 constexpr size_t kGemmTicketBytes = 64 * 1024;
-constexpr size_t kScratchOffset = 128 * 1024;
+constexpr size_t kAttendTicketOffset = 128 * 1024;
+constexpr size_t kScratchOffset = 132 * 1024;
 
 mgpu_k::LaunchCtx ctx_of(const mgpu_device* d) {
     mgpu_k::LaunchCtx c;
@@ -1016,6 +1018,7 @@ struct mgpu_kv_cache {
     mgpu_buf* k;
     mgpu_buf* v;
     int num_pages, page_size, kv_heads, head_dim, type;
+    CUtensorMap map_k, map_v;
 };
 
 namespace {
@@ -1091,7 +1094,7 @@ mgpu_kv_cache* mgpu_kv_cache_create(const mgpu_device* cd, int num_pages, int pa
         REQUIRE(!rk.overlaps(rv), "kv_cache_create: k and v overlap");
     }
     DeviceGuard g(d->ordinal);
-    mgpu_kv_cache* c = new mgpu_kv_cache{d, nullptr, nullptr, num_pages, page_size, kv_heads, head_dim, type};
+    mgpu_kv_cache* c = new mgpu_kv_cache{d, nullptr, nullptr, num_pages, page_size, kv_heads, head_dim, type, {}, {}};
     c->k = k ? new_buf(d, k->ptr, bytes, false) : mgpu_create_buffer(d, bytes, nullptr);
     c->v = v ? new_buf(d, v->ptr, bytes, false) : mgpu_create_buffer(d, bytes, nullptr);
     if (!c->k || !c->v ||
@@ -1101,6 +1104,12 @@ mgpu_kv_cache* mgpu_kv_cache_create(const mgpu_device* cd, int num_pages, int pa
         return nullptr;
     }
     c->k->type = c->v->type = type;
+    if (!mgpu_k::make_cache_map(&c->map_k, c->k->ptr, type, num_pages, page_size, kv_heads, head_dim) ||
+        !mgpu_k::make_cache_map(&c->map_v, c->v->ptr, type, num_pages, page_size, kv_heads, head_dim)) {
+        set_error(MGPU_ERR_CUDA, "kv_cache_create: tensor map");
+        mgpu_kv_cache_release(c);
+        return nullptr;
+    }
     return c;
 }
 
@@ -1252,12 +1261,15 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch*
     a.D = c->head_dim;
     a.num_pages = c->num_pages;
     a.page_size = c->page_size;
-    a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)c->head_dim);
+    a.scale_log2 = (float)((scale > 0.0f ? (double)scale : 1.0 / sqrt((double)c->head_dim)) * 1.4426950408889634);
     a.causal = causal != 0;
     a.window = window;
     a.status = d->d_status;
+    if (!ensure_workspace(d, kScratchOffset + mgpu_k::attend_scratch_bytes(d->sm_count))) return nullptr;
+    a.tickets = (unsigned int*)((char*)d->workspace + kAttendTicketOffset);
+    a.partials = (float*)((char*)d->workspace + kScratchOffset);
     mgpu_event* ev = event_begin(d);
-    if (!cuda_ok(mgpu_k::paged_attention(ctx_of(d), a), "paged_attention")) {
+    if (!cuda_ok(mgpu_k::paged_attention(ctx_of(d), c->map_k, c->map_v, a), "paged_attention")) {
         if (ev) d->event_pool.push_back(ev);
         return nullptr;
     }

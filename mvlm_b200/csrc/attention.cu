@@ -65,12 +65,16 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4
 // cut into equal shares, one per CTA, whatever the sequences' lengths; an item cut by a share's end
 // is joined by the last of its CTAs to finish.  One warp feeds a ring of blocks by TMA; eight warps
 // in two groups take every other block, a warp 16 of its keys, each with its own running state.
-constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 1);
+constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 2);
 constexpr int kRowsMax = 16;
 constexpr int kSeqCap = 1024;  // sequences whose block counts are kept in shared memory
 
 template <int DP> constexpr int rows_stage_bytes() { return 2 * kBlock * DP * 2; }
-template <int DP> constexpr int rows_stages() { return 160 * 1024 / rows_stage_bytes<DP>(); }
+// 128 KB in flight, some three times what HBM's latency at full rate asks of an SM.  An even number,
+// so that a stage always belongs to one group of warps: a wait on the parity of a barrier's phase
+// must not be able to meet the phase before the last one, which a group two blocks ahead of the
+// other could when they shared a stage.
+template <int DP> constexpr int rows_stages() { return 128 * 1024 / rows_stage_bytes<DP>(); }
 template <int DP> constexpr int rows_pitch() { return DP + 4; }
 template <int DP> constexpr int rows_smem() {
     return 1024 + rows_stages<DP>() * rows_stage_bytes<DP>() + 4 * kRowsMax * rows_pitch<DP>() * 4;
@@ -100,25 +104,32 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     constexpr int S = rows_stages<DP>(), SB = rows_stage_bytes<DP>(), PITCH = rows_pitch<DP>();
     constexpr int SLABS = DP / 64, SLAB = kBlock * 128;  // 64 dims x 64 keys, 128-byte rows, swizzled
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
+    static_assert(S % 2 == 0, "a stage belongs to one group of warps");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float* scratch = reinterpret_cast<float*>(ring + S * SB);
     __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S];
     __shared__ int counts[kSeqCap];
-    __shared__ long long warp_sum[kRowsWarps + 1];
-    __shared__ long long start_before;
-    __shared__ int start_seq, is_last;
+    __shared__ long long warp_sum[kRowsWarps + 2];
+    __shared__ bool last;
+    __shared__ int start_before;
+    __shared__ int start_seq;
     __shared__ float sm_m[kRowsWarps][kRowsMax], sm_l[kRowsWarps][kRowsMax];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.hq / a.hkv;
 
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(&full_bar[s], 1);
+            mbar_init(&full_bar[s], 2);
             mbar_init(&empty_bar[s], kRowsWarps / 2);
         }
         fence_mbar_init();
+        prefetch_tensormap(&tmK);
+        prefetch_tensormap(&tmV);
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
+    // the step's contents and the cache may be the preceding kernel's
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- this CTA's share of all blocks
     auto count = [&](int b) {
         bool bad = false;
@@ -136,23 +147,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
-    long long total = 0;
-    for (int w = 0; w <= kRowsWarps; ++w) total += warp_sum[w];
-    total *= a.hkv;
-    const long long shares = min((long long)gridDim.x, total);  // none is empty
-    if (blockIdx.x >= shares) return;
-    auto share = [&](long long c) { return c * total / shares; };
-    const long long begin = share(blockIdx.x), end = share((long long)blockIdx.x + 1);
+    long long sum_all = 0;
+    for (int x = 0; x < kRowsWarps + 2; ++x) sum_all += warp_sum[x];
+    const int total = (int)(sum_all * a.hkv);  // the host has bounded it
+    const int shares = min((int)gridDim.x, total);  // none is empty
+    if ((int)blockIdx.x >= shares) return;
+    const int quota = total / shares, more = total % shares;  // the first `more` shares have one block more
+    auto share = [&](int c) { return c * quota + min(c, more); };
+    const int begin = share(blockIdx.x), end = share(blockIdx.x + 1);
     if (warp == 0) {
         // the sequence that holds block `begin`, and the blocks of the sequences before it
-        long long before = 0;
+        int before = 0;
         for (int b0 = 0; b0 < a.batch.n_seqs; b0 += 32) {
             const int b = b0 + lane;
-            const long long n = b < a.batch.n_seqs ? (long long)(b < kSeqCap ? counts[b] : count(b)) * a.hkv : 0;
-            long long incl = n;
+            const int n = b < a.batch.n_seqs ? (b < kSeqCap ? counts[b] : count(b)) * a.hkv : 0;
+            int incl = n;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, incl, off);
+                const int v = __shfl_up_sync(0xffffffffu, incl, off);
                 if (lane >= off) incl += v;
             }
             const unsigned past = __ballot_sync(0xffffffffu, before + incl > begin);
@@ -182,44 +194,46 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     };
     Walk w;
     enter(w, start_seq);
-    w.h = (int)((begin - start_before) / w.blocks);
-    w.k = (int)((begin - start_before) % w.blocks);
+    w.h = (begin - start_before) / w.blocks;
+    w.k = (begin - start_before) % w.blocks;
 
-    if (warp == kRowsWarps) {
+    if (warp >= kRowsWarps) {
         // ---------------------------------------------------------------- loads
-        const int rows = a.box_rows, chunks = kBlock / rows;  // a chunk of a block lies in one page
-        const int loads = chunks * SLABS * 2;
-        uint32_t it = 0;
-        for (long long pos = begin; pos < end;) {
-            const int k1 = (int)min((long long)w.blocks, w.k + (end - pos));
-            pos += k1 - w.k;
-            const int base = first_block(a, w.s);
-            for (int k = w.k; k < k1; ++k, ++it) {
-                const uint32_t st = it % S;
-                if (!__all_sync(0xffffffffu, mbar_wait(&empty_bar[st], ((it / S) & 1u) ^ 1u, a.status))) return;
-                uint8_t* dst = ring + st * SB;
-                if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB);
-                __syncwarp();
-                for (int i = lane; i < loads; i += 32) {
-                    const int c = i % chunks, slab = (i / chunks) % SLABS, side = i / (chunks * SLABS);
-                    const int j = (base + k) * kBlock + c * rows;
-                    // chunks past the end are read from outside the map: zeros
-                    int z = a.num_pages * a.hkv, y = 0;
-                    if (j < w.s.kv) {
-                        const int page = a.batch.page_table[(int64_t)w.b * a.batch.max_pages + j / a.page_size];
-                        if (page >= 0 && page < a.num_pages) {
-                            z = page * a.hkv + w.h;
-                            y = j % a.page_size;
-                        } else {
-                            atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-                        }
-                    }
-                    tma_load_3d(dst + side * (SB / 2) + slab * SLAB + c * rows * 128, side ? &tmV : &tmK, slab * 64, y, z,
-                                &full_bar[st]);
+        // one warp for the keys, one for the values; a lane loads one chunk (rows of one page) of a slab
+        const int rows = a.box_rows, chunks = kBlock / rows, side = warp - kRowsWarps;
+        const bool loads = lane < chunks * SLABS;
+        const int first = (lane % chunks) * rows, slab = lane / chunks;
+        const CUtensorMap* map = side ? &tmV : &tmK;
+        int base = first_block(a, w.s);
+        // the page of this lane's chunk of block k, asked for one block ahead; chunks past the end are
+        // read from outside the map, which gives zeros
+        auto key = [&] { return (base + w.k) * kBlock + first; };
+        auto page_of = [&](int j) {
+            if (!loads || j >= w.s.kv) return -2;
+            return __ldg(a.batch.page_table + (int64_t)w.b * a.batch.max_pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size));
+        };
+        int j = key(), page = page_of(j);
+        for (int pos = begin, it = 0; pos < end; ++pos, ++it) {
+            const uint32_t st = it % S;
+            if (!__all_sync(0xffffffffu, mbar_wait(&empty_bar[st], ((it / S) & 1u) ^ 1u, a.status))) return;
+            if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB / 2);
+            __syncwarp();
+            if (loads) {
+                const bool in = page >= 0 && page < a.num_pages;
+                if (!in && page != -2) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                const int z = in ? page * a.hkv + w.h : a.num_pages * a.hkv;
+                const int y = in ? (a.page_shift >= 0 ? j & ((1 << a.page_shift) - 1) : j % a.page_size) : 0;
+                tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);
+            }
+            if (++w.k == w.blocks && pos + 1 < end) {
+                w.k = 0;
+                if (++w.h == a.hkv) {
+                    enter(w, w.b + 1);
+                    base = first_block(a, w.s);
                 }
             }
-            w.k = 0;
-            if (++w.h == a.hkv && pos < end) enter(w, w.b + 1);
+            j = key();
+            if (pos + 1 < end) page = page_of(j);
         }
         return;
     }
@@ -229,8 +243,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const int g = lane >> 2, c2 = 2 * (lane & 3);  // this thread's rows g and g + 8, and first column
     bool dead = false;  // a wait ran out: walk on without data, so that every barrier is still met
     uint32_t it = 0;
-    for (long long pos = begin; pos < end;) {
-        const int k0 = w.k, k1 = (int)min((long long)w.blocks, k0 + (end - pos));
+    for (int pos = begin; pos < end;) {
+        const int k0 = w.k, k1 = min(w.blocks, k0 + (end - pos));
         const int base = first_block(a, w.s), R = w.s.n * G;
         // queries: A fragments of every 16 dims
         uint32_t qf[DP / 16][4];
@@ -437,7 +451,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         };
         // pieces of CTA c: slot 2c for the item its share begins in, 2c + 1 for a later one
         constexpr int PIECE = kRowsMax * (DP + 2);
-        const long long item_begin = pos - k0;
+        const int item_begin = pos - k0;
         float* piece = a.partials + (2 * (int64_t)blockIdx.x + (item_begin > begin ? 1 : 0)) * PIECE;
         for (int e = tid; e < R * (DP / 2); e += 32 * kRowsWarps) {
             const int r = e / (DP / 2), d = 2 * (e % (DP / 2));
@@ -465,44 +479,77 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
         if (!complete) {
             // CTAs c0 .. c1 have the item's blocks; the last of them to arrive joins their pieces in order
-            auto owner = [&](long long x) {  // the CTA whose share holds block x
-                long long c = x * shares / total;
-                while (share(c) > x) --c;
-                while (share(c + 1) <= x) ++c;
-                return (int)c;
-            };
-            const int c0 = owner(item_begin), c1 = owner(item_begin + w.blocks - 1);
+            const int cut = more * (quota + 1);
+            auto owner = [&](int x) { return x < cut ? x / (quota + 1) : more + (x - cut) / quota; };
+            const int c0 = owner(item_begin), c1 = owner(item_begin + w.blocks - 1), pieces = c1 - c0 + 1;
             __threadfence();
             named_barrier_sync(1, 32 * kRowsWarps);
             if (tid == 0) {
-                is_last = atomicAdd(&a.tickets[c0], 1u) == (unsigned)(c1 - c0);
-                if (is_last) a.tickets[c0] = 0;
+                last = atomicAdd(&a.tickets[c0], 1u) == (unsigned)(pieces - 1);
+                if (last) a.tickets[c0] = 0;
             }
             named_barrier_sync(1, 32 * kRowsWarps);
-            if (is_last) {
+            if (last) {
                 __threadfence();
-                for (int e = tid; e < R * (DP / 2); e += 32 * kRowsWarps) {
+                auto piece_of = [&](int i) {
+                    return a.partials + (2 * (int64_t)(c0 + i) + (i == 0 && item_begin > share(c0) ? 1 : 0)) * PIECE;
+                };
+                // Every thread sums a pair of a row's values over some of the pieces; with few values the
+                // threads take turns at the pieces, and their sums are added in order.
+                const int values = R * (DP / 2);
+                int turns = 1;
+                while (2 * turns * values <= 32 * kRowsWarps) turns *= 2;
+                for (int e0 = 0; e0 < values; e0 += 32 * kRowsWarps / turns) {
+                    const int e = e0 + tid % (32 * kRowsWarps / turns), turn = tid / (32 * kRowsWarps / turns);
                     const int r = e / (DP / 2), d = 2 * (e % (DP / 2));
-                    if (d >= a.D) continue;
+                    const bool mine_too = e < values && d < a.D;
                     float top = -INFINITY, den = 0.0f;
                     float2 v = make_float2(0.0f, 0.0f);
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* p = a.partials + (2 * (int64_t)c + (c == c0 && item_begin > share(c0) ? 1 : 0)) * PIECE;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + kRowsMax * DP + 2 * r));
-                        const float2 x = __ldcg(reinterpret_cast<const float2*>(p + r * DP + d));
-                        if (ml.x == -INFINITY) {  // saw nothing; what Inf or NaN it added stays
-                            v.x += x.x;
-                            v.y += x.y;
-                            continue;
+                    if (mine_too) {
+                        for (int i = 0; i < pieces; i += 8) {
+                            float t[8];
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)
+                                t[x] = i + x < pieces ? __ldcg(piece_of(i + x) + kRowsMax * DP + 2 * r) : -INFINITY;
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) top = fmaxf(top, t[x]);
                         }
-                        const float mn = fmaxf(top, ml.x), f0 = ex2(top - mn), f1 = ex2(ml.x - mn);
-                        v.x = v.x * f0 + x.x * f1;
-                        v.y = v.y * f0 + x.y * f1;
-                        den = den * f0 + ml.y * f1;
-                        top = mn;
+                        const float mu = top == -INFINITY ? 0.0f : top;
+                        for (int i = turn; i < pieces; i += 8 * turns) {
+                            float2 ml[8], o2[8];
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                const bool has = i + x * turns < pieces;
+                                const float* p = piece_of(has ? i + x * turns : 0);
+                                ml[x] = has ? __ldcg(reinterpret_cast<const float2*>(p + kRowsMax * DP + 2 * r)) : make_float2(-INFINITY, 0.0f);
+                                o2[x] = has ? __ldcg(reinterpret_cast<const float2*>(p + r * DP + d)) : make_float2(0.0f, 0.0f);
+                            }
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                const float f = ex2(ml[x].x - mu);
+                                v.x += o2[x].x * f;
+                                v.y += o2[x].y * f;
+                                den += ml[x].y * f;
+                            }
+                        }
                     }
-                    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-                    write(r, d, v.x * inv, v.y * inv);
+                    if (turns > 1) {
+                        scratch[3 * tid] = v.x;
+                        scratch[3 * tid + 1] = v.y;
+                        scratch[3 * tid + 2] = den;
+                        named_barrier_sync(1, 32 * kRowsWarps);
+                        if (turn == 0)
+                            for (int x = 1; x < turns; ++x) {
+                                const float* o = scratch + 3 * (tid + x * (32 * kRowsWarps / turns));
+                                v.x += o[0];
+                                v.y += o[1];
+                                den += o[2];
+                            }
+                    }
+                    if (mine_too && turn == 0) {
+                        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+                        write(r, d, v.x * inv, v.y * inv);
+                    }
                 }
             }
         }
@@ -533,8 +580,17 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
     static std::atomic<uint64_t> configured{0};
     const cudaError_t e = allow_smem(kern, rows_smem<DP>(), configured);
     if (e != cudaSuccess) return e;
-    kern<<<(unsigned)c.sm_count, kRowsThreads, rows_smem<DP>(), c.stream>>>(mk, mv, a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)c.sm_count);
+    cfg.blockDim = dim3(kRowsThreads);
+    cfg.dynamicSmemBytes = rows_smem<DP>();
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, mk, mv, a);
 }
 
 // One warp per (token, query head): one pass over the visible keys with a running maximum and sum.
@@ -614,6 +670,9 @@ cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUt
     a.box_rows = kBlock;
     while (a.page_size % a.box_rows) a.box_rows /= 2;
     a.max_rows = kRowsMax;
+    a.page_shift = -1;
+    for (int i = 3; i < 31; ++i)
+        if (a.page_size == 1 << i) a.page_shift = i;
     a.q_pairs = ((uintptr_t)a.q & 3) == 0 && a.ldq % 2 == 0;
     a.out_pairs = ((uintptr_t)a.out & 3) == 0 && a.ldo % 2 == 0;
     return a.type == MGPU_F16 ? launch_attend<__half>(c, mk, mv, a) : launch_attend<__nv_bfloat16>(c, mk, mv, a);

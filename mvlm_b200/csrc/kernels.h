@@ -136,7 +136,7 @@ struct AttendArgs {
     float* partials;        // attend_scratch_bytes
     unsigned int* tickets;  // one per CTA, zero between calls (the kernel leaves them so)
     // set by paged_attention
-    int box_rows, max_rows, q_pairs, out_pairs;
+    int box_rows, page_shift, max_rows, q_pairs, out_pairs;
 };
 size_t attend_scratch_bytes(int sm_count);
 // The TMA map of one side of a cache: [num_pages * kv_heads][page_size][head_dim], boxes of 64

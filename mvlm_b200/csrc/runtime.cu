@@ -1249,6 +1249,12 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch*
     REQUIRE(!ro.overlaps(rows_range(q, rows, width, a.ldq)), "paged_attention: out overlaps q");
     REQUIRE(!ro.overlaps(range_of(c->k, c->k->bytes)) && !ro.overlaps(range_of(c->v, c->v->bytes)),
             "paged_attention: out overlaps the cache");
+    // the kernels count blocks of 64 keys, and tiles of rows, in 32 bits
+    if (((int64_t)batch->max_pages * c->page_size / 64 + 2) * batch->n_seqs * c->kv_heads > INT32_MAX ||
+        (int64_t)batch->max_pages * c->page_size > INT32_MAX || rows * q_heads > INT32_MAX) {
+        set_error(MGPU_ERR_UNSUPPORTED, "paged_attention: more than 2^31 blocks of keys or rows of queries");
+        return nullptr;
+    }
     mgpu_device* d = c->dev;
     DeviceGuard g(d->ordinal);
     a.q = q->ptr;

@@ -9,6 +9,8 @@
 // The rows of one key head - its G query heads times the sequence's new tokens - share every key
 // they load.  Rows are ordered token-major: row r is token r / G, head r % G of the group.
 #include <atomic>
+#include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -36,7 +38,12 @@ __device__ __forceinline__ bool odd16(uint32_t h, bool bf16) {
     const uint32_t e = bf16 ? 0x7F80u : 0x7C00u;
     return (h & e) == e;
 }
-__device__ __forceinline__ float ex2(float x) { return exp2f(x); }
+// 2^x: the hardware's approximation, some 2^-22 off, zero for results below 2^-126.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // ------------------------------------------------------------------ tensor cores ----
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -593,68 +600,698 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
     return cudaLaunchKernelEx(&cfg, kern, mk, mv, a);
 }
 
-// One warp per (token, query head): one pass over the visible keys with a running maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(128) attend_kernel(const mgpu_k::AttendArgs a) {
-    const int lane = threadIdx.x & 31, h = blockIdx.y * 4 + (threadIdx.x >> 5), t = blockIdx.x;
-    if (h >= a.hq) return;
-    const int seq = seq_of_token(a.batch, t);
-    if (seq < 0) return;
-    bool bad = false;
-    const SeqView s = seq_view(a.batch, seq, a.page_size, &bad);
-    if (bad) {
-        if (lane == 0) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-        return;
-    }
-    if ((long long)s.n * (a.hq / a.hkv) <= kRowsMax) return;
-    const int p = s.kv - s.n + (t - s.q0), kvh = h / (a.hq / a.hkv);
-    const int end = a.causal ? min(p + 1, s.kv) : s.kv;
-    const int begin = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)t * a.ldq + (int64_t)h * a.D;
-    float qv[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+// ------------------------------------------------------------------ many rows -------
+// More than 16 rows to a key head (a chunk of a prompt): bound by the tensor cores' two products,
+// 4 D operations to a row and key, and by one exponential to a row and key.  A CTA takes two tiles of
+// up to 128 rows (whole tokens: 128 / G of them) over the same blocks of 128 keys.  One thread issues
+// S_t = Q_t K^T and O_t += P_t V of both tiles in turn, so that one tile's products run while the
+// other's softmax does; scores, weights and O stay in TMEM, weights in the place of the scores.  Each
+// tile has four warps, a thread to a row, which needs no exchange for its maximum and sum.  O is
+// rescaled only when a row's maximum has grown by more than 2^8 since its reference was taken: weights
+// stay below 2^8, and most blocks then leave O alone.  All blocks of all items (sequence, key head,
+// pair of tiles) are cut into equal shares as above; where whole items are few and short, a CTA takes
+// one item instead, which saves the join.
+constexpr int kTileKeys = 128, kTileRows = 128;
+constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, and two that look over V
+constexpr int kTileSeqs = 1024;    // sequences of one launch
+constexpr int kTileEntries = 2048; // entries of the table of items
+constexpr int kJoinBlocks = 6;     // what a join costs, in blocks
+constexpr float kGrowth = 8.0f;    // log2 of how far a weight may exceed 1
+
+template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
+// K on even and V on odd stages: two blocks of 128 dims, four of 64
+template <int DP> constexpr int tile_stages() { return 128 * 1024 / tile_stage_bytes<DP>(); }
+template <int DP> constexpr int tile_smem() {
+    return 1024 + 2 * kTileRows * DP * 2 + tile_stages<DP>() * tile_stage_bytes<DP>() + 4 * (kTileSeqs + 1 + kTileEntries + 1);
+}
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// 32 columns of this thread's TMEM lane; valid after tmem_ld_wait and tmem_use.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Keeps uses of the loaded registers behind the wait.
+template <int N = 32> __device__ __forceinline__ void tmem_use(uint32_t* r) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qv[i] = lane + 32 * i < a.D ? to_f32<T>(q[lane + 32 * i]) : 0.0f;
-    for (int j = begin; j < end; ++j) {
-        const int page = a.batch.page_table[(int64_t)seq * a.batch.max_pages + j / a.page_size];
-        if (page < 0 || page >= a.num_pages) {
-            if (lane == 0) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-            return;
+    for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two tiles of one sequence's tokens.  Blocks are counted from the sequence's start.
+struct Pair {
+    SeqView s;
+    int lo, blocks;              // the blocks that either tile needs: [lo, lo + blocks)
+    int first[2], rows[2];       // a tile's first token and its rows (0: no tile)
+    int t_lo[2], t_hi[2];        // its blocks
+    int whole_lo[2], whole_hi[2];  // the keys that all its rows see
+    __device__ __forceinline__ bool in(int t, int kb) const { return kb >= t_lo[t] && kb < t_hi[t]; }
+    __device__ __forceinline__ bool whole(int t, int kb) const {
+        return kb * kTileKeys >= whole_lo[t] && (kb + 1) * kTileKeys <= whole_hi[t];
+    }
+    // some row of a tile that takes the block does not see all of it
+    __device__ __forceinline__ bool masked(int kb) const { return (in(0, kb) && !whole(0, kb)) || (in(1, kb) && !whole(1, kb)); }
+};
+__device__ __forceinline__ Pair pair_of(const mgpu_k::AttendArgs& a, const SeqView& s, int j, int per_tile) {
+    Pair p;
+    p.s = s;
+    const int G = a.hq / a.hkv;
+    int lo = INT_MAX, hi = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = (2 * j + t) * per_tile, n = min(max(s.n - first, 0), per_tile);
+        p.first[t] = first;
+        p.rows[t] = n * G;
+        p.t_lo[t] = p.t_hi[t] = p.whole_lo[t] = p.whole_hi[t] = 0;
+        if (n == 0) continue;
+        const Seen a0 = seen_by(a, s, first), a1 = seen_by(a, s, first + n - 1);
+        p.whole_lo[t] = a1.lo;
+        p.whole_hi[t] = a0.hi;
+        if (a1.hi <= a0.lo) continue;
+        p.t_lo[t] = a0.lo / kTileKeys;
+        p.t_hi[t] = (a1.hi + kTileKeys - 1) / kTileKeys;
+        lo = min(lo, p.t_lo[t]);
+        hi = max(hi, p.t_hi[t]);
+    }
+    // a pair that sees nothing has one block, which no tile takes, so that its rows are written
+    p.lo = hi > 0 ? lo : 0;
+    p.blocks = max(1, hi - p.lo);
+    return p;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    attend_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                       const mgpu_k::AttendArgs a, int seq0) {
+    constexpr int SLABS = DP / 64, QB = kTileRows * DP * 2, SB = tile_stage_bytes<DP>(), SLAB = kTileKeys * 128;
+    constexpr int S = tile_stages<DP>();
+    constexpr bool kBf16 = !std::is_same<T, __half>::value;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* ring = qs + 2 * QB;
+    int* seq_first = reinterpret_cast<int*>(ring + S * SB);  // [n + 1] pairs before a sequence
+    int* cum = seq_first + kTileSeqs + 1;                    // [entries + 1] blocks before an entry
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], q_bar[2], s_bar[2], p_bar[2], o_bar[2], clean_bar[S], drain_bar;
+    __shared__ uint32_t tmem_slot;
+    __shared__ int odd_at[4];  // 1 + the segment in whose masked blocks of V NaN or Inf was found
+    __shared__ int warp_part[kTileThreads / 32], start[3];
+    __shared__ bool last[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = a.hq / a.hkv, per_tile = kTileRows / G;
+
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&full_bar[i], 1);
+            mbar_init(&empty_bar[i], 1);
+            mbar_init(&clean_bar[i], 2);  // V: the two warps that look it over
         }
-        const int64_t row = (((int64_t)page * a.hkv + kvh) * a.page_size + j % a.page_size) * a.D;
-        float x = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < a.D) x += qv[i] * to_f32<T>(reinterpret_cast<const T*>(a.kc)[row + lane + 32 * i]);
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-        x *= a.scale_log2;
-        const float mn = fmaxf(m, x), r = exp2f(m - mn), w = exp2f(x - mn);
-        m = mn;
-        l = l * r + w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < a.D) o[i] = o[i] * r + w * to_f32<T>(reinterpret_cast<const T*>(a.vc)[row + lane + 32 * i]);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_bar[t], 4);
+            mbar_init(&s_bar[t], 1);
+            mbar_init(&p_bar[t], 4);
+            mbar_init(&o_bar[t], 1);
+        }
+        mbar_init(&drain_bar, 1);
+        fence_mbar_init();
+        prefetch_tensormap(&tmK);
+        prefetch_tensormap(&tmV);
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
-    T* out = reinterpret_cast<T*>(a.out) + (int64_t)t * a.ldo + (int64_t)h * a.D;
+    if (tid < 4) odd_at[tid] = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // ---- the table of items: pairs before each sequence, blocks before each run of pairs
+    const int seqs = min(a.batch.n_seqs - seq0, kTileSeqs);
+    auto view = [&](int b) {
+        bool bad = false;
+        SeqView s = seq_view(a.batch, seq0 + b, a.page_size, &bad);
+        if (bad) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+        if ((long long)s.n * G <= a.max_rows) s.n = 0;  // the rows kernel's
+        return s;
+    };
+    // exclusive prefix sums of v[0 .. n) in place, the total at v[n]
+    auto scan = [&](int* v, int n) {
+        const int each = (n + kTileThreads - 1) / kTileThreads, i0 = min(n, tid * each), i1 = min(n, i0 + each);
+        int sum = 0;
+        for (int i = i0; i < i1; ++i) sum += v[i];
+        int incl = sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 32 * i < a.D) out[lane + 32 * i] = from_f32<T>(end > begin ? o[i] / l : 0.0f);
+        for (int off = 1; off < 32; off <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, incl, off);
+            if (lane >= off) incl += x;
+        }
+        if (lane == 31) warp_part[warp] = incl;
+        __syncthreads();
+        int before = incl - sum;
+        for (int w = 0; w < warp; ++w) before += warp_part[w];
+        for (int i = i0; i < i1; ++i) {
+            const int x = v[i];
+            v[i] = before;
+            before += x;
+        }
+        if (tid == kTileThreads - 1) v[n] = before;
+        __syncthreads();
+    };
+    for (int b = tid; b < seqs; b += kTileThreads) seq_first[b] = (view(b).n + 2 * per_tile - 1) / (2 * per_tile);
+    __syncthreads();
+    scan(seq_first, seqs);
+    const int pairs = seq_first[seqs];
+    if (pairs == 0) return;
+    auto seq_of_pair = [&](int p) {  // the last b with seq_first[b] <= p
+        int lo2 = 0, hi2 = seqs;
+        while (hi2 - lo2 > 1) {
+            const int mid = (lo2 + hi2) / 2;
+            if (seq_first[mid] <= p) lo2 = mid;
+            else hi2 = mid;
+        }
+        return lo2;
+    };
+    const int run = (pairs + kTileEntries - 1) / kTileEntries, entries = (pairs + run - 1) / run;
+    int most = 0;
+    for (int e = tid; e < entries; e += kTileThreads) {
+        int sum = 0, b = seq_of_pair(e * run);
+        SeqView s = view(b);
+        for (int p = e * run; p < min(pairs, (e + 1) * run); ++p) {
+            while (seq_first[b + 1] <= p) s = view(++b);
+            const int n = pair_of(a, s, p - seq_first[b], per_tile).blocks;
+            sum += n;
+            most = max(most, n);
+        }
+        cum[e] = sum;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    __syncthreads();
+    scan(cum, entries);
+    if (lane == 0) warp_part[warp] = most;
+    __syncthreads();
+    for (int w = 0; w < kTileThreads / 32; ++w) most = max(most, warp_part[w]);
+    const int head_blocks = cum[entries], total = head_blocks * a.hkv, items = pairs * a.hkv;
+    // whole items, one to a CTA, unless cutting them saves more than a join costs
+    const bool by_item = items <= (int)gridDim.x && most <= (total + (int)gridDim.x - 1) / (int)gridDim.x + kJoinBlocks;
+    const int shares = by_item ? items : min((int)gridDim.x, total);
+    if ((int)blockIdx.x >= shares) return;
+    const int quota = total / shares, more = total % shares;
+    auto share = [&](int c) { return c * quota + min(c, more); };
+    if (tid == 0) {
+        int h, p, k = 0;
+        if (by_item) {
+            h = blockIdx.x / pairs;
+            p = blockIdx.x % pairs;
+        } else {
+            const int x = share(blockIdx.x);
+            h = x / head_blocks;
+            int y = x % head_blocks, lo2 = 0, hi2 = entries;
+            while (hi2 - lo2 > 1) {
+                const int mid = (lo2 + hi2) / 2;
+                if (cum[mid] <= y) lo2 = mid;
+                else hi2 = mid;
+            }
+            y -= cum[lo2];
+            for (p = lo2 * run;; ++p) {
+                const int b = seq_of_pair(p), n = pair_of(a, view(b), p - seq_first[b], per_tile).blocks;
+                if (y < n) break;
+                y -= n;
+            }
+            k = y;
+        }
+        start[0] = h;
+        start[1] = p;
+        start[2] = k;
+    }
+    if (warp == 8) {
+        tmem_alloc(&tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const int begin = by_item ? 0 : share(blockIdx.x);
+    int end = by_item ? 0 : share(blockIdx.x + 1);  // by_item: set below
+    int h = start[0], p = start[1], k = start[2], b = seq_of_pair(p);
+    Pair pr = pair_of(a, view(b), p - seq_first[b], per_tile);
+    if (by_item) end = pr.blocks;
+    auto next_item = [&] {
+        k = 0;
+        if (++p == pairs) {
+            p = 0;
+            ++h;
+            b = 0;
+        }
+        while (seq_first[b + 1] <= p) ++b;
+        pr = pair_of(a, view(b), p - seq_first[b], per_tile);
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        bool ok = true;
+        if (warp == 8) {
+            // ------------------------------------------------------------ products
+            if (lane == 0) {
+                const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys);
+                const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
+                const int dims = (a.D + 15) / 16;
+                uint32_t n = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};  // n: blocks so far
+                auto product_s = [&](int t, uint32_t stage) {
+                    const uint32_t qa = smem_u32(qs) + t * QB, kb = smem_u32(ring) + stage * SB;
+                    for (int d = 0; d < dims; ++d) {
+                        const uint32_t off = (d >> 2) * SLAB + (d & 3) * 32;  // Q and K have the same slabs
+                        umma_f16(tmem + t * kTileKeys, smem_desc(qa + off, 16, 1024, kSwizzle128B),
+                                 smem_desc(kb + off, 16, 1024, kSwizzle128B), id_s, d != 0);
+                    }
+                    umma_commit(&s_bar[t]);
+                };
+                for (int pos = begin; ok && pos < end;) {
+                    const int k1 = min(pr.blocks, k + (end - pos));
+                    bool started[2] = {false, false};  // the tile has its Q, and O its first product
+                    bool has_o[2] = {false, false};
+                    auto score = [&](int t, int kb, uint32_t stage) {
+                        if (!started[t]) {
+                            ok = ok && mbar_wait(&q_bar[t], q_phase[t]++ & 1u, a.status);
+                            started[t] = true;
+                        }
+                        if (ok) product_s(t, stage);
+                    };
+                    for (int i = k; ok && i < k1; ++i, ++n) {
+                        const int kb = pr.lo + i;
+                        const uint32_t ks = (2 * n) % S, vs = (2 * n + 1) % S, kn = (2 * n + 2) % S;
+                        if (i == k) {
+                            ok = mbar_wait(&full_bar[ks], (2 * n / S) & 1u, a.status);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int t = 0; t < 2; ++t)
+                                if (pr.in(t, kb)) score(t, kb, ks);
+                            umma_commit(&empty_bar[ks]);
+                        }
+                        ok = ok && mbar_wait(&full_bar[vs], ((2 * n + 1) / S) & 1u, a.status);
+                        ok = ok && mbar_wait(&clean_bar[vs], ((2 * n + 1) / S) & 1u, a.status);
+                        bool have_next = false;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            if (!ok) break;
+                            if (pr.in(t, kb)) {
+                                ok = mbar_wait(&p_bar[t], p_phase[t]++ & 1u, a.status);
+                                if (!ok) break;
+                                tc_fence_after();
+                                const uint32_t vb = smem_u32(ring) + vs * SB;
+                                for (int d = 0; d < kTileKeys / 16; ++d)
+                                    umma_f16_ts(tmem + 256 + t * 128, tmem + t * kTileKeys + d * 8,
+                                                smem_desc(vb + d * 2048, SLAB, 1024, kSwizzle128B), id_o, has_o[t] || d != 0);
+                                has_o[t] = true;
+                                if (i + 1 == k1 || !pr.in(t, kb + 1)) umma_commit(&o_bar[t]);
+                            }
+                            if (i + 1 < k1 && pr.in(t, kb + 1)) {
+                                if (!have_next) ok = mbar_wait(&full_bar[kn], ((2 * n + 2) / S) & 1u, a.status);
+                                if (!ok) break;
+                                have_next = true;
+                                tc_fence_after();
+                                score(t, kb + 1, kn);
+                            }
+                        }
+                        if (!ok) break;
+                        umma_commit(&empty_bar[vs]);
+                        if (i + 1 < k1) {
+                            // a block that no tile takes still has to arrive before its stage is given back
+                            if (!have_next) ok = mbar_wait(&full_bar[kn], ((2 * n + 2) / S) & 1u, a.status);
+                            umma_commit(&empty_bar[kn]);
+                        }
+                    }
+                    pos += k1 - k;
+                    if (pos < end) next_item();
+                }
+                umma_commit(&drain_bar);  // all products have ended before TMEM is given back
+                mbar_wait(&drain_bar, 0, a.status);
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ loads
+            const int rows = a.box_rows, chunks = kTileKeys / rows;
+            const bool loads = lane < chunks;
+            uint32_t it = 0;
+            for (int pos = begin; ok && pos < end;) {
+                const int k1 = min(pr.blocks, k + (end - pos));
+                for (int i = k; ok && i < k1; ++i) {
+                    const int j = (pr.lo + i) * kTileKeys + lane * rows;
+                    int z = a.num_pages * a.hkv, y = 0;
+                    if (loads && j < pr.s.kv) {
+                        const int at = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+                        const int page = __ldg(a.batch.page_table + (int64_t)(seq0 + b) * a.batch.max_pages + at);
+                        if (page >= 0 && page < a.num_pages) {
+                            z = page * a.hkv + h;
+                            y = j - at * a.page_size;
+                        } else {
+                            atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                        }
+                    }
+#pragma unroll
+                    for (int side = 0; side < 2; ++side, ++it) {
+                        const uint32_t st = it % S;
+                        ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[st], ((it / S) & 1u) ^ 1u, a.status));
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB);
+                        __syncwarp();
+                        if (loads)
+                            for (int slab = 0; slab < SLABS; ++slab)
+                                tma_load_3d(ring + st * SB + slab * SLAB + lane * rows * 128, side ? &tmV : &tmK, slab * 64, y, z,
+                                            &full_bar[st]);
+                    }
+                }
+                pos += k1 - k;
+                if (pos < end) next_item();
+            }
+        } else {
+            // ------------------------------------------------------------ NaN and Inf in V
+            // A weight of 0 times NaN or Inf is not 0: where some row does not see all keys of a block,
+            // such values leave the block, and the rows that see them add them at the end.
+            uint32_t n = 0;
+            int seg = 0;
+            for (int pos = begin; ok && pos < end; ++seg) {
+                const int k1 = min(pr.blocks, k + (end - pos));
+                for (int i = k; ok && i < k1; ++i, ++n) {
+                    const uint32_t st = (2 * n + 1) % S;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[st], ((2 * n + 1) / S) & 1u, a.status));
+                    if (!ok) break;
+                    if (pr.masked(pr.lo + i)) {
+                        uint4* v = reinterpret_cast<uint4*>(ring + st * SB);
+                        bool found = false;
+                        for (int x = (warp - 10) * 32 + lane; x < SB / 16; x += 64) {
+                            const uint4 q = v[x];
+                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                            bool any = false;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) any |= odd16(w[e], kBf16) || odd16(w[e] >> 16, kBf16);
+                            if (any) {
+                                uint16_t* u = reinterpret_cast<uint16_t*>(v + x);
+                                for (int e = 0; e < 8; ++e)
+                                    if (odd16(u[e], kBf16)) u[e] = 0;
+                                found = true;
+                            }
+                        }
+                        if (found) *reinterpret_cast<volatile int*>(&odd_at[seg & 3]) = seg + 1;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive(&clean_bar[st]);
+                }
+                pos += k1 - k;
+                if (pos < end) next_item();
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax: a thread to a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int t = warp >> 2, row = tid & 127, bar = 1 + t;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of TMEM
+        const uint32_t s_tm = tmem + t * kTileKeys + lanes, o_tm = tmem + 256 + t * 128 + lanes;
+        bool dead = false;
+        auto mine = [&](const int (&v)[2]) { return t ? v[1] : v[0]; };  // no indexing: the pair stays in registers
+        // this warp's 32 rows of Q into the swizzled slabs, zeros beyond the tile's rows and the head's dims
+        auto stage_q = [&] {
+            constexpr int PER = DP / 8;  // 16-byte chunks of a row
+            uint8_t* dst = qs + t * QB;
+            for (int x = lane; x < 32 * PER; x += 32) {
+                const int r = (warp & 3) * 32 + x / PER, c = x % PER;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < mine(pr.rows) && c * 8 < a.D) {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(pr.s.q0 + mine(pr.first) + r / G) * a.ldq +
+                                        (int64_t)(h * G + r % G) * a.D + c * 8;
+                    if (a.q_vec) {
+                        v = *reinterpret_cast<const uint4*>(q);
+                    } else {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)q[2 * e] | ((uint32_t)q[2 * e + 1] << 16);
+                        v = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * SLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_bar[t]);
+        };
+        uint32_t s_phase = 0, o_phase = 0;
+        int seg = 0;
+        // does the tile take any block of [k, k1) of the item?
+        auto takes = [&](int k0, int k1) { return max(mine(pr.t_lo), pr.lo + k0) < min(mine(pr.t_hi), pr.lo + k1); };
+        if (takes(k, min(pr.blocks, k + (end - begin)))) stage_q();
+        for (int pos = begin; pos < end; ++seg) {
+            const int k0 = k, k1 = min(pr.blocks, k + (end - pos));
+            const int kb0 = max(mine(pr.t_lo), pr.lo + k0), kb1 = min(mine(pr.t_hi), pr.lo + k1);
+            const int whole_lo = mine(pr.whole_lo), whole_hi = mine(pr.whole_hi), rows = mine(pr.rows), blocks = pr.blocks;
+            const int64_t token = (int64_t)pr.s.q0 + mine(pr.first) + row / G;
+            const bool valid = row < rows;
+            const Seen sr = valid ? seen_by(a, pr.s, mine(pr.first) + row / G) : Seen{0, 0};
+            float m = -INFINITY, l = 0.0f;  // the reference (log2 units) and the sum of 2^(s - m)
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&s_bar[t], s_phase++ & 1u, a.status));
+                if (dead) break;
+                tc_fence_after();
+                uint32_t s[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(s_tm + 32 * c, s + 32 * c);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_use(s + 32 * c);
+                if (kb * kTileKeys < whole_lo || (kb + 1) * kTileKeys > whole_hi) {
+                    const int c0 = sr.lo - kb * kTileKeys, c1 = sr.hi - kb * kTileKeys;
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c < c0 || c >= c1) s[c] = 0xFF800000u;
+                }
+                float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 128; c += 4) {
+                    x0 = fmaxf(x0, __uint_as_float(s[c]));
+                    x1 = fmaxf(x1, __uint_as_float(s[c + 1]));
+                    x2 = fmaxf(x2, __uint_as_float(s[c + 2]));
+                    x3 = fmaxf(x3, __uint_as_float(s[c + 3]));
+                }
+                const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2;
+                const bool grown = top > m + kGrowth;
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float f = grown ? ex2(m - top) : 1.0f;
+                    if (grown) m = top;
+                    l *= f;
+                    // this tile's product before this block's scores has ended: its scores were issued after it
+                    if (kb > kb0) {
+#pragma unroll 1
+                        for (int c = 0; c < DP; c += 16) {  // few registers: the scores are still in theirs
+                            uint32_t o[16];
+                            tmem_ld16(o_tm + c, o);
+                            tmem_ld_wait();
+                            tmem_use<16>(o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(o_tm + c, o);
+                        }
+                    }
+                }
+                const float neg = m == -INFINITY ? 0.0f : -m;
+                float2 sum = make_float2(0.0f, 0.0f);
+                const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), neg2 = make_float2(neg, neg);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[32 * c + 2 * e]), __uint_as_float(s[32 * c + 2 * e + 1])),
+                                                    sc2, neg2);
+                        const float2 w2 = make_float2(ex2(z.x), ex2(z.y));
+                        sum = __fadd2_rn(sum, w2);
+                        w[e] = pack2<T>(w2.x, w2.y);
+                    }
+                    tmem_st16(s_tm + 16 * c, w);
+                }
+                l += sum.x + sum.y;
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_bar[t]);
+            }
+            const bool took = kb0 < kb1;
+            if (took && !dead) dead = !__all_sync(0xffffffffu, mbar_wait(&o_bar[t], o_phase++ & 1u, a.status));
+            tc_fence_after();
+            // The item's place, and the next one's queries before its rows are written: their first scores
+            // can then run beside that.
+            const bool odd = took && *reinterpret_cast<volatile int*>(&odd_at[seg & 3]) == seg + 1;
+            const int ch = h, cb = b, cp = p, item_begin = pos - k0;
+            pos += k1 - k0;
+            if (pos < end) {
+                next_item();
+                if (takes(0, min(pr.blocks, end - pos))) stage_q();
+            }
+            // what NaN and Inf of the masked blocks this row sees, added to 32 values from dim d0 on
+            auto add_odd = [&](float (&o)[32], int d0) {
+                const Pair cur = pair_of(a, view(cb), cp - seq_first[cb], per_tile);
+                for (int j = max(sr.lo, max(kb0, 0) * kTileKeys); j < min(sr.hi, kb1 * kTileKeys); ++j) {
+                    if (!cur.masked(j / kTileKeys)) continue;
+                    const int page = a.batch.page_table[(int64_t)(seq0 + cb) * a.batch.max_pages + j / a.page_size];
+                    if (page < 0 || page >= a.num_pages) continue;
+                    const uint16_t* v = reinterpret_cast<const uint16_t*>(a.vc) +
+                                        (((int64_t)page * a.hkv + ch) * a.page_size + j % a.page_size) * a.D + d0;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (d0 + e < a.D && odd16(v[e], kBf16)) o[e] += unpack2<T>(v[e]).x;
+                }
+            };
+            auto write = [&](const float (&o)[32], int d0, float inv) {
+                T* out = reinterpret_cast<T*>(a.out) + token * a.ldo +
+                         (int64_t)(ch * G + row % G) * a.D + d0;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    if (d0 + e >= a.D) break;
+                    if (a.out_vec) {
+                        uint4 v;
+                        v.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
+                        v.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
+                        v.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
+                        v.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
+                        *reinterpret_cast<uint4*>(out + e) = v;
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 8; ++x) out[e + x] = from_f32<T>(o[e + x] * inv);
+                    }
+                }
+            };
+            auto load_o = [&](float (&o)[32], int d0) {  // every lane of the warp
+                uint32_t r[32];
+                if (took) {
+                    tmem_ld32(o_tm + d0, r);
+                    tmem_ld_wait();
+                    tmem_use(r);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = took ? __uint_as_float(r[e]) : 0.0f;
+                if (odd && valid) add_odd(o, d0);
+            };
+            const bool complete = k0 == 0 && k1 == blocks;
+            constexpr int PIECE = kTileRows * (DP + 2);
+            auto piece_of = [&](int c, bool later) { return a.partials + ((2 * (int64_t)c + later) * 2 + t) * PIECE; };
+            if (rows > 0 && complete) {
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+                for (int d0 = 0; d0 < a.D; d0 += 32) {
+                    float o[32];
+                    load_o(o, d0);
+                    if (valid) write(o, d0, inv);
+                }
+            } else if (rows > 0) {
+                float* piece = piece_of(blockIdx.x, item_begin > begin);
+#pragma unroll 1
+                for (int d0 = 0; d0 < a.D; d0 += 32) {
+                    float o[32];
+                    load_o(o, d0);
+                    float* to = piece + d0 * kTileRows + row;  // dims outside, rows inside: whole lines
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) __stcg(to + e * kTileRows, o[e]);
+                }
+                __stcg(reinterpret_cast<float2*>(piece + DP * kTileRows) + row, make_float2(m, l));
+                const int cut = more * (quota + 1);
+                auto owner = [&](int x) { return x < cut ? x / (quota + 1) : more + (x - cut) / quota; };
+                const int c0 = owner(item_begin), c1 = owner(item_begin + blocks - 1), pieces = c1 - c0 + 1;
+                __threadfence();
+                named_barrier_sync(bar, 128);
+                if (row == 0) {
+                    last[t] = atomicAdd(&a.tickets[2 * c0 + t], 1u) == (unsigned)(pieces - 1);
+                    if (last[t]) a.tickets[2 * c0 + t] = 0;
+                }
+                named_barrier_sync(bar, 128);
+                if (last[t]) {
+                    __threadfence();
+                    const bool first_later = item_begin > share(c0);
+                    float mm = -INFINITY, ll = 0.0f;
+                    for (int i = 0; i < pieces; ++i)
+                        mm = fmaxf(mm, __ldcg(reinterpret_cast<const float2*>(piece_of(c0 + i, i == 0 && first_later) + DP * kTileRows) + row).x);
+                    const float mu = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll 1
+                    for (int d0 = 0; d0 < a.D; d0 += 32) {
+                        float o[32] = {};
+                        ll = 0.0f;
+                        for (int i = 0; i < pieces; ++i) {
+                            const float* pc = piece_of(c0 + i, i == 0 && first_later);
+                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pc + DP * kTileRows) + row);
+                            const float f = ex2(ml.x - mu);
+                            ll += ml.y * f;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] += __ldcg(pc + (d0 + e) * kTileRows + row) * f;
+                        }
+                        if (valid) write(o, d0, ll > 0.0f ? 1.0f / ll : 0.0f);
+                    }
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int DP>
+cudaError_t launch_tiles(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const mgpu_k::AttendArgs& a) {
+    auto kern = attend_tile_kernel<T, DP>;
+    static std::atomic<uint64_t> configured{0};
+    cudaError_t e = allow_smem(kern, tile_smem<DP>(), configured);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)c.sm_count);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = tile_smem<DP>();
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    for (int seq0 = 0; seq0 < a.batch.n_seqs && e == cudaSuccess; seq0 += kTileSeqs)
+        e = cudaLaunchKernelEx(&cfg, kern, mk, mv, a, seq0);
+    return e;
 }
 
 template <typename T>
 cudaError_t launch_attend(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const mgpu_k::AttendArgs& a) {
     cudaError_t e = a.D <= 64 ? launch_rows<T, 64>(c, mk, mv, a) : launch_rows<T, 128>(c, mk, mv, a);
-    if (e != cudaSuccess || a.batch.max_q_len * (int64_t)(a.hq / a.hkv) <= kRowsMax) return e;
-    const dim3 grid((unsigned)a.batch.n_tokens, (unsigned)((a.hq + 3) / 4));
-    attend_kernel<T><<<grid, 128, 0, c.stream>>>(a);
-    return cudaGetLastError();
+    if (e != cudaSuccess || !mgpu_k::attend_many_rows(a)) return e;
+    return a.D <= 64 ? launch_tiles<T, 64>(c, mk, mv, a) : launch_tiles<T, 128>(c, mk, mv, a);
 }
 
 }  // namespace
 
 namespace mgpu_k {
 
-size_t attend_scratch_bytes(int sm_count) { return (size_t)sm_count * 2 * kRowsMax * (128 + 2) * sizeof(float); }
+size_t attend_scratch_bytes(int sm_count, bool many_rows) {
+    return (size_t)sm_count * 2 * (many_rows ? 2 * kTileRows : kRowsMax) * (128 + 2) * sizeof(float);
+}
+bool attend_many_rows(const AttendArgs& a) { return a.batch.max_q_len * (int64_t)(a.hq / a.hkv) > kRowsMax; }
 
 bool make_cache_map(CUtensorMap* m, const void* side, int type, int num_pages, int page_size, int kv_heads, int head_dim) {
     int rows = kBlock;
@@ -673,6 +1310,8 @@ cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUt
     a.page_shift = -1;
     for (int i = 3; i < 31; ++i)
         if (a.page_size == 1 << i) a.page_shift = i;
+    a.q_vec = ((uintptr_t)a.q & 15) == 0 && a.ldq % 8 == 0;
+    a.out_vec = ((uintptr_t)a.out & 15) == 0 && a.ldo % 8 == 0;
     a.q_pairs = ((uintptr_t)a.q & 3) == 0 && a.ldq % 2 == 0;
     a.out_pairs = ((uintptr_t)a.out & 3) == 0 && a.ldo % 2 == 0;
     return a.type == MGPU_F16 ? launch_attend<__half>(c, mk, mv, a) : launch_attend<__nv_bfloat16>(c, mk, mv, a);

@@ -134,11 +134,14 @@ struct AttendArgs {
     int causal, window;
     int* status;
     float* partials;        // attend_scratch_bytes
-    unsigned int* tickets;  // one per CTA, zero between calls (the kernel leaves them so)
+    unsigned int* tickets;  // two per CTA, zero between calls (the kernels leave them so)
     // set by paged_attention
-    int box_rows, page_shift, max_rows, q_pairs, out_pairs;
+    int box_rows, page_shift, max_rows, q_pairs, out_pairs, q_vec, out_vec;
 };
-size_t attend_scratch_bytes(int sm_count);
+// Whether some sequence may have more rows (new tokens x query heads of a key head) than the
+// kernel for few rows takes, and the scratch that needs.
+bool attend_many_rows(const AttendArgs& a);
+size_t attend_scratch_bytes(int sm_count, bool many_rows);
 // The TMA map of one side of a cache: [num_pages * kv_heads][page_size][head_dim], boxes of 64
 // dims x the most rows that divide both a page and a block of keys.
 bool make_cache_map(CUtensorMap* m, const void* side, int type, int num_pages, int page_size, int kv_heads, int head_dim);

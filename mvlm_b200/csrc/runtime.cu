@@ -106,7 +106,7 @@ bool is_quant_type(int t) { return t == MGPU_Q4_0 || t == MGPU_Q8_0; }
 size_t quant_row_bytes(int t, int64_t k) { return (size_t)((k + 31) / 32) * (t == MGPU_Q4_0 ? 18 : 34); }
 
 // Scratch arena layout: [0, 64 KB) holds the split-K tickets of gemv_kn, [64 KB, 128 KB) those of
-// the split-K GEMM and [128 KB, 132 KB) those of the paged attention's shares (one per CTA of a
+// the split-K GEMM and [128 KB, 132 KB) those of the paged attention's shares (two per CTA of a
 // one-wave grid); all must stay zero between launches (the kernels reset them).
 // Everything from kScratchOffset on is free for per-call use (split-K partials, im2col
 // patches, staged operands), in stream order.
@@ -1249,9 +1249,12 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch*
     REQUIRE(!ro.overlaps(rows_range(q, rows, width, a.ldq)), "paged_attention: out overlaps q");
     REQUIRE(!ro.overlaps(range_of(c->k, c->k->bytes)) && !ro.overlaps(range_of(c->v, c->v->bytes)),
             "paged_attention: out overlaps the cache");
-    // the kernels count blocks of 64 keys, and tiles of rows, in 32 bits
-    if (((int64_t)batch->max_pages * c->page_size / 64 + 2) * batch->n_seqs * c->kv_heads > INT32_MAX ||
-        (int64_t)batch->max_pages * c->page_size > INT32_MAX || rows * q_heads > INT32_MAX) {
+    // the kernels count blocks of 64 or 128 keys, and pairs of tiles over them, in 32 bits
+    const int64_t most_kv = (int64_t)batch->max_pages * c->page_size, group = q_heads / c->kv_heads;
+    const int64_t pairs = rows / (2 * (kMaxGroup / group)) + batch->n_seqs;
+    if (most_kv > INT32_MAX / 2 || rows * q_heads > INT32_MAX / 2 ||
+        (double)(most_kv / 64 + 2) * batch->n_seqs * c->kv_heads > INT32_MAX ||
+        (batch->max_q_len * group > 16 && (double)(most_kv / 128 + 2) * (double)pairs * c->kv_heads > INT32_MAX)) {
         set_error(MGPU_ERR_UNSUPPORTED, "paged_attention: more than 2^31 blocks of keys or rows of queries");
         return nullptr;
     }
@@ -1271,7 +1274,7 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch*
     a.causal = causal != 0;
     a.window = window;
     a.status = d->d_status;
-    if (!ensure_workspace(d, kScratchOffset + mgpu_k::attend_scratch_bytes(d->sm_count))) return nullptr;
+    if (!ensure_workspace(d, kScratchOffset + mgpu_k::attend_scratch_bytes(d->sm_count, mgpu_k::attend_many_rows(a)))) return nullptr;
     a.tickets = (unsigned int*)((char*)d->workspace + kAttendTicketOffset);
     a.partials = (float*)((char*)d->workspace + kScratchOffset);
     mgpu_event* ev = event_begin(d);

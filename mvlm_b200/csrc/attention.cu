@@ -27,12 +27,15 @@ constexpr int kBlock = 64;  // keys of a block: one row of the TMA boxes' 64-row
 struct Seen {
     int lo, hi;
 };
-__device__ __forceinline__ Seen seen_by(const mgpu_k::AttendArgs& a, const SeqView& s, int i) {
-    const long long p = (long long)s.kv - s.n + i;
+// `p`: the row's token's index in a sequence of kv (lengths, windows and counts stay below 2^30).
+__device__ __forceinline__ Seen seen_at(const mgpu_k::AttendArgs& a, int kv, int p) {
     Seen r;
-    r.hi = (int)max(0ll, a.causal ? min(p + 1, (long long)s.kv) : (long long)s.kv);
-    r.lo = a.window > 0 ? (int)min((long long)r.hi, max(0ll, p - a.window + 1)) : 0;
+    r.hi = max(0, a.causal ? min(p + 1, kv) : kv);
+    r.lo = a.window > 0 ? min(r.hi, max(0, p - a.window + 1)) : 0;
     return r;
+}
+__device__ __forceinline__ Seen seen_by(const mgpu_k::AttendArgs& a, const SeqView& s, int i) {
+    return seen_at(a, s.kv, s.kv - s.n + i);
 }
 __device__ __forceinline__ bool odd16(uint32_t h, bool bf16) {
     const uint32_t e = bf16 ? 0x7F80u : 0x7C00u;
@@ -605,7 +608,7 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
 // 4 D operations to a row and key, and by one exponential to a row and key.  A CTA takes two tiles of
 // up to 128 rows (whole tokens: 128 / G of them) over the same blocks of 128 keys.  One thread issues
 // S_t = Q_t K^T and O_t += P_t V of both tiles in turn, so that one tile's products run while the
-// other's softmax does; scores, weights and O stay in TMEM, weights in the place of the scores.  Each
+// other's softmax does; scores, weights and O stay in TMEM, weights in the place of half the scores.  Each
 // tile has four warps, a thread to a row, which needs no exchange for its maximum and sum.  O is
 // rescaled only when a row's maximum has grown by more than 2^8 since its reference was taken: weights
 // stay below 2^8, and most blocks then leave O alone.  All blocks of all items (sequence, key head,
@@ -669,21 +672,13 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 // Two tiles of one sequence's tokens.  Blocks are counted from the sequence's start.
 struct Pair {
-    SeqView s;
-    int lo, blocks;              // the blocks that either tile needs: [lo, lo + blocks)
-    int first[2], rows[2];       // a tile's first token and its rows (0: no tile)
-    int t_lo[2], t_hi[2];        // its blocks
+    int lo, blocks;                // the blocks that either tile needs: [lo, lo + blocks)
+    int first[2], rows[2];         // a tile's first token and its rows (0: no tile)
+    int t_lo[2], t_hi[2];          // its blocks
     int whole_lo[2], whole_hi[2];  // the keys that all its rows see
-    __device__ __forceinline__ bool in(int t, int kb) const { return kb >= t_lo[t] && kb < t_hi[t]; }
-    __device__ __forceinline__ bool whole(int t, int kb) const {
-        return kb * kTileKeys >= whole_lo[t] && (kb + 1) * kTileKeys <= whole_hi[t];
-    }
-    // some row of a tile that takes the block does not see all of it
-    __device__ __forceinline__ bool masked(int kb) const { return (in(0, kb) && !whole(0, kb)) || (in(1, kb) && !whole(1, kb)); }
 };
 __device__ __forceinline__ Pair pair_of(const mgpu_k::AttendArgs& a, const SeqView& s, int j, int per_tile) {
     Pair p;
-    p.s = s;
     const int G = a.hq / a.hkv;
     int lo = INT_MAX, hi = 0;
 #pragma unroll
@@ -708,23 +703,50 @@ __device__ __forceinline__ Pair pair_of(const mgpu_k::AttendArgs& a, const SeqVi
     return p;
 }
 
+// What a CTA does of one item, as its scheduling warp hands it to the others.
+struct Segment {
+    int kb0, kb1;                  // blocks
+    int lo[2], hi[2];              // those that each tile takes (none: lo >= hi)
+    int whole_lo[2], whole_hi[2];  // keys that all rows of a tile see
+    int rows[2], row0[2], index[2];  // rows of a tile; activation row and index in the sequence of its first token
+    int kv, seq, h;
+    int complete;                  // all of the item's blocks; else the piece's slot and who has the others
+    int slot, c0, pieces, first_slot;
+    int more;                      // another segment follows
+    int odd;                       // NaN or Inf was taken out of a block of V
+    __device__ __forceinline__ bool in(int t, int kb) const { return kb >= lo[t] && kb < hi[t]; }
+    __device__ __forceinline__ bool whole(int t, int kb) const {
+        return kb * kTileKeys >= whole_lo[t] && (kb + 1) * kTileKeys <= whole_hi[t];
+    }
+    // some row of a tile that takes the block does not see all of it
+    __device__ __forceinline__ bool masked(int kb) const { return (in(0, kb) && !whole(0, kb)) || (in(1, kb) && !whole(1, kb)); }
+};
+constexpr int kSegments = 4;  // handed out ahead
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attend_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const mgpu_k::AttendArgs a, int seq0) {
     constexpr int SLABS = DP / 64, QB = kTileRows * DP * 2, SB = tile_stage_bytes<DP>(), SLAB = kTileKeys * 128;
     constexpr int S = tile_stages<DP>();
+    constexpr int PIECE = kTileRows * (DP + 2);
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = qs + 2 * QB;
     int* seq_first = reinterpret_cast<int*>(ring + S * SB);  // [n + 1] pairs before a sequence
     int* cum = seq_first + kTileSeqs + 1;                    // [entries + 1] blocks before an entry
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], q_bar[2], s_bar[2], p_bar[2], o_bar[2], clean_bar[S], drain_bar;
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2], p_bar[2], o_bar[2], drain_bar,
+        seg_full[kSegments], seg_empty[kSegments];
+    __shared__ Segment segs[kSegments];
     __shared__ uint32_t tmem_slot;
-    __shared__ int odd_at[4];  // 1 + the segment in whose masked blocks of V NaN or Inf was found
-    __shared__ int warp_part[kTileThreads / 32], start[3];
-    __shared__ bool last[2];
+    __shared__ int warp_part[kTileThreads / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.hq / a.hkv, per_tile = kTileRows / G;
 
@@ -732,7 +754,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = 0; i < S; ++i) {
             mbar_init(&full_bar[i], 1);
             mbar_init(&empty_bar[i], 1);
-            mbar_init(&clean_bar[i], 2);  // V: the two warps that look it over
+            mbar_init(&clean_bar[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_bar[t], 4);
@@ -741,12 +763,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             mbar_init(&o_bar[t], 1);
         }
         mbar_init(&drain_bar, 1);
+        for (int i = 0; i < kSegments; ++i) {
+            mbar_init(&seg_full[i], 1);
+            mbar_init(&seg_empty[i], 11);  // every other warp
+        }
         fence_mbar_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
-    if (tid < 4) odd_at[tid] = 0;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // ---- the table of items: pairs before each sequence, blocks before each run of pairs
     const int seqs = min(a.batch.n_seqs - seq0, kTileSeqs);
@@ -818,34 +843,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const bool by_item = items <= (int)gridDim.x && most <= (total + (int)gridDim.x - 1) / (int)gridDim.x + kJoinBlocks;
     const int shares = by_item ? items : min((int)gridDim.x, total);
     if ((int)blockIdx.x >= shares) return;
-    const int quota = total / shares, more = total % shares;
-    auto share = [&](int c) { return c * quota + min(c, more); };
-    if (tid == 0) {
-        int h, p, k = 0;
-        if (by_item) {
-            h = blockIdx.x / pairs;
-            p = blockIdx.x % pairs;
-        } else {
-            const int x = share(blockIdx.x);
-            h = x / head_blocks;
-            int y = x % head_blocks, lo2 = 0, hi2 = entries;
-            while (hi2 - lo2 > 1) {
-                const int mid = (lo2 + hi2) / 2;
-                if (cum[mid] <= y) lo2 = mid;
-                else hi2 = mid;
-            }
-            y -= cum[lo2];
-            for (p = lo2 * run;; ++p) {
-                const int b = seq_of_pair(p), n = pair_of(a, view(b), p - seq_first[b], per_tile).blocks;
-                if (y < n) break;
-                y -= n;
-            }
-            k = y;
-        }
-        start[0] = h;
-        start[1] = p;
-        start[2] = k;
-    }
     if (warp == 8) {
         tmem_alloc(&tmem_slot, 512);
         tmem_relinquish();
@@ -854,195 +851,270 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    const int begin = by_item ? 0 : share(blockIdx.x);
-    int end = by_item ? 0 : share(blockIdx.x + 1);  // by_item: set below
-    int h = start[0], p = start[1], k = start[2], b = seq_of_pair(p);
-    Pair pr = pair_of(a, view(b), p - seq_first[b], per_tile);
-    if (by_item) end = pr.blocks;
-    auto next_item = [&] {
-        k = 0;
-        if (++p == pairs) {
-            p = 0;
-            ++h;
-            b = 0;
-        }
-        while (seq_first[b + 1] <= p) ++b;
-        pr = pair_of(a, view(b), p - seq_first[b], per_tile);
-    };
+    auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, a.status)); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        bool ok = true;
-        if (warp == 8) {
-            // ------------------------------------------------------------ products
-            if (lane == 0) {
-                const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys);
-                const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
-                const int dims = (a.D + 15) / 16;
-                uint32_t n = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};  // n: blocks so far
-                auto product_s = [&](int t, uint32_t stage) {
-                    const uint32_t qa = smem_u32(qs) + t * QB, kb = smem_u32(ring) + stage * SB;
-                    for (int d = 0; d < dims; ++d) {
-                        const uint32_t off = (d >> 2) * SLAB + (d & 3) * 32;  // Q and K have the same slabs
-                        umma_f16(tmem + t * kTileKeys, smem_desc(qa + off, 16, 1024, kSwizzle128B),
-                                 smem_desc(kb + off, 16, 1024, kSwizzle128B), id_s, d != 0);
+        // Every warp below walks as one; only single instructions are one thread's.
+        if (warp == 11) {
+            // ------------------------------------------------------------ scheduling
+            const int quota = total / shares, extra = total % shares;
+            auto share = [&](int c) { return c * quota + min(c, extra); };
+            const int cut = extra * (quota + 1);
+            auto owner = [&](int x) { return x < cut ? x / (quota + 1) : extra + (x - cut) / quota; };
+            const int begin = by_item ? 0 : share(blockIdx.x);
+            int h, p, k = 0, b;
+            if (by_item) {
+                h = blockIdx.x / pairs;
+                p = blockIdx.x % pairs;
+                b = seq_of_pair(p);
+            } else {
+                h = begin / head_blocks;
+                int y = begin % head_blocks, lo2 = 0, hi2 = entries;
+                while (hi2 - lo2 > 1) {
+                    const int mid = (lo2 + hi2) / 2;
+                    if (cum[mid] <= y) lo2 = mid;
+                    else hi2 = mid;
+                }
+                y -= cum[lo2];
+                for (p = lo2 * run, b = seq_of_pair(p);; ++p) {
+                    while (seq_first[b + 1] <= p) ++b;
+                    const int n = pair_of(a, view(b), p - seq_first[b], per_tile).blocks;
+                    if (y < n) break;
+                    y -= n;
+                }
+                k = y;
+            }
+            int end = by_item ? INT_MAX : share(blockIdx.x + 1);
+            int i = 0;
+            for (int pos = begin; pos < end; ++i) {
+                const SeqView s = view(b);
+                const Pair pr = pair_of(a, s, p - seq_first[b], per_tile);
+                if (by_item) end = pr.blocks;
+                const int k1 = min(pr.blocks, k + (end - pos)), item = pos - k;
+                if (!wait(&seg_empty[i % kSegments], (i / kSegments) ^ 1)) break;
+                if (lane == 0) {
+                    Segment& g = segs[i % kSegments];
+                    g.kb0 = pr.lo + k;
+                    g.kb1 = pr.lo + k1;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        g.lo[t] = max(pr.t_lo[t], pr.lo + k);
+                        g.hi[t] = min(pr.t_hi[t], pr.lo + k1);
+                        g.whole_lo[t] = pr.whole_lo[t];
+                        g.whole_hi[t] = pr.whole_hi[t];
+                        g.rows[t] = pr.rows[t];
+                        g.row0[t] = s.q0 + pr.first[t];
+                        g.index[t] = s.kv - s.n + pr.first[t];
                     }
-                    umma_commit(&s_bar[t]);
-                };
-                for (int pos = begin; ok && pos < end;) {
-                    const int k1 = min(pr.blocks, k + (end - pos));
-                    bool started[2] = {false, false};  // the tile has its Q, and O its first product
-                    bool has_o[2] = {false, false};
-                    auto score = [&](int t, int kb, uint32_t stage) {
+                    g.kv = s.kv;
+                    g.seq = seq0 + b;
+                    g.h = h;
+                    g.complete = k == 0 && k1 == pr.blocks;
+                    if (!g.complete) {
+                        // a share's pieces: slot 2c for the item it begins in, 2c + 1 for a later one
+                        g.slot = 2 * blockIdx.x + (item > begin);
+                        g.c0 = owner(item);
+                        g.pieces = owner(item + pr.blocks - 1) - g.c0 + 1;
+                        g.first_slot = 2 * g.c0 + (item > share(g.c0));
+                    }
+                    g.more = pos + k1 - k < end;
+                    g.odd = 0;
+                    mbar_arrive(&seg_full[i % kSegments]);
+                }
+                __syncwarp();
+                pos += k1 - k;
+                k = 0;
+                if (++p == pairs) {
+                    p = 0;
+                    ++h;
+                    b = 0;
+                }
+                if (pos < end)
+                    while (seq_first[b + 1] <= p) ++b;
+            }
+        } else {
+            uint32_t n = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};  // n: blocks so far
+            // Descriptors of tile 0's Q, of stage 0 as keys and as values; steps and stages are added to
+            // their address fields, in units of 16 bytes.  The fewer instructions between two products,
+            // the less the tensor cores wait.
+            const uint64_t q_desc = smem_desc(smem_u32(qs), 16, 1024, kSwizzle128B);
+            const uint64_t k_desc = smem_desc(smem_u32(ring), 16, 1024, kSwizzle128B);
+            const uint64_t v_desc = smem_desc(smem_u32(ring), SLAB, 1024, kSwizzle128B);
+            const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys);
+            const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
+            const int dims = (a.D + 15) / 16;
+            const int rows = a.box_rows, chunks = kTileKeys / rows;  // loads: a lane has a chunk of one page
+            bool ok = true, more = true;
+            for (int i = 0; ok && more; ++i) {
+                ok = wait(&seg_full[i % kSegments], i / kSegments);
+                if (!ok) break;
+                const Segment& g = segs[i % kSegments];
+                more = g.more;
+                const int kb0 = g.kb0, kb1 = g.kb1;
+                if (warp == 8) {
+                    // -------------------------------------------------------- products
+                    bool started[2] = {false, false}, has_o[2] = {false, false};
+                    auto score = [&](const int t, uint32_t stage) {
                         if (!started[t]) {
-                            ok = ok && mbar_wait(&q_bar[t], q_phase[t]++ & 1u, a.status);
+                            ok = wait(&q_bar[t], q_phase[t]++);
+                            if (!ok) return;
                             started[t] = true;
                         }
-                        if (ok) product_s(t, stage);
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint64_t qd = q_desc + t * (QB >> 4), kd = k_desc + stage * (SB >> 4);
+#pragma unroll
+                            for (int d = 0; d < DP / 16; ++d) {
+                                const int step = (d >> 2) * (SLAB >> 4) + (d & 3) * 2;  // Q and K have the same slabs
+                                if (d < dims) umma_f16(tmem + t * kTileKeys, qd + step, kd + step, id_s, d != 0);
+                            }
+                            umma_commit(&s_bar[t]);
+                        }
+                        __syncwarp();
                     };
-                    for (int i = k; ok && i < k1; ++i, ++n) {
-                        const int kb = pr.lo + i;
+                    auto release = [&](uint32_t stage) {
+                        if (elect_one()) umma_commit(&empty_bar[stage]);
+                        __syncwarp();
+                    };
+                    for (int kb = kb0; ok && kb < kb1; ++kb, ++n) {
                         const uint32_t ks = (2 * n) % S, vs = (2 * n + 1) % S, kn = (2 * n + 2) % S;
-                        if (i == k) {
-                            ok = mbar_wait(&full_bar[ks], (2 * n / S) & 1u, a.status);
-                            if (!ok) break;
-                            tc_fence_after();
+                        const bool last = kb + 1 == kb1;
+                        if (kb == kb0) {
+                            ok = wait(&full_bar[ks], 2 * n / S);
 #pragma unroll
                             for (int t = 0; t < 2; ++t)
-                                if (pr.in(t, kb)) score(t, kb, ks);
-                            umma_commit(&empty_bar[ks]);
+                                if (ok && g.in(t, kb)) score(t, ks);
+                            release(ks);
                         }
-                        ok = ok && mbar_wait(&full_bar[vs], ((2 * n + 1) / S) & 1u, a.status);
-                        ok = ok && mbar_wait(&clean_bar[vs], ((2 * n + 1) / S) & 1u, a.status);
+                        ok = ok && wait(&full_bar[vs], (2 * n + 1) / S);
+                        ok = ok && wait(&clean_bar[vs], (2 * n + 1) / S);
                         bool have_next = false;
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
-                            if (!ok) break;
-                            if (pr.in(t, kb)) {
-                                ok = mbar_wait(&p_bar[t], p_phase[t]++ & 1u, a.status);
+                            if (ok && g.in(t, kb)) {
+                                ok = wait(&p_bar[t], p_phase[t]++);
                                 if (!ok) break;
                                 tc_fence_after();
-                                const uint32_t vb = smem_u32(ring) + vs * SB;
-                                for (int d = 0; d < kTileKeys / 16; ++d)
-                                    umma_f16_ts(tmem + 256 + t * 128, tmem + t * kTileKeys + d * 8,
-                                                smem_desc(vb + d * 2048, SLAB, 1024, kSwizzle128B), id_o, has_o[t] || d != 0);
+                                if (elect_one()) {
+                                    const uint64_t vd = v_desc + vs * (SB >> 4);
+#pragma unroll
+                                    for (int d = 0; d < kTileKeys / 16; ++d)
+                                        umma_f16_ts(tmem + 256 + t * 128, tmem + t * kTileKeys + 64 + d * 8, vd + d * (2048 >> 4), id_o,
+                                                    has_o[t] || d != 0);
+                                    if (last || !g.in(t, kb + 1)) umma_commit(&o_bar[t]);
+                                }
+                                __syncwarp();
                                 has_o[t] = true;
-                                if (i + 1 == k1 || !pr.in(t, kb + 1)) umma_commit(&o_bar[t]);
                             }
-                            if (i + 1 < k1 && pr.in(t, kb + 1)) {
-                                if (!have_next) ok = mbar_wait(&full_bar[kn], ((2 * n + 2) / S) & 1u, a.status);
-                                if (!ok) break;
+                            if (ok && !last && g.in(t, kb + 1)) {
+                                if (!have_next) ok = wait(&full_bar[kn], (2 * n + 2) / S);
                                 have_next = true;
-                                tc_fence_after();
-                                score(t, kb + 1, kn);
+                                if (ok) score(t, kn);
                             }
                         }
                         if (!ok) break;
-                        umma_commit(&empty_bar[vs]);
-                        if (i + 1 < k1) {
+                        release(vs);
+                        if (!last) {
                             // a block that no tile takes still has to arrive before its stage is given back
-                            if (!have_next) ok = mbar_wait(&full_bar[kn], ((2 * n + 2) / S) & 1u, a.status);
-                            umma_commit(&empty_bar[kn]);
+                            if (!have_next) ok = wait(&full_bar[kn], (2 * n + 2) / S);
+                            release(kn);
                         }
                     }
-                    pos += k1 - k;
-                    if (pos < end) next_item();
-                }
-                umma_commit(&drain_bar);  // all products have ended before TMEM is given back
-                mbar_wait(&drain_bar, 0, a.status);
-            }
-        } else if (warp == 9) {
-            // ------------------------------------------------------------ loads
-            const int rows = a.box_rows, chunks = kTileKeys / rows;
-            const bool loads = lane < chunks;
-            uint32_t it = 0;
-            for (int pos = begin; ok && pos < end;) {
-                const int k1 = min(pr.blocks, k + (end - pos));
-                for (int i = k; ok && i < k1; ++i) {
-                    const int j = (pr.lo + i) * kTileKeys + lane * rows;
-                    int z = a.num_pages * a.hkv, y = 0;
-                    if (loads && j < pr.s.kv) {
-                        const int at = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
-                        const int page = __ldg(a.batch.page_table + (int64_t)(seq0 + b) * a.batch.max_pages + at);
-                        if (page >= 0 && page < a.num_pages) {
-                            z = page * a.hkv + h;
-                            y = j - at * a.page_size;
-                        } else {
-                            atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-                        }
-                    }
-#pragma unroll
-                    for (int side = 0; side < 2; ++side, ++it) {
-                        const uint32_t st = it % S;
-                        ok = __all_sync(0xffffffffu, mbar_wait(&empty_bar[st], ((it / S) & 1u) ^ 1u, a.status));
-                        if (!ok) break;
-                        if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB);
-                        __syncwarp();
-                        if (loads)
-                            for (int slab = 0; slab < SLABS; ++slab)
-                                tma_load_3d(ring + st * SB + slab * SLAB + lane * rows * 128, side ? &tmV : &tmK, slab * 64, y, z,
-                                            &full_bar[st]);
-                    }
-                }
-                pos += k1 - k;
-                if (pos < end) next_item();
-            }
-        } else {
-            // ------------------------------------------------------------ NaN and Inf in V
-            // A weight of 0 times NaN or Inf is not 0: where some row does not see all keys of a block,
-            // such values leave the block, and the rows that see them add them at the end.
-            uint32_t n = 0;
-            int seg = 0;
-            for (int pos = begin; ok && pos < end; ++seg) {
-                const int k1 = min(pr.blocks, k + (end - pos));
-                for (int i = k; ok && i < k1; ++i, ++n) {
-                    const uint32_t st = (2 * n + 1) % S;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&full_bar[st], ((2 * n + 1) / S) & 1u, a.status));
-                    if (!ok) break;
-                    if (pr.masked(pr.lo + i)) {
-                        uint4* v = reinterpret_cast<uint4*>(ring + st * SB);
-                        bool found = false;
-                        for (int x = (warp - 10) * 32 + lane; x < SB / 16; x += 64) {
-                            const uint4 q = v[x];
-                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-                            bool any = false;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) any |= odd16(w[e], kBf16) || odd16(w[e] >> 16, kBf16);
-                            if (any) {
-                                uint16_t* u = reinterpret_cast<uint16_t*>(v + x);
-                                for (int e = 0; e < 8; ++e)
-                                    if (odd16(u[e], kBf16)) u[e] = 0;
-                                found = true;
+                } else if (warp == 9) {
+                    // -------------------------------------------------------- loads
+                    for (int kb = kb0; ok && kb < kb1; ++kb, ++n) {
+                        const int j = kb * kTileKeys + lane * rows;
+                        // chunks past the end are read from outside the map, which gives zeros
+                        int z = a.num_pages * a.hkv, y = 0;
+                        if (lane < chunks && j < g.kv) {
+                            const int at = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+                            const int page = a.batch.page_table[(int64_t)g.seq * a.batch.max_pages + at];
+                            if (page >= 0 && page < a.num_pages) {
+                                z = page * a.hkv + g.h;
+                                y = j - at * a.page_size;
+                            } else {
+                                atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
                             }
                         }
-                        if (found) *reinterpret_cast<volatile int*>(&odd_at[seg & 3]) = seg + 1;
-                        fence_proxy_async_smem();
+#pragma unroll
+                        for (int side = 0; side < 2; ++side) {
+                            const uint32_t it = 2 * n + side, st = it % S;
+                            if (!ok) break;
+                            ok = wait(&empty_bar[st], (it / S) ^ 1);
+                            if (!ok) break;
+                            if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB);
+                            __syncwarp();
+                            if (lane < chunks) {
+#pragma unroll
+                                for (int slab = 0; slab < SLABS; ++slab)
+                                    tma_load_3d(ring + st * SB + slab * SLAB + lane * rows * 128, side ? &tmV : &tmK, slab * 64, y, z,
+                                                &full_bar[st]);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                } else {
+                    // -------------------------------------------------------- NaN and Inf in V
+                    // A weight of 0 times NaN or Inf is not 0: where some row does not see all keys of a
+                    // block, such values leave the block, and the rows that see them add them at the end.
+                    for (int kb = kb0; ok && kb < kb1; ++kb, ++n) {
+                        const uint32_t st = (2 * n + 1) % S;
+                        ok = wait(&full_bar[st], (2 * n + 1) / S);
+                        if (!ok) break;
+                        if (g.masked(kb)) {
+                            uint4* v = reinterpret_cast<uint4*>(ring + st * SB);
+                            bool found = false;
+#pragma unroll 8
+                            for (int x = lane; x < SB / 16; x += 32) {
+                                const uint4 q = v[x];
+                                found |= odd16(q.x, kBf16) || odd16(q.x >> 16, kBf16) || odd16(q.y, kBf16) || odd16(q.y >> 16, kBf16) ||
+                                         odd16(q.z, kBf16) || odd16(q.z >> 16, kBf16) || odd16(q.w, kBf16) || odd16(q.w >> 16, kBf16);
+                            }
+                            if (__any_sync(0xffffffffu, found)) {
+                                for (int x = lane; x < SB / 2; x += 32) {
+                                    uint16_t* u = reinterpret_cast<uint16_t*>(v) + x;
+                                    if (odd16(*u, kBf16)) *u = 0;
+                                }
+                                if (lane == 0) segs[i % kSegments].odd = 1;
+                                fence_proxy_async_smem();
+                                __syncwarp();
+                            }
+                        }
+                        if (lane == 0) mbar_arrive(&clean_bar[st]);
                         __syncwarp();
                     }
-                    if (lane == 0) mbar_arrive(&clean_bar[st]);
                 }
-                pos += k1 - k;
-                if (pos < end) next_item();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
+            }
+            if (warp == 8) {
+                if (elect_one()) umma_commit(&drain_bar);  // all products have ended before TMEM is given back
+                __syncwarp();
+                wait(&drain_bar, 0);
+            } else if (warp == 9 && !ok) {
+                // a wait ran out: the copies under way still have to land before the CTA may end
+                for (uint32_t it = n > S ? 2 * n - S : 0; it < 2 * n; ++it) wait(&full_bar[it % S], it / S);
             }
         }
     } else {
         // ---------------------------------------------------------------- softmax: a thread to a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int t = warp >> 2, row = tid & 127, bar = 1 + t;
+        const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of TMEM
         const uint32_t s_tm = tmem + t * kTileKeys + lanes, o_tm = tmem + 256 + t * 128 + lanes;
-        bool dead = false;
-        auto mine = [&](const int (&v)[2]) { return t ? v[1] : v[0]; };  // no indexing: the pair stays in registers
         // this warp's 32 rows of Q into the swizzled slabs, zeros beyond the tile's rows and the head's dims
-        auto stage_q = [&] {
+        auto stage_q = [&](const Segment& g) {
+            if (g.lo[t] >= g.hi[t]) return;
             constexpr int PER = DP / 8;  // 16-byte chunks of a row
             uint8_t* dst = qs + t * QB;
+#pragma unroll 4
             for (int x = lane; x < 32 * PER; x += 32) {
                 const int r = (warp & 3) * 32 + x / PER, c = x % PER;
                 uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < mine(pr.rows) && c * 8 < a.D) {
-                    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(pr.s.q0 + mine(pr.first) + r / G) * a.ldq +
-                                        (int64_t)(h * G + r % G) * a.D + c * 8;
+                if (r < g.rows[t] && c * 8 < a.D) {
+                    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(g.row0[t] + r / G) * a.ldq +
+                                        (int64_t)(g.h * G + r % G) * a.D + c * 8;
                     if (a.q_vec) {
                         v = *reinterpret_cast<const uint4*>(q);
                     } else {
@@ -1057,54 +1129,71 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_bar[t]);
+            __syncwarp();
         };
         uint32_t s_phase = 0, o_phase = 0;
-        int seg = 0;
-        // does the tile take any block of [k, k1) of the item?
-        auto takes = [&](int k0, int k1) { return max(mine(pr.t_lo), pr.lo + k0) < min(mine(pr.t_hi), pr.lo + k1); };
-        if (takes(k, min(pr.blocks, k + (end - begin)))) stage_q();
-        for (int pos = begin; pos < end; ++seg) {
-            const int k0 = k, k1 = min(pr.blocks, k + (end - pos));
-            const int kb0 = max(mine(pr.t_lo), pr.lo + k0), kb1 = min(mine(pr.t_hi), pr.lo + k1);
-            const int whole_lo = mine(pr.whole_lo), whole_hi = mine(pr.whole_hi), rows = mine(pr.rows), blocks = pr.blocks;
-            const int64_t token = (int64_t)pr.s.q0 + mine(pr.first) + row / G;
-            const bool valid = row < rows;
-            const Seen sr = valid ? seen_by(a, pr.s, mine(pr.first) + row / G) : Seen{0, 0};
+        bool ok = wait(&seg_full[0], 0), more = ok;
+        if (ok) stage_q(segs[0]);
+        for (int i = 0; ok && more; ++i) {
+            const Segment& g = segs[i % kSegments];
+            const int kb0 = g.lo[t], kb1 = g.hi[t];
+            const bool valid = row < g.rows[t];
+            const Seen sr = valid ? seen_at(a, g.kv, g.index[t] + row / G) : Seen{0, 0};
             float m = -INFINITY, l = 0.0f;  // the reference (log2 units) and the sum of 2^(s - m)
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!dead) dead = !__all_sync(0xffffffffu, mbar_wait(&s_bar[t], s_phase++ & 1u, a.status));
-                if (dead) break;
+                ok = wait(&s_bar[t], s_phase++);
+                if (!ok) break;
                 tc_fence_after();
-                uint32_t s[128];
+                // The scores are read twice in part: all 128 and the state beside them do not fit the
+                // registers.  Columns 64 .. 127 stay from the search for the maximum; the weights go to
+                // their place, 64 + key / 2, so that columns 0 .. 63 can be read again.
+                const bool all = g.whole(t, kb);
+                const int c0 = sr.lo - kb * kTileKeys, c1 = sr.hi - kb * kTileKeys;
+                auto mask = [&](uint32_t (&s)[32], int at) {
+                    if (all) return;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(s_tm + 32 * c, s + 32 * c);
-                tmem_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_use(s + 32 * c);
-                if (kb * kTileKeys < whole_lo || (kb + 1) * kTileKeys > whole_hi) {
-                    const int c0 = sr.lo - kb * kTileKeys, c1 = sr.hi - kb * kTileKeys;
-#pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c < c0 || c >= c1) s[c] = 0xFF800000u;
-                }
+                    for (int e = 0; e < 32; ++e)
+                        if (at + e < c0 || at + e >= c1) s[e] = 0xFF800000u;
+                };
                 float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+                auto search = [&](const uint32_t (&s)[32]) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 4) {
-                    x0 = fmaxf(x0, __uint_as_float(s[c]));
-                    x1 = fmaxf(x1, __uint_as_float(s[c + 1]));
-                    x2 = fmaxf(x2, __uint_as_float(s[c + 2]));
-                    x3 = fmaxf(x3, __uint_as_float(s[c + 3]));
-                }
+                    for (int e = 0; e < 32; e += 4) {
+                        x0 = fmaxf(x0, __uint_as_float(s[e]));
+                        x1 = fmaxf(x1, __uint_as_float(s[e + 1]));
+                        x2 = fmaxf(x2, __uint_as_float(s[e + 2]));
+                        x3 = fmaxf(x3, __uint_as_float(s[e + 3]));
+                    }
+                };
+                uint32_t sa[32], sb[32];
+                tmem_ld32(s_tm, sa);
+                tmem_ld32(s_tm + 32, sb);
+                tmem_ld_wait();
+                tmem_use(sa);
+                tmem_use(sb);
+                mask(sa, 0);
+                mask(sb, 32);
+                search(sa);
+                search(sb);
+                tmem_ld32(s_tm + 64, sa);
+                tmem_ld32(s_tm + 96, sb);
+                tmem_ld_wait();
+                tmem_use(sa);
+                tmem_use(sb);
+                mask(sa, 64);
+                mask(sb, 96);
+                search(sa);
+                search(sb);
                 const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2;
                 const bool grown = top > m + kGrowth;
                 if (__any_sync(0xffffffffu, grown)) {
                     const float f = grown ? ex2(m - top) : 1.0f;
                     if (grown) m = top;
                     l *= f;
-                    // this tile's product before this block's scores has ended: its scores were issued after it
+                    // the product of the block before has ended: this block's scores were issued after it
                     if (kb > kb0) {
 #pragma unroll 1
-                        for (int c = 0; c < DP; c += 16) {  // few registers: the scores are still in theirs
+                        for (int c = 0; c < DP; c += 16) {
                             uint32_t o[16];
                             tmem_ld16(o_tm + c, o);
                             tmem_ld_wait();
@@ -1118,54 +1207,80 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const float neg = m == -INFINITY ? 0.0f : -m;
                 float2 sum = make_float2(0.0f, 0.0f);
                 const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), neg2 = make_float2(neg, neg);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                auto weigh = [&](const uint32_t (&s)[32], int at) {
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[32 * c + 2 * e]), __uint_as_float(s[32 * c + 2 * e + 1])),
-                                                    sc2, neg2);
+                        const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, neg2);
                         const float2 w2 = make_float2(ex2(z.x), ex2(z.y));
                         sum = __fadd2_rn(sum, w2);
                         w[e] = pack2<T>(w2.x, w2.y);
                     }
-                    tmem_st16(s_tm + 16 * c, w);
-                }
+                    tmem_st16(s_tm + 64 + at / 2, w);
+                };
+                uint32_t sc[32];
+                tmem_ld32(s_tm, sc);
+                weigh(sa, 64);
+                tmem_ld_wait();
+                tmem_use(sc);
+                mask(sc, 0);
+                tmem_ld32(s_tm + 32, sa);
+                weigh(sb, 96);
+                weigh(sc, 0);
+                tmem_ld_wait();
+                tmem_use(sa);
+                mask(sa, 32);
+                weigh(sa, 32);
                 l += sum.x + sum.y;
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_bar[t]);
+                __syncwarp();
             }
+            if (!ok) break;
             const bool took = kb0 < kb1;
-            if (took && !dead) dead = !__all_sync(0xffffffffu, mbar_wait(&o_bar[t], o_phase++ & 1u, a.status));
-            tc_fence_after();
-            // The item's place, and the next one's queries before its rows are written: their first scores
-            // can then run beside that.
-            const bool odd = took && *reinterpret_cast<volatile int*>(&odd_at[seg & 3]) == seg + 1;
-            const int ch = h, cb = b, cp = p, item_begin = pos - k0;
-            pos += k1 - k0;
-            if (pos < end) {
-                next_item();
-                if (takes(0, min(pr.blocks, end - pos))) stage_q();
+            if (took) {
+                ok = wait(&o_bar[t], o_phase++);
+                if (!ok) break;
+                tc_fence_after();
             }
-            // what NaN and Inf of the masked blocks this row sees, added to 32 values from dim d0 on
-            auto add_odd = [&](float (&o)[32], int d0) {
-                const Pair cur = pair_of(a, view(cb), cp - seq_first[cb], per_tile);
-                for (int j = max(sr.lo, max(kb0, 0) * kTileKeys); j < min(sr.hi, kb1 * kTileKeys); ++j) {
-                    if (!cur.masked(j / kTileKeys)) continue;
-                    const int page = a.batch.page_table[(int64_t)(seq0 + cb) * a.batch.max_pages + j / a.page_size];
-                    if (page < 0 || page >= a.num_pages) continue;
-                    const uint16_t* v = reinterpret_cast<const uint16_t*>(a.vc) +
-                                        (((int64_t)page * a.hkv + ch) * a.page_size + j % a.page_size) * a.D + d0;
+            // the next segment's queries before this one's rows are written: their first scores run beside that
+            more = g.more;
+            if (more) {
+                ok = wait(&seg_full[(i + 1) % kSegments], (i + 1) / kSegments);
+                if (ok) stage_q(segs[(i + 1) % kSegments]);
+            }
+            const bool odd = took && valid && *reinterpret_cast<const volatile int*>(&g.odd) != 0;
+            // 32 values of O; every lane of the warp comes here
+            auto load_o = [&](float (&o)[32], int d0) {
+                __syncwarp();
+                uint32_t r[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (d0 + e < a.D && odd16(v[e], kBf16)) o[e] += unpack2<T>(v[e]).x;
+                for (int e = 0; e < 32; ++e) r[e] = 0;
+                if (took) {
+                    tmem_ld32(o_tm + d0, r);
+                    tmem_ld_wait();
+                    tmem_use(r);
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(r[e]);
+                if (odd) {  // NaN and Inf that this row sees
+#pragma unroll 1
+                    for (int j = max(sr.lo, kb0 * kTileKeys); j < min(sr.hi, kb1 * kTileKeys); ++j) {
+                        if (!g.masked(j / kTileKeys)) continue;
+                        const int page = a.batch.page_table[(int64_t)g.seq * a.batch.max_pages + j / a.page_size];
+                        if (page < 0 || page >= a.num_pages) continue;
+                        const uint16_t* v = reinterpret_cast<const uint16_t*>(a.vc) +
+                                            (((int64_t)page * a.hkv + g.h) * a.page_size + j % a.page_size) * a.D + d0;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (d0 + e < a.D && odd16(v[e], kBf16)) o[e] += unpack2<T>(v[e]).x;
+                    }
                 }
             };
             auto write = [&](const float (&o)[32], int d0, float inv) {
-                T* out = reinterpret_cast<T*>(a.out) + token * a.ldo +
-                         (int64_t)(ch * G + row % G) * a.D + d0;
+                T* out = reinterpret_cast<T*>(a.out) + (int64_t)(g.row0[t] + row / G) * a.ldo + (int64_t)(g.h * G + row % G) * a.D + d0;
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
                     if (d0 + e >= a.D) break;
@@ -1182,21 +1297,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
             };
-            auto load_o = [&](float (&o)[32], int d0) {  // every lane of the warp
-                uint32_t r[32];
-                if (took) {
-                    tmem_ld32(o_tm + d0, r);
-                    tmem_ld_wait();
-                    tmem_use(r);
-                }
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = took ? __uint_as_float(r[e]) : 0.0f;
-                if (odd && valid) add_odd(o, d0);
-            };
-            const bool complete = k0 == 0 && k1 == blocks;
-            constexpr int PIECE = kTileRows * (DP + 2);
-            auto piece_of = [&](int c, bool later) { return a.partials + ((2 * (int64_t)c + later) * 2 + t) * PIECE; };
-            if (rows > 0 && complete) {
+            const bool any = (warp & 3) * 32 < g.rows[t];  // this warp has rows
+            if (any && g.complete) {
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll 1
                 for (int d0 = 0; d0 < a.D; d0 += 32) {
@@ -1204,51 +1306,60 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     load_o(o, d0);
                     if (valid) write(o, d0, inv);
                 }
-            } else if (rows > 0) {
-                float* piece = piece_of(blockIdx.x, item_begin > begin);
+            } else if (any) {
+                // a piece: dims outside, rows inside, so that a warp writes whole lines
+                auto piece_of = [&](int slot) { return a.partials + (int64_t)(2 * slot + t) * PIECE + row; };
+                float* piece = piece_of(g.slot);
 #pragma unroll 1
                 for (int d0 = 0; d0 < a.D; d0 += 32) {
                     float o[32];
                     load_o(o, d0);
-                    float* to = piece + d0 * kTileRows + row;  // dims outside, rows inside: whole lines
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) __stcg(to + e * kTileRows, o[e]);
+                    for (int e = 0; e < 32; ++e) __stcg(piece + (d0 + e) * kTileRows, o[e]);
                 }
-                __stcg(reinterpret_cast<float2*>(piece + DP * kTileRows) + row, make_float2(m, l));
-                const int cut = more * (quota + 1);
-                auto owner = [&](int x) { return x < cut ? x / (quota + 1) : more + (x - cut) / quota; };
-                const int c0 = owner(item_begin), c1 = owner(item_begin + blocks - 1), pieces = c1 - c0 + 1;
+                __stcg(piece + DP * kTileRows, m);
+                __stcg(piece + (DP + 1) * kTileRows, l);
+                // the last warp to come to these rows joins their pieces, in order
                 __threadfence();
-                named_barrier_sync(bar, 128);
-                if (row == 0) {
-                    last[t] = atomicAdd(&a.tickets[2 * c0 + t], 1u) == (unsigned)(pieces - 1);
-                    if (last[t]) a.tickets[2 * c0 + t] = 0;
+                __syncwarp();
+                unsigned last = 0;
+                if (lane == 0) {
+                    unsigned int* ticket = a.tickets + 8 * g.c0 + warp;
+                    last = atomicAdd(ticket, 1u) == (unsigned)(g.pieces - 1);
+                    if (last) *ticket = 0;
                 }
-                named_barrier_sync(bar, 128);
-                if (last[t]) {
+                if (__shfl_sync(0xffffffffu, last, 0)) {
                     __threadfence();
-                    const bool first_later = item_begin > share(c0);
-                    float mm = -INFINITY, ll = 0.0f;
-                    for (int i = 0; i < pieces; ++i)
-                        mm = fmaxf(mm, __ldcg(reinterpret_cast<const float2*>(piece_of(c0 + i, i == 0 && first_later) + DP * kTileRows) + row).x);
-                    const float mu = mm == -INFINITY ? 0.0f : mm;
+                    const int pieces = g.pieces;
+                    auto slot_of = [&](int x) { return x == 0 ? g.first_slot : 2 * (g.c0 + x); };
+                    float top = -INFINITY, den = 0.0f;
+                    for (int x = 0; x < pieces; ++x) top = fmaxf(top, __ldcg(piece_of(slot_of(x)) + DP * kTileRows));
+                    const float mu = top == -INFINITY ? 0.0f : top;
+                    for (int x = 0; x < pieces; ++x) {
+                        const float* pc = piece_of(slot_of(x));
+                        den += __ldcg(pc + (DP + 1) * kTileRows) * ex2(__ldcg(pc + DP * kTileRows) - mu);
+                    }
+                    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
 #pragma unroll 1
                     for (int d0 = 0; d0 < a.D; d0 += 32) {
-                        float o[32] = {};
-                        ll = 0.0f;
-                        for (int i = 0; i < pieces; ++i) {
-                            const float* pc = piece_of(c0 + i, i == 0 && first_later);
-                            const float2 ml = __ldcg(reinterpret_cast<const float2*>(pc + DP * kTileRows) + row);
-                            const float f = ex2(ml.x - mu);
-                            ll += ml.y * f;
+                        float o[32];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] += __ldcg(pc + (d0 + e) * kTileRows + row) * f;
+                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+#pragma unroll 1
+                        for (int x = 0; x < pieces; ++x) {
+                            const float* pc = piece_of(slot_of(x));
+                            const float f = ex2(__ldcg(pc + DP * kTileRows) - mu);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] += __ldcg(pc + (d0 + e) * kTileRows) * f;
                         }
-                        if (valid) write(o, d0, ll > 0.0f ? 1.0f / ll : 0.0f);
+                        if (valid) write(o, d0, inv);
                     }
                 }
             }
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
+            __syncwarp();
         }
     }
     tc_fence_before();

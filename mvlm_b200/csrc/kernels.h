@@ -134,7 +134,7 @@ struct AttendArgs {
     int causal, window;
     int* status;
     float* partials;        // attend_scratch_bytes
-    unsigned int* tickets;  // two per CTA, zero between calls (the kernels leave them so)
+    unsigned int* tickets;  // eight per CTA, zero between calls (the kernels leave them so)
     // set by paged_attention
     int box_rows, page_shift, max_rows, q_pairs, out_pairs, q_vec, out_vec;
 };

@@ -106,7 +106,7 @@ bool is_quant_type(int t) { return t == MGPU_Q4_0 || t == MGPU_Q8_0; }
 size_t quant_row_bytes(int t, int64_t k) { return (size_t)((k + 31) / 32) * (t == MGPU_Q4_0 ? 18 : 34); }
 
 // Scratch arena layout: [0, 64 KB) holds the split-K tickets of gemv_kn, [64 KB, 128 KB) those of
-// the split-K GEMM and [128 KB, 132 KB) those of the paged attention's shares (two per CTA of a
+// the split-K GEMM and [128 KB, 136 KB) those of the paged attention's shares (eight per CTA of a
 // one-wave grid); all must stay zero between launches (the kernels reset them).
 // Everything from kScratchOffset on is free for per-call use (split-K partials, im2col
 // patches, staged operands), in stream order.
@@ -114,7 +114,7 @@ constexpr size_t kGemvTicketBytes = 64 * 1024;
 constexpr size_t kGemmTicketOffset = 64 * 1024;
 constexpr size_t kGemmTicketBytes = 64 * 1024;
 constexpr size_t kAttendTicketOffset = 128 * 1024;
-constexpr size_t kScratchOffset = 132 * 1024;
+constexpr size_t kScratchOffset = 136 * 1024;
 
 mgpu_k::LaunchCtx ctx_of(const mgpu_device* d) {
     mgpu_k::LaunchCtx c;
@@ -186,6 +186,9 @@ bool check_status(mgpu_device* d) {
     if (!cuda_ok(cudaMemcpy(&st, d->d_status, sizeof(int), cudaMemcpyDeviceToHost), "read status")) return false;
     if (st != 0) {
         cudaMemsetAsync(d->d_status, 0, sizeof(int), d->stream);
+        // CTAs that gave up have not counted themselves
+        if (st == MGPU_ERR_DEVICE_TIMEOUT && d->workspace_bytes >= kScratchOffset)
+            cudaMemsetAsync((char*)d->workspace + kAttendTicketOffset, 0, kScratchOffset - kAttendTicketOffset, d->stream);
         if (st == MGPU_ERR_INVALID_ARG)
             set_error(st, "a kernel skipped sequences whose lengths, pages or positions do not fit their buffers");
         else
@@ -1272,7 +1275,7 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch*
     a.page_size = c->page_size;
     a.scale_log2 = (float)((scale > 0.0f ? (double)scale : 1.0 / sqrt((double)c->head_dim)) * 1.4426950408889634);
     a.causal = causal != 0;
-    a.window = window;
+    a.window = std::min(window, 1 << 30);
     a.status = d->d_status;
     if (!ensure_workspace(d, kScratchOffset + mgpu_k::attend_scratch_bytes(d->sm_count, mgpu_k::attend_many_rows(a)))) return nullptr;
     a.tickets = (unsigned int*)((char*)d->workspace + kAttendTicketOffset);

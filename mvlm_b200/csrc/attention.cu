@@ -606,16 +606,16 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
 // ------------------------------------------------------------------ many rows -------
 // More than 16 rows to a key head (a chunk of a prompt): bound by the tensor cores' two products,
 // 4 D operations to a row and key, and by one exponential to a row and key.  A CTA takes two tiles of
-// up to 128 rows (whole tokens: 128 / G of them) over the same blocks of 128 keys.  One thread issues
-// S_t = Q_t K^T and O_t += P_t V of both tiles in turn, so that one tile's products run while the
-// other's softmax does; scores, weights and O stay in TMEM, weights in the place of half the scores.  Each
+// up to 128 rows (whole tokens: 128 / G of them) over the same blocks of 128 keys.  A warp to
+// each tile issues S_t = Q_t K^T and O_t += P_t V, so that one tile's products run while the other's
+// softmax does; scores, weights and O stay in TMEM, weights in the place of half the scores.  Each
 // tile has four warps, a thread to a row, which needs no exchange for its maximum and sum.  O is
 // rescaled only when a row's maximum has grown by more than 2^8 since its reference was taken: weights
 // stay below 2^8, and most blocks then leave O alone.  All blocks of all items (sequence, key head,
 // pair of tiles) are cut into equal shares as above; where whole items are few and short, a CTA takes
 // one item instead, which saves the join.
 constexpr int kTileKeys = 128, kTileRows = 128;
-constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, and two that look over V
+constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, products, scheduling
 constexpr int kTileSeqs = 1024;    // sequences of one launch
 constexpr int kTileEntries = 2048; // entries of the table of items
 constexpr int kJoinBlocks = 6;     // what a join costs, in blocks
@@ -624,6 +624,30 @@ constexpr float kGrowth = 8.0f;    // log2 of how far a weight may exceed 1
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
 // K on even and V on odd stages: two blocks of 128 dims, four of 64
 template <int DP> constexpr int tile_stages() { return 128 * 1024 / tile_stage_bytes<DP>(); }
+// mbar_wait for the waits of the loop between products and softmax: asks again at once, where
+// try_wait may put the warp to sleep and wake it some 300 clocks late.
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, int* status) {
+    const uint32_t addr = smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(addr), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((i & 1023u) == 1023u) {
+            const uint64_t t = globaltimer();
+            if (t0 == 0) t0 = t;
+            if (t - t0 > kWaitLimitNs) {
+                if (status) atomicExch(status, (int)MGPU_ERR_DEVICE_TIMEOUT);
+                return false;
+            }
+        }
+    }
+}
+
 template <int DP> constexpr int tile_smem() {
     return 1024 + 2 * kTileRows * DP * 2 + tile_stages<DP>() * tile_stage_bytes<DP>() + 4 * (kTileSeqs + 1 + kTileEntries + 1);
 }
@@ -742,7 +766,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t* ring = qs + 2 * QB;
     int* seq_first = reinterpret_cast<int*>(ring + S * SB);  // [n + 1] pairs before a sequence
     int* cum = seq_first + kTileSeqs + 1;                    // [entries + 1] blocks before an entry
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2], p_bar[2], o_bar[2], drain_bar,
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2], p_bar[2], o_bar[2], turn_bar[2], drain_bar,
         seg_full[kSegments], seg_empty[kSegments];
     __shared__ Segment segs[kSegments];
     __shared__ uint32_t tmem_slot;
@@ -753,7 +777,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (tid == 0) {
         for (int i = 0; i < S; ++i) {
             mbar_init(&full_bar[i], 1);
-            mbar_init(&empty_bar[i], 1);
+            mbar_init(&empty_bar[i], 2);  // both tiles' products
             mbar_init(&clean_bar[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
@@ -761,11 +785,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             mbar_init(&s_bar[t], 1);
             mbar_init(&p_bar[t], 4);
             mbar_init(&o_bar[t], 1);
+            mbar_init(&turn_bar[t], 1);
         }
-        mbar_init(&drain_bar, 1);
+        mbar_init(&drain_bar, 2);
         for (int i = 0; i < kSegments; ++i) {
             mbar_init(&seg_full[i], 1);
-            mbar_init(&seg_empty[i], 11);  // every other warp
+            mbar_init(&seg_empty[i], 11);  // all warps but the scheduling one
         }
         fence_mbar_init();
         prefetch_tensormap(&tmK);
@@ -852,12 +877,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, a.status)); };
+    auto poll = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_poll(bar, phase & 1u, a.status)); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         // Every warp below walks as one; only single instructions are one thread's.
+        bool ok = true, more = true;
+        uint32_t n = 0;  // blocks so far
         if (warp == 11) {
-            // ------------------------------------------------------------ scheduling
+            // ------------------------------------------------------------ scheduling, and NaN and Inf in V
             const int quota = total / shares, extra = total % shares;
             auto share = [&](int c) { return c * quota + min(c, extra); };
             const int cut = extra * (quota + 1);
@@ -879,22 +907,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 y -= cum[lo2];
                 for (p = lo2 * run, b = seq_of_pair(p);; ++p) {
                     while (seq_first[b + 1] <= p) ++b;
-                    const int n = pair_of(a, view(b), p - seq_first[b], per_tile).blocks;
-                    if (y < n) break;
-                    y -= n;
+                    const int blocks = pair_of(a, view(b), p - seq_first[b], per_tile).blocks;
+                    if (y < blocks) break;
+                    y -= blocks;
                 }
                 k = y;
             }
-            int end = by_item ? INT_MAX : share(blockIdx.x + 1);
-            int i = 0;
-            for (int pos = begin; pos < end; ++i) {
+            int end = by_item ? INT_MAX : share(blockIdx.x + 1), pos = begin, handed = 0;
+            auto hand_out = [&] {  // the next segment, if there is one
+                if (pos >= end) return;
                 const SeqView s = view(b);
                 const Pair pr = pair_of(a, s, p - seq_first[b], per_tile);
                 if (by_item) end = pr.blocks;
                 const int k1 = min(pr.blocks, k + (end - pos)), item = pos - k;
-                if (!wait(&seg_empty[i % kSegments], (i / kSegments) ^ 1)) break;
+                ok = wait(&seg_empty[handed % kSegments], (handed / kSegments) ^ 1);
+                if (!ok) return;
                 if (lane == 0) {
-                    Segment& g = segs[i % kSegments];
+                    Segment& g = segs[handed % kSegments];
                     g.kb0 = pr.lo + k;
                     g.kb1 = pr.lo + k1;
 #pragma unroll
@@ -920,9 +949,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                     g.more = pos + k1 - k < end;
                     g.odd = 0;
-                    mbar_arrive(&seg_full[i % kSegments]);
+                    mbar_arrive(&seg_full[handed % kSegments]);
                 }
                 __syncwarp();
+                ++handed;
                 pos += k1 - k;
                 k = 0;
                 if (++p == pairs) {
@@ -932,170 +962,155 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 if (pos < end)
                     while (seq_first[b + 1] <= p) ++b;
+            };
+            hand_out();
+            for (int i = 0; ok && more; ++i) {
+                hand_out();  // one ahead of the values looked over below
+                if (!ok) break;
+                Segment& g = segs[i % kSegments];
+                more = g.more;
+                // A weight of 0 times NaN or Inf is not 0: where some row does not see all keys of a block,
+                // such values leave the block, and the rows that see them add them at the end.
+                const int kb1 = g.kb1;
+                for (int kb = g.kb0; ok && kb < kb1; ++kb, ++n) {
+                    const uint32_t st = (2 * n + 1) % S;
+                    ok = wait(&full_bar[st], (2 * n + 1) / S);
+                    if (!ok) break;
+                    if (g.masked(kb)) {
+                        uint4* v = reinterpret_cast<uint4*>(ring + st * SB);
+                        bool found = false;
+#pragma unroll 8
+                        for (int x = lane; x < SB / 16; x += 32) {
+                            const uint4 q = v[x];
+                            found |= odd16(q.x, kBf16) || odd16(q.x >> 16, kBf16) || odd16(q.y, kBf16) || odd16(q.y >> 16, kBf16) ||
+                                     odd16(q.z, kBf16) || odd16(q.z >> 16, kBf16) || odd16(q.w, kBf16) || odd16(q.w >> 16, kBf16);
+                        }
+                        if (__any_sync(0xffffffffu, found)) {
+                            for (int x = lane; x < SB / 2; x += 32) {
+                                uint16_t* u = reinterpret_cast<uint16_t*>(v) + x;
+                                if (odd16(*u, kBf16)) *u = 0;
+                            }
+                            if (lane == 0) g.odd = 1;
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                    }
+                    if (lane == 0) mbar_arrive(&clean_bar[st]);
+                    __syncwarp();
+                }
             }
-        } else {
-            uint32_t n = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};  // n: blocks so far
-            // Descriptors of tile 0's Q, of stage 0 as keys and as values; steps and stages are added to
-            // their address fields, in units of 16 bytes.  The fewer instructions between two products,
-            // the less the tensor cores wait.
-            const uint64_t q_desc = smem_desc(smem_u32(qs), 16, 1024, kSwizzle128B);
-            const uint64_t k_desc = smem_desc(smem_u32(ring), 16, 1024, kSwizzle128B);
-            const uint64_t v_desc = smem_desc(smem_u32(ring), SLAB, 1024, kSwizzle128B);
-            const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys);
-            const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
-            const int dims = (a.D + 15) / 16;
-            const int rows = a.box_rows, chunks = kTileKeys / rows;  // loads: a lane has a chunk of one page
-            bool ok = true, more = true;
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ loads: a lane has a chunk of one page
+            const int rows = a.box_rows, chunks = kTileKeys / rows;
             for (int i = 0; ok && more; ++i) {
                 ok = wait(&seg_full[i % kSegments], i / kSegments);
                 if (!ok) break;
                 const Segment& g = segs[i % kSegments];
                 more = g.more;
-                const int kb0 = g.kb0, kb1 = g.kb1;
-                if (warp == 8) {
-                    // -------------------------------------------------------- products
-                    bool started[2] = {false, false}, has_o[2] = {false, false};
-                    auto score = [&](const int t, uint32_t stage) {
-                        if (!started[t]) {
-                            ok = wait(&q_bar[t], q_phase[t]++);
-                            if (!ok) return;
-                            started[t] = true;
-                        }
-                        tc_fence_after();
-                        if (elect_one()) {
-                            const uint64_t qd = q_desc + t * (QB >> 4), kd = k_desc + stage * (SB >> 4);
-#pragma unroll
-                            for (int d = 0; d < DP / 16; ++d) {
-                                const int step = (d >> 2) * (SLAB >> 4) + (d & 3) * 2;  // Q and K have the same slabs
-                                if (d < dims) umma_f16(tmem + t * kTileKeys, qd + step, kd + step, id_s, d != 0);
-                            }
-                            umma_commit(&s_bar[t]);
-                        }
-                        __syncwarp();
-                    };
-                    auto release = [&](uint32_t stage) {
-                        if (elect_one()) umma_commit(&empty_bar[stage]);
-                        __syncwarp();
-                    };
-                    for (int kb = kb0; ok && kb < kb1; ++kb, ++n) {
-                        const uint32_t ks = (2 * n) % S, vs = (2 * n + 1) % S, kn = (2 * n + 2) % S;
-                        const bool last = kb + 1 == kb1;
-                        if (kb == kb0) {
-                            ok = wait(&full_bar[ks], 2 * n / S);
-#pragma unroll
-                            for (int t = 0; t < 2; ++t)
-                                if (ok && g.in(t, kb)) score(t, ks);
-                            release(ks);
-                        }
-                        ok = ok && wait(&full_bar[vs], (2 * n + 1) / S);
-                        ok = ok && wait(&clean_bar[vs], (2 * n + 1) / S);
-                        bool have_next = false;
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            if (ok && g.in(t, kb)) {
-                                ok = wait(&p_bar[t], p_phase[t]++);
-                                if (!ok) break;
-                                tc_fence_after();
-                                if (elect_one()) {
-                                    const uint64_t vd = v_desc + vs * (SB >> 4);
-#pragma unroll
-                                    for (int d = 0; d < kTileKeys / 16; ++d)
-                                        umma_f16_ts(tmem + 256 + t * 128, tmem + t * kTileKeys + 64 + d * 8, vd + d * (2048 >> 4), id_o,
-                                                    has_o[t] || d != 0);
-                                    if (last || !g.in(t, kb + 1)) umma_commit(&o_bar[t]);
-                                }
-                                __syncwarp();
-                                has_o[t] = true;
-                            }
-                            if (ok && !last && g.in(t, kb + 1)) {
-                                if (!have_next) ok = wait(&full_bar[kn], (2 * n + 2) / S);
-                                have_next = true;
-                                if (ok) score(t, kn);
-                            }
-                        }
-                        if (!ok) break;
-                        release(vs);
-                        if (!last) {
-                            // a block that no tile takes still has to arrive before its stage is given back
-                            if (!have_next) ok = wait(&full_bar[kn], (2 * n + 2) / S);
-                            release(kn);
+                const int kb1 = g.kb1;
+                for (int kb = g.kb0; ok && kb < kb1; ++kb, ++n) {
+                    const int j = kb * kTileKeys + lane * rows;
+                    // chunks past the end are read from outside the map, which gives zeros
+                    int z = a.num_pages * a.hkv, y = 0;
+                    if (lane < chunks && j < g.kv) {
+                        const int at = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+                        const int page = a.batch.page_table[(int64_t)g.seq * a.batch.max_pages + at];
+                        if (page >= 0 && page < a.num_pages) {
+                            z = page * a.hkv + g.h;
+                            y = j - at * a.page_size;
+                        } else {
+                            atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
                         }
                     }
-                } else if (warp == 9) {
-                    // -------------------------------------------------------- loads
-                    for (int kb = kb0; ok && kb < kb1; ++kb, ++n) {
-                        const int j = kb * kTileKeys + lane * rows;
-                        // chunks past the end are read from outside the map, which gives zeros
-                        int z = a.num_pages * a.hkv, y = 0;
-                        if (lane < chunks && j < g.kv) {
-                            const int at = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
-                            const int page = a.batch.page_table[(int64_t)g.seq * a.batch.max_pages + at];
-                            if (page >= 0 && page < a.num_pages) {
-                                z = page * a.hkv + g.h;
-                                y = j - at * a.page_size;
-                            } else {
-                                atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-                            }
-                        }
 #pragma unroll
-                        for (int side = 0; side < 2; ++side) {
-                            const uint32_t it = 2 * n + side, st = it % S;
-                            if (!ok) break;
-                            ok = wait(&empty_bar[st], (it / S) ^ 1);
-                            if (!ok) break;
-                            if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB);
-                            __syncwarp();
-                            if (lane < chunks) {
-#pragma unroll
-                                for (int slab = 0; slab < SLABS; ++slab)
-                                    tma_load_3d(ring + st * SB + slab * SLAB + lane * rows * 128, side ? &tmV : &tmK, slab * 64, y, z,
-                                                &full_bar[st]);
-                            }
-                            __syncwarp();
-                        }
-                    }
-                } else {
-                    // -------------------------------------------------------- NaN and Inf in V
-                    // A weight of 0 times NaN or Inf is not 0: where some row does not see all keys of a
-                    // block, such values leave the block, and the rows that see them add them at the end.
-                    for (int kb = kb0; ok && kb < kb1; ++kb, ++n) {
-                        const uint32_t st = (2 * n + 1) % S;
-                        ok = wait(&full_bar[st], (2 * n + 1) / S);
+                    for (int side = 0; side < 2; ++side) {
+                        const uint32_t it = 2 * n + side, st = it % S;
                         if (!ok) break;
-                        if (g.masked(kb)) {
-                            uint4* v = reinterpret_cast<uint4*>(ring + st * SB);
-                            bool found = false;
-#pragma unroll 8
-                            for (int x = lane; x < SB / 16; x += 32) {
-                                const uint4 q = v[x];
-                                found |= odd16(q.x, kBf16) || odd16(q.x >> 16, kBf16) || odd16(q.y, kBf16) || odd16(q.y >> 16, kBf16) ||
-                                         odd16(q.z, kBf16) || odd16(q.z >> 16, kBf16) || odd16(q.w, kBf16) || odd16(q.w >> 16, kBf16);
-                            }
-                            if (__any_sync(0xffffffffu, found)) {
-                                for (int x = lane; x < SB / 2; x += 32) {
-                                    uint16_t* u = reinterpret_cast<uint16_t*>(v) + x;
-                                    if (odd16(*u, kBf16)) *u = 0;
-                                }
-                                if (lane == 0) segs[i % kSegments].odd = 1;
-                                fence_proxy_async_smem();
-                                __syncwarp();
-                            }
+                        ok = wait(&empty_bar[st], (it / S) ^ 1);
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB);
+                        __syncwarp();
+                        if (lane < chunks) {
+#pragma unroll
+                            for (int slab = 0; slab < SLABS; ++slab)
+                                tma_load_3d(ring + st * SB + slab * SLAB + lane * rows * 128, side ? &tmV : &tmK, slab * 64, y, z,
+                                            &full_bar[st]);
                         }
-                        if (lane == 0) mbar_arrive(&clean_bar[st]);
                         __syncwarp();
                     }
                 }
-                __syncwarp();
                 if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
-            }
-            if (warp == 8) {
-                if (elect_one()) umma_commit(&drain_bar);  // all products have ended before TMEM is given back
                 __syncwarp();
-                wait(&drain_bar, 0);
-            } else if (warp == 9 && !ok) {
-                // a wait ran out: the copies under way still have to land before the CTA may end
-                for (uint32_t it = n > S ? 2 * n - S : 0; it < 2 * n; ++it) wait(&full_bar[it % S], it / S);
             }
+            // a wait ran out: the copies under way still have to land before the CTA may end
+            if (!ok)
+                for (uint32_t it = 2 * n > S ? 2 * n - S : 0; it < 2 * n; ++it) wait(&full_bar[it % S], it / S);
+        } else {
+            // ------------------------------------------------------------ products: a warp to a tile
+            // Descriptors of the tile's Q, of stage 0 as keys and as values; steps and stages are added to
+            // their address fields, in units of 16 bytes.  All waits but the one for the weights come before
+            // it: from there to the commit of the next scores is what the tile's softmax waits for.  The
+            // tiles take turns: left alone they fall into step, and then products and softmax alternate
+            // instead of running side by side.
+            const int t = warp == 8 ? 0 : 1;
+            uint32_t q_phase = 0, p_phase = 0, turn = 0;
+            const uint64_t q_desc = smem_desc(smem_u32(qs + t * QB), 16, 1024, kSwizzle128B);
+            const uint64_t k_desc = smem_desc(smem_u32(ring), 16, 1024, kSwizzle128B);
+            const uint64_t v_desc = smem_desc(smem_u32(ring), SLAB, 1024, kSwizzle128B);
+            const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys);
+            const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
+            const uint32_t d_s = tmem + t * kTileKeys, d_p = d_s + 64, d_o = tmem + 256 + t * 128;
+            const int dims = (a.D + 15) / 16;
+            for (int i = 0; ok && more; ++i) {
+                ok = wait(&seg_full[i % kSegments], i / kSegments);
+                if (!ok) break;
+                const Segment& g = segs[i % kSegments];
+                more = g.more;
+                const int kb0 = g.kb0, kb1 = g.kb1, lo = g.lo[t], hi = g.hi[t];
+                // kb0 - 1 stands for the scores of the first block alone
+                for (int kb = kb0 - 1; kb < kb1; ++kb) {
+                    const uint32_t ks = (2 * n) % S, vs = (2 * n + S - 1) % S;  // keys of kb + 1, values of kb
+                    const bool scores = kb + 1 < kb1, score = scores && kb + 1 >= lo && kb + 1 < hi, weigh = kb >= lo && kb < hi;
+                    if (scores) ok = wait(&full_bar[ks], 2 * n / S);
+                    if (kb >= kb0) {
+                        ok = ok && wait(&full_bar[vs], (2 * n - 1) / S);
+                        ok = ok && wait(&clean_bar[vs], (2 * n - 1) / S);
+                    }
+                    if (score && kb + 1 == lo) ok = ok && wait(&q_bar[t], q_phase++);
+                    if (weigh) ok = ok && poll(&p_bar[t], p_phase++);
+                    ok = ok && poll(&turn_bar[t], turn++ ^ (t == 0));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (weigh) {
+                            const uint64_t vd = v_desc + vs * (SB >> 4);
+#pragma unroll
+                            for (int d = 0; d < kTileKeys / 16; ++d)
+                                umma_f16_ts(d_o, d_p + d * 8, vd + d * (2048 >> 4), id_o, kb > lo || d != 0);
+                            if (kb + 1 >= hi || !scores) umma_commit(&o_bar[t]);
+                        }
+                        if (score) {
+                            const uint64_t kd = k_desc + ks * (SB >> 4);
+#pragma unroll
+                            for (int d = 0; d < DP / 16; ++d) {
+                                const int step = (d >> 2) * (SLAB >> 4) + (d & 3) * 2;  // Q and K have the same slabs
+                                if (d < dims) umma_f16(d_s, q_desc + step, kd + step, id_s, d != 0);
+                            }
+                            umma_commit(&s_bar[t]);
+                        }
+                        mbar_arrive(&turn_bar[1 - t]);
+                        if (kb >= kb0) umma_commit(&empty_bar[vs]);
+                        if (scores) umma_commit(&empty_bar[ks]);
+                    }
+                    __syncwarp();
+                    if (scores) ++n;
+                }
+                if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
+                __syncwarp();
+            }
+            if (elect_one()) umma_commit(&drain_bar);  // all products have ended before TMEM is given back
+            __syncwarp();
+            wait(&drain_bar, 0);
         }
     } else {
         // ---------------------------------------------------------------- softmax: a thread to a row
@@ -1106,25 +1121,34 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // this warp's 32 rows of Q into the swizzled slabs, zeros beyond the tile's rows and the head's dims
         auto stage_q = [&](const Segment& g) {
             if (g.lo[t] >= g.hi[t]) return;
-            constexpr int PER = DP / 8;  // 16-byte chunks of a row
-            uint8_t* dst = qs + t * QB;
-#pragma unroll 4
-            for (int x = lane; x < 32 * PER; x += 32) {
-                const int r = (warp & 3) * 32 + x / PER, c = x % PER;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < g.rows[t] && c * 8 < a.D) {
-                    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(g.row0[t] + r / G) * a.ldq +
-                                        (int64_t)(g.h * G + r % G) * a.D + c * 8;
-                    if (a.q_vec) {
-                        v = *reinterpret_cast<const uint4*>(q);
-                    } else {
-                        uint32_t w[4];
+            constexpr int PER = DP / 8, AT_ONCE = 8, ROWS = 32 / PER;  // 16-byte chunks of a row; rows of one access
+            const int c = lane % PER, r0 = (warp & 3) * 32 + lane / PER, rows = g.rows[t];
+            uint8_t* dst = qs + t * QB + (c >> 3) * SLAB;
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)g.row0[t] * a.ldq + (int64_t)g.h * G * a.D + c * 8;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)q[2 * e] | ((uint32_t)q[2 * e + 1] << 16);
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int x = 0; x < 32; x += ROWS * AT_ONCE) {
+                uint4 v[AT_ONCE];
+#pragma unroll
+                for (int e = 0; e < AT_ONCE; ++e) {
+                    const int r = r0 + x + ROWS * e, token = r / G;
+                    v[e] = make_uint4(0, 0, 0, 0);
+                    if (r < rows && c * 8 < a.D) {
+                        const uint16_t* at = q + (int64_t)token * a.ldq + (r - token * G) * a.D;
+                        if (a.q_vec) {
+                            v[e] = *reinterpret_cast<const uint4*>(at);
+                        } else {
+                            v[e].x = (uint32_t)at[0] | ((uint32_t)at[1] << 16);
+                            v[e].y = (uint32_t)at[2] | ((uint32_t)at[3] << 16);
+                            v[e].z = (uint32_t)at[4] | ((uint32_t)at[5] << 16);
+                            v[e].w = (uint32_t)at[6] | ((uint32_t)at[7] << 16);
+                        }
                     }
                 }
-                *reinterpret_cast<uint4*>(dst + (c >> 3) * SLAB + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+                for (int e = 0; e < AT_ONCE; ++e) {
+                    const int r = r0 + x + ROWS * e;
+                    *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[e];
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -1141,7 +1165,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const Seen sr = valid ? seen_at(a, g.kv, g.index[t] + row / G) : Seen{0, 0};
             float m = -INFINITY, l = 0.0f;  // the reference (log2 units) and the sum of 2^(s - m)
             for (int kb = kb0; kb < kb1; ++kb) {
-                ok = wait(&s_bar[t], s_phase++);
+                ok = poll(&s_bar[t], s_phase++);
                 if (!ok) break;
                 tc_fence_after();
                 // The scores are read twice in part: all 128 and the state beside them do not fit the
@@ -1279,21 +1303,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
             };
+            T* const out_row = reinterpret_cast<T*>(a.out) + (int64_t)(g.row0[t] + row / G) * a.ldo + (int64_t)(g.h * G + row % G) * a.D;
             auto write = [&](const float (&o)[32], int d0, float inv) {
-                T* out = reinterpret_cast<T*>(a.out) + (int64_t)(g.row0[t] + row / G) * a.ldo + (int64_t)(g.h * G + row % G) * a.D + d0;
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    if (d0 + e >= a.D) break;
-                    if (a.out_vec) {
-                        uint4 v;
-                        v.x = pack2<T>(o[e] * inv, o[e + 1] * inv);
-                        v.y = pack2<T>(o[e + 2] * inv, o[e + 3] * inv);
-                        v.z = pack2<T>(o[e + 4] * inv, o[e + 5] * inv);
-                        v.w = pack2<T>(o[e + 6] * inv, o[e + 7] * inv);
-                        *reinterpret_cast<uint4*>(out + e) = v;
-                    } else {
+                for (int e = 0; e < 32; e += 16) {
+                    uint32_t w[8];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) out[e + x] = from_f32<T>(o[e + x] * inv);
+                    for (int x = 0; x < 8; ++x) w[x] = pack2<T>(o[e + 2 * x] * inv, o[e + 2 * x + 1] * inv);
+                    if (a.out_wide && d0 + e + 16 <= a.D) {
+                        // a whole 32-byte sector to a thread
+                        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out_row + d0 + e), "r"(w[0]), "r"(w[1]),
+                                     "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                                     : "memory");
+                        continue;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 16; x += 8) {
+                        if (d0 + e + x >= a.D) break;
+                        T* out = out_row + d0 + e + x;
+                        if (a.out_vec) {
+                            *reinterpret_cast<uint4*>(out) = make_uint4(w[x / 2], w[x / 2 + 1], w[x / 2 + 2], w[x / 2 + 3]);
+                        } else {
+#pragma unroll
+                            for (int y = 0; y < 8; ++y) out[y] = from_f32<T>(o[e + x + y] * inv);
+                        }
                     }
                 }
             };
@@ -1423,6 +1456,7 @@ cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUt
         if (a.page_size == 1 << i) a.page_shift = i;
     a.q_vec = ((uintptr_t)a.q & 15) == 0 && a.ldq % 8 == 0;
     a.out_vec = ((uintptr_t)a.out & 15) == 0 && a.ldo % 8 == 0;
+    a.out_wide = ((uintptr_t)a.out & 31) == 0 && a.ldo % 16 == 0 && a.D % 16 == 0;
     a.q_pairs = ((uintptr_t)a.q & 3) == 0 && a.ldq % 2 == 0;
     a.out_pairs = ((uintptr_t)a.out & 3) == 0 && a.ldo % 2 == 0;
     return a.type == MGPU_F16 ? launch_attend<__half>(c, mk, mv, a) : launch_attend<__nv_bfloat16>(c, mk, mv, a);

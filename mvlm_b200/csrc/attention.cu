@@ -48,6 +48,32 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// 2^z for two values on the FMA pipe: z = n + f with n the nearest integer, a polynomial in f on
+// [-1/2, 1/2] (least largest relative error; 2^-13.7 of degree 3, 2^-18.5 of degree 4, each below
+// the rounding of the weight that follows, 2^-9 of bf16 and 2^-12 of fp16), n added to the exponent.
+// Below 2^-126 it is 0, as ex2 has it.
+template <typename T> __device__ __forceinline__ float2 ex2_poly(float2 z) {
+    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are n
+    const float2 zc = make_float2(fmaxf(z.x, -126.0f), fmaxf(z.y, -126.0f));
+    const float2 t = __fadd2_rn(zc, make_float2(kRound, kRound));
+    const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
+    const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), zc);
+    float2 p;
+    if constexpr (std::is_same<T, __half>::value) {
+        p = __ffma2_rn(make_float2(9.5700979e-3f, 9.5700979e-3f), f, make_float2(5.5917859e-2f, 5.5917859e-2f));
+        p = __ffma2_rn(p, f, make_float2(2.4024744e-1f, 2.4024744e-1f));
+        p = __ffma2_rn(p, f, make_float2(6.9312179e-1f, 6.9312179e-1f));
+        p = __ffma2_rn(p, f, make_float2(9.9999928e-1f, 9.9999928e-1f));
+    } else {
+        p = __ffma2_rn(make_float2(5.5171665e-2f, 5.5171665e-2f), f, make_float2(2.4261113e-1f, 2.4261113e-1f));
+        p = __ffma2_rn(p, f, make_float2(6.9326097e-1f, 6.9326097e-1f));
+        p = __ffma2_rn(p, f, make_float2(9.9992806e-1f, 9.9992806e-1f));
+    }
+    const float x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+    const float y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+    return make_float2(z.x < -126.0f ? 0.0f : x, z.y < -126.0f ? 0.0f : y);
+}
+
 // ------------------------------------------------------------------ tensor cores ----
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -619,6 +645,7 @@ constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, pr
 constexpr int kTileSeqs = 1024;    // sequences of one launch
 constexpr int kTileEntries = 2048; // entries of the table of items
 constexpr int kJoinBlocks = 6;     // what a join costs, in blocks
+constexpr int kPoly = 4;
 constexpr float kGrowth = 8.0f;    // log2 of how far a weight may exceed 1
 
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
@@ -766,7 +793,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t* ring = qs + 2 * QB;
     int* seq_first = reinterpret_cast<int*>(ring + S * SB);  // [n + 1] pairs before a sequence
     int* cum = seq_first + kTileSeqs + 1;                    // [entries + 1] blocks before an entry
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2], p_bar[2], o_bar[2], turn_bar[2], drain_bar,
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2], p_bar[2][2], o_bar[2], turn_bar[2], drain_bar,
         seg_full[kSegments], seg_empty[kSegments];
     __shared__ Segment segs[kSegments];
     __shared__ uint32_t tmem_slot;
@@ -783,7 +810,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_bar[t], 4);
             mbar_init(&s_bar[t], 1);
-            mbar_init(&p_bar[t], 4);
+            mbar_init(&p_bar[t][0], 4);
+            mbar_init(&p_bar[t][1], 4);
             mbar_init(&o_bar[t], 1);
             mbar_init(&turn_bar[t], 1);
         }
@@ -905,7 +933,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     else hi2 = mid;
                 }
                 y -= cum[lo2];
-                for (p = lo2 * run, b = seq_of_pair(p);; ++p) {
+                for (p = lo2 * run, b = seq_of_pair(p); run > 1; ++p) {
                     while (seq_first[b + 1] <= p) ++b;
                     const int blocks = pair_of(a, view(b), p - seq_first[b], per_tile).blocks;
                     if (y < blocks) break;
@@ -963,10 +991,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (pos < end)
                     while (seq_first[b + 1] <= p) ++b;
             };
-            hand_out();
-            for (int i = 0; ok && more; ++i) {
+            for (int i = -1; ok && more; ++i) {
                 hand_out();  // one ahead of the values looked over below
                 if (!ok) break;
+                if (i < 0) continue;
                 Segment& g = segs[i % kSegments];
                 more = g.more;
                 // A weight of 0 times NaN or Inf is not 0: where some row does not see all keys of a block,
@@ -1077,18 +1105,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         ok = ok && wait(&clean_bar[vs], (2 * n - 1) / S);
                     }
                     if (score && kb + 1 == lo) ok = ok && wait(&q_bar[t], q_phase++);
-                    if (weigh) ok = ok && poll(&p_bar[t], p_phase++);
                     ok = ok && poll(&turn_bar[t], turn++ ^ (t == 0));
+                    const uint64_t vd = v_desc + vs * (SB >> 4);
+                    // the upper half of the keys has its weights first
+#pragma unroll 1
+                    for (int half = 1; weigh && half >= 0; --half) {
+                        ok = ok && poll(&p_bar[t][half], p_phase);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int d = 0; d < kTileKeys / 32; ++d) {
+                                const int step = d + half * (kTileKeys / 32);
+                                umma_f16_ts(d_o, d_p + step * 8, vd + step * (2048 >> 4), id_o, kb > lo || half == 0 || d != 0);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    p_phase ^= weigh;
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        if (weigh) {
-                            const uint64_t vd = v_desc + vs * (SB >> 4);
-#pragma unroll
-                            for (int d = 0; d < kTileKeys / 16; ++d)
-                                umma_f16_ts(d_o, d_p + d * 8, vd + d * (2048 >> 4), id_o, kb > lo || d != 0);
-                            if (kb + 1 >= hi || !scores) umma_commit(&o_bar[t]);
-                        }
+                        if (weigh && (kb + 1 >= hi || !scores)) umma_commit(&o_bar[t]);
                         if (score) {
                             const uint64_t kd = k_desc + ks * (SB >> 4);
 #pragma unroll
@@ -1121,35 +1159,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // this warp's 32 rows of Q into the swizzled slabs, zeros beyond the tile's rows and the head's dims
         auto stage_q = [&](const Segment& g) {
             if (g.lo[t] >= g.hi[t]) return;
-            constexpr int PER = DP / 8, AT_ONCE = 8, ROWS = 32 / PER;  // 16-byte chunks of a row; rows of one access
-            const int c = lane % PER, r0 = (warp & 3) * 32 + lane / PER, rows = g.rows[t];
-            uint8_t* dst = qs + t * QB + (c >> 3) * SLAB;
+            constexpr int PER = DP / 8, ROWS = 32 / PER;  // 16-byte chunks of a row; rows of one access
+            const int c = lane % PER, rows = g.rows[t];
+            const uint32_t dst = smem_u32(qs + t * QB + (c >> 3) * SLAB);
             const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)g.row0[t] * a.ldq + (int64_t)g.h * G * a.D + c * 8;
+            int r = (warp & 3) * 32 + lane / PER, token = r / G, head = r % G;
+            // A short loop of asynchronous copies: unrolled loads would wait for their instructions longer
+            // than for their data, as this is run once a segment.
+#pragma unroll 1
+            for (int x = 0; x < 32; x += ROWS) {
+                const bool in = r < rows && c * 8 < a.D;
+                const uint16_t* at = in ? q + (int64_t)token * a.ldq + head * a.D : reinterpret_cast<const uint16_t*>(a.q);
+                const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                if (a.q_vec) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(in ? 16 : 0) : "memory");
+                } else {
+                    uint32_t w[4] = {0, 0, 0, 0};
+                    if (in)
 #pragma unroll
-            for (int x = 0; x < 32; x += ROWS * AT_ONCE) {
-                uint4 v[AT_ONCE];
-#pragma unroll
-                for (int e = 0; e < AT_ONCE; ++e) {
-                    const int r = r0 + x + ROWS * e, token = r / G;
-                    v[e] = make_uint4(0, 0, 0, 0);
-                    if (r < rows && c * 8 < a.D) {
-                        const uint16_t* at = q + (int64_t)token * a.ldq + (r - token * G) * a.D;
-                        if (a.q_vec) {
-                            v[e] = *reinterpret_cast<const uint4*>(at);
-                        } else {
-                            v[e].x = (uint32_t)at[0] | ((uint32_t)at[1] << 16);
-                            v[e].y = (uint32_t)at[2] | ((uint32_t)at[3] << 16);
-                            v[e].z = (uint32_t)at[4] | ((uint32_t)at[5] << 16);
-                            v[e].w = (uint32_t)at[6] | ((uint32_t)at[7] << 16);
-                        }
-                    }
+                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)at[2 * e] | ((uint32_t)at[2 * e + 1] << 16);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                 }
-#pragma unroll
-                for (int e = 0; e < AT_ONCE; ++e) {
-                    const int r = r0 + x + ROWS * e;
-                    *reinterpret_cast<uint4*>(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[e];
+                r += ROWS;
+                head += ROWS;
+                while (head >= G) {
+                    head -= G;
+                    ++token;
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_bar[t]);
@@ -1236,11 +1274,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, neg2);
-                        const float2 w2 = make_float2(ex2(z.x), ex2(z.y));
+                        // the exponential unit takes 4 values a clock and quarter of an SM, two tiles' 256 a row more
+                        // than the products take: every kPoly-th pair goes to the FMA pipe
+                        const float2 w2 = e % kPoly == kPoly - 1 ? ex2_poly<T>(z) : make_float2(ex2(z.x), ex2(z.y));
                         sum = __fadd2_rn(sum, w2);
                         w[e] = pack2<T>(w2.x, w2.y);
                     }
                     tmem_st16(s_tm + 64 + at / 2, w);
+                };
+                auto given = [&](int half) {  // the weights of half the keys are in place
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_bar[t][half]);
+                    __syncwarp();
                 };
                 uint32_t sc[32];
                 tmem_ld32(s_tm, sc);
@@ -1250,17 +1297,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mask(sc, 0);
                 tmem_ld32(s_tm + 32, sa);
                 weigh(sb, 96);
+                given(1);
                 weigh(sc, 0);
                 tmem_ld_wait();
                 tmem_use(sa);
                 mask(sa, 32);
                 weigh(sa, 32);
+                given(0);
                 l += sum.x + sum.y;
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_bar[t]);
-                __syncwarp();
             }
             if (!ok) break;
             const bool took = kb0 < kb1;
@@ -1423,7 +1467,8 @@ cudaError_t launch_tiles(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, cons
 
 template <typename T>
 cudaError_t launch_attend(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const mgpu_k::AttendArgs& a) {
-    cudaError_t e = a.D <= 64 ? launch_rows<T, 64>(c, mk, mv, a) : launch_rows<T, 128>(c, mk, mv, a);
+    cudaError_t e = cudaSuccess;
+    if (a.max_rows > 0) e = a.D <= 64 ? launch_rows<T, 64>(c, mk, mv, a) : launch_rows<T, 128>(c, mk, mv, a);
     if (e != cudaSuccess || !mgpu_k::attend_many_rows(a)) return e;
     return a.D <= 64 ? launch_tiles<T, 64>(c, mk, mv, a) : launch_tiles<T, 128>(c, mk, mv, a);
 }
@@ -1450,7 +1495,8 @@ cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUt
     AttendArgs a = in;
     a.box_rows = kBlock;
     while (a.page_size % a.box_rows) a.box_rows /= 2;
-    a.max_rows = kRowsMax;
+    // one sequence of a chunk: the kernel for many rows alone, however few it turns out to have
+    a.max_rows = a.batch.n_seqs == 1 && attend_many_rows(a) ? 0 : kRowsMax;
     a.page_shift = -1;
     for (int i = 3; i < 31; ++i)
         if (a.page_size == 1 << i) a.page_shift = i;

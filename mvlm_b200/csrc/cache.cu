@@ -5,6 +5,8 @@
 // (dispatch_rope_apply and kv_cache_append, src/models/moondream2.cpp:406-420): three passes over
 // the activations.  Here each value is read once and written once: the bound is
 // T (Hq + 2 Hkv) D (source + cache bytes) at HBM rate.
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.cuh"
@@ -26,142 +28,217 @@ __global__ void rope_table_kernel(float2* __restrict__ table, int64_t n, int pai
     }
 }
 
-// VEC consecutive values at p[i], of a type known at run time.
-template <int VEC>
-__device__ __forceinline__ void load_vec(const void* p, int type, int64_t i, float (&o)[VEC]) {
-    if constexpr (VEC == 8) {
-        if (type == MGPU_F32) {
-            const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
-            const float4 a = q[0], b = q[1];
-            o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w; o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
-            return;
-        }
-        const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 f = type == MGPU_F16 ? unpack2<__half>(w[k]) : unpack2<__nv_bfloat16>(w[k]);
-            o[2 * k] = f.x;
-            o[2 * k + 1] = f.y;
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) o[k] = load_float(p, type, (size_t)(i + k));
-    }
-}
-template <int VEC>
-__device__ __forceinline__ void store_vec(void* p, int type, int64_t i, const float (&v)[VEC]) {
-    if constexpr (VEC == 8) {
-        if (type == MGPU_F32) {
-            float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
-            q[0] = make_float4(v[0], v[1], v[2], v[3]);
-            q[1] = make_float4(v[4], v[5], v[6], v[7]);
-            return;
-        }
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            w[k] = type == MGPU_F16 ? pack2<__half>(v[2 * k], v[2 * k + 1]) : pack2<__nv_bfloat16>(v[2 * k], v[2 * k + 1]);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            if (type == MGPU_F32) reinterpret_cast<float*>(p)[i + k] = v[k];
-            else if (type == MGPU_F16) reinterpret_cast<__half*>(p)[i + k] = from_f32<__half>(v[k]);
-            else reinterpret_cast<__nv_bfloat16*>(p)[i + k] = from_f32<__nv_bfloat16>(v[k]);
-        }
-    }
-}
-
-// One CTA per (token, share of its heads).  A head is cut into units, one per thread: a unit of
-// the rotated part holds whole pairs (VEC dims and their partners rot/2 further on, or, with
-// adjacent pairs, VEC dims that are their own partners), a unit of the rest VEC dims.  A thread
-// keeps its unit over all its heads, so the angles are read once per token and thread.
-template <int VEC, bool ADJ>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const mgpu_k::AppendArgs a) {
-    constexpr int PW = ADJ ? (VEC == 1 ? 2 : VEC) : VEC;  // dims of the first (or only) vector of a pair unit
-    constexpr int NP = ADJ ? PW / 2 : VEC;                // pairs of a unit
-    const int t = blockIdx.x;
+// Where token t of a step goes and by what angles it turns; false where it goes nowhere.  Every warp
+// of the CTA calls it with the same t.
+struct Place {
+    int64_t slot;  // first element of its place in key head 0 of its page
+    int pos[3];
+};
+__device__ __forceinline__ bool place_of(const mgpu_k::AppendArgs& a, int t, Place& p) {
     const int seq = seq_of_token(a.batch, t);
-    if (seq < 0) return;
+    if (seq < 0) return false;
     const int q0 = a.batch.cu_q[seq], q1 = a.batch.cu_q[seq + 1];
     const int index = a.batch.kv_lens[seq] - (q1 - t);  // of this token in its sequence
     int page = -1;
     if (index >= 0 && index / a.page_size < a.batch.max_pages)
         page = a.batch.page_table[(int64_t)seq * a.batch.max_pages + index / a.page_size];
     bool bad = page < 0 || page >= a.num_pages || q1 > a.batch.n_tokens || q1 - q0 > a.batch.max_q_len;
-    int pos[3] = {index, index, index};
-    if (a.table) {
 #pragma unroll
-        for (int x = 0; x < 3; ++x) {
-            if (x >= a.n_axes) break;
-            if (a.positions) pos[x] = a.positions[(int64_t)x * a.batch.n_tokens + t];
-            bad |= pos[x] < 0 || pos[x] >= a.max_pos;
+    for (int x = 0; x < 3; ++x) {
+        p.pos[x] = index;
+        if (a.table && x < a.n_axes) {
+            if (a.positions) p.pos[x] = a.positions[(int64_t)x * a.batch.n_tokens + t];
+            bad |= p.pos[x] < 0 || p.pos[x] >= a.max_pos;
         }
     }
     if (bad) {
         if (threadIdx.x == 0) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+        return false;
+    }
+    p.slot = ((int64_t)page * a.hkv * a.page_size + index % a.page_size) * a.D;
+    return true;
+}
+__device__ __forceinline__ float2 angle_of(const mgpu_k::AppendArgs& a, const Place& p, int pair) {
+    const int pos = pair < a.end0 ? p.pos[0] : pair < a.end1 ? p.pos[1] : p.pos[2];
+    return __ldg(reinterpret_cast<const float2*>(a.table) + (int64_t)pos * (a.rot / 2) + pair);
+}
+
+// A head of the step's q, k, v (in this order): where it is read and written.  A place in the cache
+// counts from the token's slot.
+struct Head {
+    const void* src;
+    void* dst;
+    int stype, dtype;
+    int64_t in, out;
+    bool turns;
+};
+__device__ __forceinline__ Head head_of(const mgpu_k::AppendArgs& a, int t, int h) {
+    const int g = h - a.hq;  // >= 0: a key head, >= hkv: a value head
+    const bool value = g >= a.hkv;
+    Head r;
+    r.turns = !value;
+    if (g < 0) {
+        r = {a.q, a.qo, a.qt, a.qot, (int64_t)t * a.ldq + (int64_t)h * a.D, (int64_t)t * a.ldqo + (int64_t)h * a.D, true};
+    } else if (!value) {
+        r = {a.k, a.kc, a.kt, a.ctype, (int64_t)t * a.ldk + (int64_t)g * a.D, (int64_t)g * a.page_size * a.D, true};
+    } else {
+        r = {a.v, a.vc, a.vt, a.ctype, (int64_t)t * a.ldv + (int64_t)(g - a.hkv) * a.D, (int64_t)(g - a.hkv) * a.page_size * a.D, false};
+    }
+    return r;
+}
+
+// Eight consecutive values as loaded: 16 bytes, or 32 of fp32.
+struct Raw8 {
+    uint4 a, b;
+};
+__device__ __forceinline__ Raw8 load_raw(const void* p, int type, int64_t i) {
+    Raw8 r;
+    if (type == MGPU_F32) {
+        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p) + i);
+        r.a = q[0];
+        r.b = q[1];
+    } else {
+        r.a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p) + i);
+        r.b = r.a;
+    }
+    return r;
+}
+__device__ __forceinline__ void values_of(const Raw8& r, int type, float (&o)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (type == MGPU_F32) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = __uint_as_float(w[k]);
         return;
     }
-    const int pair_units = a.rot / (ADJ ? PW : 2 * VEC);
-    const int units = pair_units + (a.D - a.rot) / VEC;
-    // a head of more units than threads (single-element units of a wide head) takes several passes
-    const int abreast = max(1, (int)blockDim.x / units);
-    for (int u = threadIdx.x % units, h0 = threadIdx.x / units; h0 < abreast && u < units;
-         u += (units > (int)blockDim.x ? (int)blockDim.x : units)) {
-        const bool paired = u < pair_units;
-        const int d = paired ? u * PW : a.rot + (u - pair_units) * VEC;
-        float2 cs[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) cs[i] = make_float2(1.0f, 0.0f);
-        if (paired) {
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = type == MGPU_F16 ? unpack2<__half>(w[k]) : unpack2<__nv_bfloat16>(w[k]);
+        o[2 * k] = f.x;
+        o[2 * k + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void store8(void* p, int type, int64_t i, const float (&v)[8]) {
+    if (type == MGPU_F32) {
+        float4* q = reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i);
+        q[0] = make_float4(v[0], v[1], v[2], v[3]);
+        q[1] = make_float4(v[4], v[5], v[6], v[7]);
+        return;
+    }
+    uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int pair = (ADJ ? d / 2 : d) + i;
-                const int p = pair < a.end0 ? pos[0] : pair < a.end1 ? pos[1] : pos[2];
-                cs[i] = __ldg(reinterpret_cast<const float2*>(a.table) + (int64_t)p * (a.rot / 2) + pair);
+    for (int k = 0; k < 4; ++k)
+        w[k] = type == MGPU_F16 ? pack2<__half>(v[2 * k], v[2 * k + 1]) : pack2<__nv_bfloat16>(v[2 * k], v[2 * k + 1]);
+    *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One CTA per (token, share of its heads), rows and halves of pairs on 16-byte boundaries.  A head is
+// cut into units of one thread: 8 dims and their partners rot/2 further on, or, with adjacent pairs,
+// 8 dims that hold their own partners; and 8 dims of the rest.  A thread keeps its unit over its
+// heads, so that it reads its angles once, and asks for its first kAhead heads before it looks up
+// where they go: five dependent reads (sequence, length, page, position, angle) that would otherwise
+// come before the first byte of data.
+constexpr int kAhead = 3;
+// ST, DT: the type of q, k and v, and that of q_out and the cache; -1 where they are not one.
+template <bool ADJ, int ST, int DT>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const mgpu_k::AppendArgs a) {
+    constexpr int NP = ADJ ? 4 : 8;  // pairs of a unit
+    const int t = blockIdx.x, half = a.rot / 2;
+    const int pair_units = a.rot / (ADJ ? 8 : 16), units = pair_units + (a.D - a.rot) / 8, abreast = kAppendThreads / units;
+    const int u = threadIdx.x % units, h0 = threadIdx.x / units;
+    const bool paired = u < pair_units;
+    const int d = paired ? u * 8 : a.rot + (u - pair_units) * 8;
+    const int step = (int)gridDim.y * abreast, heads = h0 < abreast ? a.hq + 2 * a.hkv : 0;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Raw8 x[kAhead], y[kAhead];
+    auto src_type = [&](const Head& s) { return ST >= 0 ? ST : s.stype; };
+    auto dst_type = [&](const Head& s) { return DT >= 0 ? DT : s.dtype; };
+    auto fetch = [&](int h) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (h + i * step < heads) {
+                const Head s = head_of(a, t, h + i * step);
+                x[i] = load_raw(s.src, src_type(s), s.in + d);
+                if (!ADJ && paired) y[i] = load_raw(s.src, src_type(s), s.in + d + half);
             }
-        }
-        const int heads = a.hq + 2 * a.hkv;
-        for (int h = blockIdx.y * abreast + h0; h < heads; h += gridDim.y * abreast) {
-            const int g = h - a.hq;  // >= 0: a key head, >= hkv: a value head
-            const bool value = g >= a.hkv;
-            const void* src = g < 0 ? a.q : value ? a.v : a.k;
-            const int st = g < 0 ? a.qt : value ? a.vt : a.kt;
-            const int hh = g < 0 ? h : value ? g - a.hkv : g;
-            const int64_t in = (int64_t)t * (g < 0 ? a.ldq : value ? a.ldv : a.ldk) + (int64_t)hh * a.D + d;
-            void* dst = g < 0 ? a.qo : value ? a.vc : a.kc;
-            const int dt = g < 0 ? a.qot : a.ctype;
-            const int64_t out = g < 0 ? (int64_t)t * a.ldqo + (int64_t)hh * a.D + d
-                                      : (((int64_t)page * a.hkv + hh) * a.page_size + index % a.page_size) * a.D + d;
+    };
+    int h = (int)blockIdx.y * abreast + h0;
+    fetch(h);
+    Place place;
+    if (!place_of(a, t, place)) return;
+    float2 cs[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) cs[i] = paired ? angle_of(a, place, (ADJ ? d / 2 : d) + i) : make_float2(1.0f, 0.0f);
+    for (; h < heads; h += kAhead * step) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (h + i * step >= heads) break;
+            const Head s = head_of(a, t, h + i * step);
+            const int64_t out = s.out + d + (h + i * step < a.hq ? 0 : place.slot);
+            float v[8];
+            values_of(x[i], src_type(s), v);
             if (!paired) {
-                float x[VEC];
-                load_vec<VEC>(src, st, in, x);
-                store_vec<VEC>(dst, dt, out, x);
+                store8(s.dst, dst_type(s), out, v);
             } else if constexpr (ADJ) {
-                float x[PW], y[PW];
-                load_vec<PW>(src, st, in, x);
+                if (s.turns) {
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    const float c = value ? 1.0f : cs[i].x, s = value ? 0.0f : cs[i].y;
-                    y[2 * i] = value ? x[2 * i] : x[2 * i] * c - x[2 * i + 1] * s;
-                    y[2 * i + 1] = value ? x[2 * i + 1] : x[2 * i] * s + x[2 * i + 1] * c;
+                    for (int p = 0; p < NP; ++p) {
+                        const float b = v[2 * p];
+                        v[2 * p] = b * cs[p].x - v[2 * p + 1] * cs[p].y;
+                        v[2 * p + 1] = b * cs[p].y + v[2 * p + 1] * cs[p].x;
+                    }
                 }
-                store_vec<PW>(dst, dt, out, y);
+                store8(s.dst, dst_type(s), out, v);
             } else {
-                const int half = a.rot / 2;
-                float x[VEC], y[VEC], xr[VEC], yr[VEC];
-                load_vec<VEC>(src, st, in, x);
-                load_vec<VEC>(src, st, in + half, y);
+                float w[8];
+                values_of(y[i], src_type(s), w);
+                if (s.turns) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    xr[i] = value ? x[i] : x[i] * cs[i].x - y[i] * cs[i].y;
-                    yr[i] = value ? y[i] : x[i] * cs[i].y + y[i] * cs[i].x;
+                    for (int p = 0; p < NP; ++p) {
+                        const float b = v[p];
+                        v[p] = b * cs[p].x - w[p] * cs[p].y;
+                        w[p] = b * cs[p].y + w[p] * cs[p].x;
+                    }
                 }
-                store_vec<VEC>(dst, dt, out, xr);
-                store_vec<VEC>(dst, dt, out + half, yr);
+                store8(s.dst, dst_type(s), out, v);
+                store8(s.dst, dst_type(s), out + half, w);
             }
         }
+        fetch(h + kAhead * step);
+    }
+}
+
+__device__ __forceinline__ void store1(void* p, int type, int64_t i, float v) {
+    if (type == MGPU_F32) reinterpret_cast<float*>(p)[i] = v;
+    else if (type == MGPU_F16) reinterpret_cast<__half*>(p)[i] = from_f32<__half>(v);
+    else reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
+}
+
+// The same for rows, pitches or rotations that do not fall on 16-byte boundaries: a thread to a pair,
+// or to a value that does not turn.
+__global__ void __launch_bounds__(kAppendThreads) kv_append_single_kernel(const mgpu_k::AppendArgs a) {
+    const int t = blockIdx.x, half = a.rot / 2, units = half + a.D - a.rot, heads = a.hq + 2 * a.hkv;
+    Place place;
+    if (!place_of(a, t, place)) return;
+    for (int i = blockIdx.y * kAppendThreads + threadIdx.x; i < heads * units; i += gridDim.y * kAppendThreads) {
+        const int h = i / units, u = i % units;
+        const Head s = head_of(a, t, h);
+        const int64_t out = s.out + (h < a.hq ? 0 : place.slot);
+        if (u >= half) {
+            const int d = a.rot + u - half;
+            store1(s.dst, s.dtype, out + d, load_float(s.src, s.stype, (size_t)(s.in + d)));
+            continue;
+        }
+        const int d0 = a.interleaved ? 2 * u : u, d1 = a.interleaved ? 2 * u + 1 : u + half;
+        float x = load_float(s.src, s.stype, (size_t)(s.in + d0)), y = load_float(s.src, s.stype, (size_t)(s.in + d1));
+        if (s.turns) {
+            const float2 cs = angle_of(a, place, u);
+            const float b = x;
+            x = b * cs.x - y * cs.y;
+            y = b * cs.y + y * cs.x;
+        }
+        store1(s.dst, s.dtype, out + d0, x);
+        store1(s.dst, s.dtype, out + d1, y);
     }
 }
 
@@ -184,23 +261,44 @@ cudaError_t kv_append(const LaunchCtx& c, const AppendArgs& a) {
     };
     const bool vec = ok(a.q, a.qt, a.ldq) && ok(a.k, a.kt, a.ldk) && ok(a.v, a.vt, a.ldv) && ok(a.qo, a.qot, a.ldqo) &&
                      a.rot % (a.interleaved ? 8 : 16) == 0;
-    const int w = vec ? 8 : 1;
-    const int units = (a.interleaved ? a.rot / (vec ? 8 : 2) : a.rot / (2 * w)) + (a.D - a.rot) / w;
-    const int abreast = units < kAppendThreads ? kAppendThreads / units : 1;
-    const int passes = (a.hq + 2 * a.hkv + abreast - 1) / abreast;
-    // Few tokens: one pass of heads per CTA, so that a decode step's launch is one round of loads.
-    // Many: a CTA keeps its token's heads, so that the sequence search and the angles are paid once.
-    int gy = 1;
-    while (gy < passes && (int64_t)a.batch.n_tokens * gy < 4 * c.sm_count) ++gy;
-    const dim3 grid((unsigned)a.batch.n_tokens, (unsigned)gy);
-    if (a.interleaved) {
-        if (vec) kv_append_kernel<8, true><<<grid, kAppendThreads, 0, c.stream>>>(a);
-        else kv_append_kernel<1, true><<<grid, kAppendThreads, 0, c.stream>>>(a);
+    const int heads = a.hq + 2 * a.hkv;
+    int passes;  // of a CTA over a token's heads
+    if (vec) {
+        const int units = a.rot / (a.interleaved ? 8 : 16) + (a.D - a.rot) / 8, abreast = kAppendThreads / units;
+        passes = (heads + abreast - 1) / abreast;
     } else {
-        if (vec) kv_append_kernel<8, false><<<grid, kAppendThreads, 0, c.stream>>>(a);
-        else kv_append_kernel<1, false><<<grid, kAppendThreads, 0, c.stream>>>(a);
+        passes = (int)(((int64_t)heads * (a.D - a.rot / 2) + kAppendThreads - 1) / kAppendThreads);
     }
-    return cudaGetLastError();
+    // Few tokens: one pass of heads per CTA, so that a decode step's launch is one round of loads.
+    // Many: a CTA keeps its token's heads, so that the look-ups are paid once.
+    int gy = 1;
+    while (gy < passes && gy < 65535 && (int64_t)a.batch.n_tokens * gy < 4 * c.sm_count) ++gy;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.batch.n_tokens, (unsigned)gy);
+    cfg.blockDim = dim3(kAppendThreads);
+    cfg.stream = c.stream;
+    if (!vec) return cudaLaunchKernelEx(&cfg, kv_append_single_kernel, a);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto launch = [&](auto st, auto dt) {
+        constexpr int ST = decltype(st)::value, DT = decltype(dt)::value;
+        return cudaLaunchKernelEx(&cfg, a.interleaved ? kv_append_kernel<true, ST, DT> : kv_append_kernel<false, ST, DT>, a);
+    };
+    // The usual types are compiled in; others (types that differ between q, k and v, or q_out's from the
+    // cache's) are looked at value by value, at some 2.3 times the instructions.
+    using F32 = std::integral_constant<int, MGPU_F32>;
+    using F16 = std::integral_constant<int, MGPU_F16>;
+    using BF16 = std::integral_constant<int, MGPU_BF16>;
+    using Any = std::integral_constant<int, -1>;
+    if (a.kt == a.vt && (!a.q || (a.qt == a.kt && a.qot == a.ctype))) {
+        if (a.kt == MGPU_F32) return a.ctype == MGPU_F16 ? launch(F32(), F16()) : launch(F32(), BF16());
+        if (a.kt == MGPU_F16 && a.ctype == MGPU_F16) return launch(F16(), F16());
+        if (a.kt == MGPU_BF16 && a.ctype == MGPU_BF16) return launch(BF16(), BF16());
+    }
+    return launch(Any(), Any());
 }
 
 }  // namespace mgpu_k

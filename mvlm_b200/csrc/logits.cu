@@ -17,9 +17,10 @@ using namespace mgpu_dev;
 
 namespace {
 
-constexpr int kRulesThreads = 512;
-constexpr int kPiece = 8192;  // tokens of a CTA's round: 32 KB of logits and 32 KB of words
-constexpr uint32_t kUsed = 1u << 31, kCount = kUsed - 1;
+constexpr int kRulesThreads = 256;
+constexpr int kPiece = 8192;  // tokens of a CTA's round: at most 32 KB of logits, 32 KB of words, 16 KB of places
+constexpr int kIds = 8;        // entries of the history that a thread keeps
+constexpr uint32_t kUsed = 1u << 31, kBiased = 1u << 30, kCount = kBiased - 1;
 
 // A logit as mgpu_argmax compares it: exponent field zero -> 0, all ones -> +-1e30 by the sign.
 template <typename T> __device__ __forceinline__ float compared(T v) {
@@ -37,6 +38,20 @@ template <typename T> __device__ __forceinline__ float compared(T v) {
     }
 }
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Values below the type's smallest normal one as 0.
+template <typename T> __device__ __forceinline__ float flush(float v) {
+    if constexpr (std::is_same<T, __half>::value) {
+        return fabsf(v) < 6.103515625e-5f ? 0.0f : v;
+    } else {
+        float r;
+        asm("add.ftz.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+        return r;
+    }
+}
+
 struct Best {
     float v;
     int i;
@@ -47,6 +62,18 @@ struct Best {
         }
     }
 };
+
+// The warp's best, in every lane: the largest value by an integer that orders as it does, then the
+// smallest of its indexes.
+__device__ __forceinline__ Best warp_best_of(Best b) {
+    const uint32_t bits = __float_as_uint(b.v + 0.0f);  // one zero
+    const uint32_t key = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+    Best r;
+    r.i = __reduce_min_sync(0xffffffffu, key == top ? b.i : 0x7FFFFFFF);
+    r.v = __uint_as_float(top & 0x80000000u ? top & 0x7FFFFFFFu : ~top);
+    return r;
+}
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float m;
@@ -59,20 +86,25 @@ template <typename T, int VEC> struct alignas(16) Pack {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kRulesThreads, 3) rules_kernel(const mgpu_k::RulesArgs a, int ctas, int range, int slots) {
-    constexpr int VEC = 16 / (int)sizeof(T), U = kPiece / (kRulesThreads * VEC);
+__global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::RulesArgs a, int ctas, int range, int slots) {
+    constexpr int VEC = 16 / (int)sizeof(T);
     extern __shared__ __align__(16) uint8_t smem[];
-    float* vals = reinterpret_cast<float*>(smem);                 // [slots] the piece's logits
-    uint32_t* words = reinterpret_cast<uint32_t*>(vals + slots);  // [slots] counts, then bias entries
+    T* vals = reinterpret_cast<T*>(smem);                                                // [slots] the piece's logits
+    uint32_t* words = reinterpret_cast<uint32_t*>(smem + (size_t)slots * sizeof(T));     // [slots] marks and counts
+    uint32_t* mask = words + slots;                                                      // [kPiece / 32 + 2] allowed tokens
+    uint16_t* marked = reinterpret_cast<uint16_t*>(mask + kPiece / 32 + 2);              // [slots] places of marked tokens
     __shared__ Best warp_best[kRulesThreads / 32];
-    __shared__ Best cta_best;
+    __shared__ Best cta_best[8];  // the first CTA's: all CTAs' results
+    __shared__ int n_marked;
     const int tid = threadIdx.x, row = blockIdx.x / ctas, rank = blockIdx.x % ctas;
+    if (a.best && ctas > 1) cluster_arrive();  // this CTA runs: the others may write to it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx;
     T* out = a.out ? reinterpret_cast<T*>(a.out) + (int64_t)row * a.ldo : nullptr;
     const int first = (int)min((int64_t)a.n, (int64_t)rank * range), last = (int)min((int64_t)a.n, (int64_t)first + range);
     const uint32_t* allowed = a.allowed ? a.allowed + (int64_t)row * ((a.n + 31) / 32) : nullptr;
+    const int* ids = a.history ? a.history + (int64_t)row * a.history_ld : nullptr;
     Best best{-1e30f, 0x7FFFFFFF};
 
     for (int p0 = first; p0 < last; p0 += kPiece) {
@@ -84,17 +116,21 @@ __global__ void __launch_bounds__(kRulesThreads, 3) rules_kernel(const mgpu_k::R
         const int tail = head + vecs * VEC, ends = (head - p0) + (p1 - tail);  // single tokens, before and after
         auto end_token = [&](int i) { return i < head - p0 ? p0 + i : tail + i - (head - p0); };
         const bool vec_out = (((uintptr_t)(out + p0) ^ (uintptr_t)(x + p0)) & 15) == 0;
-        // the piece's logits are on their way while its words are cleared
-        uint4 raw[U];
+        // Everything that does not hang on something else is asked for at once: a CTA's time is the
+        // number of reads it waits for one after another, not their bytes.
+        const uint32_t to = smem_u32(vals + head - base);
+        for (int i = tid; i < vecs; i += kRulesThreads)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 16 * i), "l"(x + head + i * VEC) : "memory");
+        if (allowed)
+            for (int i = (p0 >> 5) + tid; i <= (p1 - 1) >> 5; i += kRulesThreads)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(mask + i - (p0 >> 5))), "l"(allowed + i) : "memory");
+        int id[kIds];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (tid + u * kRulesThreads < vecs) raw[u] = *reinterpret_cast<const uint4*>(x + head + (tid + u * kRulesThreads) * VEC);
-        if (tid < ends) vals[end_token(tid) - base] = to_f32<T>(x[end_token(tid)]);
+        for (int k = 0; k < kIds; ++k) id[k] = ids && tid + k * kRulesThreads < a.history_ld ? __ldg(ids + tid + k * kRulesThreads) : -1;
+        if (tid < ends) vals[end_token(tid) - base] = x[end_token(tid)];
         int hist = 0, prompt = 0, b0 = 0, b1 = 0;
         float again = 1.0f, often = 0.0f, present = 0.0f;
-        const int* ids = nullptr;
         if (a.history) {
-            ids = a.history + (int64_t)row * a.history_ld;
             hist = min(max(a.history_lens[row], 0), a.history_ld);
             prompt = a.prompt_lens ? a.prompt_lens[row] : 0;
             again = a.penalties[3 * row];
@@ -105,88 +141,66 @@ __global__ void __launch_bounds__(kRulesThreads, 3) rules_kernel(const mgpu_k::R
             b0 = min(max(a.bias_offsets[row], 0), a.bias_entries);
             b1 = min(a.bias_offsets[row + 1], a.bias_entries);
         }
-        const bool marks = hist > 0 || b1 > b0;
-        if (marks) {
+        if (a.history || a.bias_offsets) {
             const int used = (p1 - base + 3) / 4;  // slots are a multiple of 4
             for (int i = tid; i < used; i += kRulesThreads) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+            if (tid == 0) n_marked = 0;
             __syncthreads();
-#pragma unroll 4
-            for (int i = tid; i < hist; i += kRulesThreads) {
-                const int t = ids[i];
-                if (t < p0 || t >= p1) continue;
-                // a token of the prompt is used but not counted
-                if (i < prompt) atomicOr(&words[t - base], kUsed);
-                else atomicAdd(&words[t - base], 1u);
+            // The few tokens that have a mark: the first to mark one lists it, and then each is changed once
+            // where it lies, so that the pass over all tokens knows nothing of penalties and biases.
+            auto mark = [&](int t, uint32_t add, uint32_t set) {
+                if (t < p0 || t >= p1) return;
+                uint32_t* w = &words[t - base];
+                if ((set ? atomicOr(w, set) : atomicAdd(w, add)) == 0) marked[atomicAdd(&n_marked, 1)] = (uint16_t)(t - base);
+            };
+            // a token of the prompt is used but not counted
+#pragma unroll
+            for (int k = 0; k < kIds; ++k) {
+                const int i = tid + k * kRulesThreads;
+                if (i < hist) mark(id[k], 1, i < prompt ? kUsed : 0);
             }
+            for (int i = tid + kIds * kRulesThreads; i < hist; i += kRulesThreads) mark(__ldg(ids + i), 1, i < prompt ? kUsed : 0);
+            for (int i = b0 + tid; i < b1; i += kRulesThreads) mark(__ldg(a.bias_tokens + i), 0, kBiased);
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = tid + u * kRulesThreads;
-            if (i >= vecs) break;
-            const Pack<T, VEC> in = *reinterpret_cast<const Pack<T, VEC>*>(&raw[u]);
-            float4* to = reinterpret_cast<float4*>(vals + head - base + i * VEC);
-#pragma unroll
-            for (int k = 0; k < VEC; k += 4)
-                to[k / 4] = make_float4(to_f32<T>(in.v[k]), to_f32<T>(in.v[k + 1]), to_f32<T>(in.v[k + 2]), to_f32<T>(in.v[k + 3]));
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
-        // The few tokens that have a mark are changed where they lie, each by the one entry that takes its
-        // word: the pass over all tokens then knows nothing of penalties and biases.  Multiplication,
-        // division, subtraction and addition are each rounded once, in the documented order.
-        if (hist > 0) {
-#pragma unroll 2
-            for (int i = tid; i < hist; i += kRulesThreads) {
-                const int t = ids[i];
-                if (t < p0 || t >= p1) continue;
-                const uint32_t w = atomicExch(&words[t - base], 0u);
-                if (w == 0) continue;
-                float v = vals[t - base];
-                v = v > 0.0f ? __fdiv_rn(v, again) : __fmul_rn(v, again);
+        if (a.history || a.bias_offsets) {
+            // multiplication, division, subtraction and addition each rounded once, in the documented order
+            for (int i = tid; i < n_marked; i += kRulesThreads) {
+                const int at = marked[i];
+                const uint32_t w = words[at];
+                float v = to_f32<T>(vals[at]);
+                if (w & (kUsed | kCount)) v = v > 0.0f ? __fdiv_rn(v, again) : __fmul_rn(v, again);
                 if (w & kCount) v = __fsub_rn(__fsub_rn(v, __fmul_rn(often, (float)(w & kCount))), present);
-                vals[t - base] = v;
+                if (w & kBiased) {  // of entries with one token, the last
+                    int e = b1 - 1;
+                    while (__ldg(a.bias_tokens + e) != at + base) --e;
+                    v = __fadd_rn(v, __ldg(a.bias_values + e));
+                }
+                vals[at] = from_f32<T>(v);
             }
             __syncthreads();
         }
-        if (b1 > b0) {  // of entries with one token, the last: the words are clear again and take its index
-            for (int i = b0 + tid; i < b1; i += kRulesThreads) {
-                const int t = a.bias_tokens[i];
-                if (t >= p0 && t < p1) atomicMax(&words[t - base], (uint32_t)(i - b0) + 1u);
-            }
-            __syncthreads();
-            for (int i = b0 + tid; i < b1; i += kRulesThreads) {
-                const int t = a.bias_tokens[i];
-                if (t >= p0 && t < p1 && words[t - base] == (uint32_t)(i - b0) + 1u)
-                    vals[t - base] = __fadd_rn(vals[t - base], a.bias_values[i]);
-            }
-            __syncthreads();
-        }
-        auto consider = [&](T y, int t) {
-            const float c = compared<T>(y);
-            if (c > best.v || (c == best.v && t < best.i && c > -1e30f)) best = Best{c, t};
+        // The maximum: a thread keeps its first greatest vector, and looks for the token in it at the end.
+        // Values compare as they stand but for three kinds that mgpu_argmax reads otherwise: subnormal ones
+        // are 0, and Inf and NaN, which a vector's maximum shows, go the long way.
+        const T none = from_f32<T>(-INFINITY);
+        auto value = [&](int t) {
+            return !allowed || (mask[(t >> 5) - (p0 >> 5)] >> (t & 31) & 1u) ? vals[t - base] : none;
         };
-        if (tid < ends) {
-            const int t = end_token(tid);
-            const bool ok = !allowed || ((allowed[t >> 5] >> (t & 31)) & 1u);
-            const T y = from_f32<T>(ok ? vals[t - base] : -INFINITY);
-            if (out) out[t] = y;
-            if (a.best) consider(y, t);
-        }
+        float top = -1e30f;
+        int top_i = -1;
+#pragma unroll 4
         for (int i = tid; i < vecs; i += kRulesThreads) {
             const int t = head + i * VEC;
-            float v[VEC];
-#pragma unroll
-            for (int k = 0; k < VEC; k += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(vals + t - base + k);
-                v[k] = q.x; v[k + 1] = q.y; v[k + 2] = q.z; v[k + 3] = q.w;
-            }
+            const uint4 q = *reinterpret_cast<const uint4*>(vals + t - base);
+            Pack<T, VEC> y = *reinterpret_cast<const Pack<T, VEC>*>(&q);
             if (allowed) {
-                const uint32_t bits = __funnelshift_r(allowed[t >> 5], allowed[(t + VEC - 1) >> 5], t & 31);
+                const uint32_t* m = mask + (t >> 5) - (p0 >> 5);
+                const uint32_t bits = __funnelshift_r(m[0], m[1], t & 31);  // m[1] may be beyond: its bits are then not used
 #pragma unroll
-                for (int k = 0; k < VEC; ++k) v[k] = (bits >> k) & 1u ? v[k] : -INFINITY;
+                for (int k = 0; k < VEC; ++k) y.v[k] = (bits >> k) & 1u ? y.v[k] : none;
             }
-            Pack<T, VEC> y;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) y.v[k] = from_f32<T>(v[k]);
             if (out) {
                 if (vec_out) {
                     *reinterpret_cast<uint4*>(out + t) = *reinterpret_cast<const uint4*>(&y);
@@ -196,53 +210,66 @@ __global__ void __launch_bounds__(kRulesThreads, 3) rules_kernel(const mgpu_k::R
                 }
             }
             if (a.best) {
-                // A value that beats the best in the comparison's own terms is above it, or NaN, as it
-                // stands: only then are the vector's values looked at one by one.
-                float top = to_f32<T>(y.v[0]);
+                float m = to_f32<T>(y.v[0]);
 #pragma unroll
-                for (int k = 1; k < VEC; ++k) top = max_nan(top, to_f32<T>(y.v[k]));
-                if (!(top <= best.v)) {
-#pragma unroll 1
-                    for (int k = 0; k < VEC; ++k) consider(y.v[k], t + k);
+                for (int k = 1; k < VEC; ++k) m = max_nan(m, to_f32<T>(y.v[k]));
+                m = flush<T>(m);
+                if (!(m < 1e30f)) {
+                    m = compared<T>(y.v[0]);
+#pragma unroll
+                    for (int k = 1; k < VEC; ++k) m = fmaxf(m, compared<T>(y.v[k]));
+                }
+                if (m > top) {
+                    top = m;
+                    top_i = i;
                 }
             }
+        }
+        if (a.best && top > best.v) {
+            const int t = head + top_i * VEC;
+            for (int k = VEC - 1; k >= 0; --k)
+                if (compared<T>(value(t + k)) == top) best.i = t + k;
+            best.v = top;
+        }
+        if (tid < ends) {
+            const int t = end_token(tid);
+            const T y = value(t);
+            if (out) out[t] = y;
+            const float c = compared<T>(y);
+            if (c > best.v || (c == best.v && t < best.i && c > -1e30f)) best = Best{c, t};
         }
         if (p1 < last) __syncthreads();  // the next piece takes the places
     }
     if (!a.best) return;
     // equal values of two threads go to the smaller index, as they did within one
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-        best.take(__shfl_xor_sync(0xffffffffu, best.v, off), __shfl_xor_sync(0xffffffffu, best.i, off));
+    best = warp_best_of(best);
     if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
-    if (tid < 32) {
-        best = tid < kRulesThreads / 32 ? warp_best[tid] : Best{-1e30f, 0x7FFFFFFF};
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1)
-            best.take(__shfl_xor_sync(0xffffffffu, best.v, off), __shfl_xor_sync(0xffffffffu, best.i, off));
-        if (tid == 0) cta_best = best;
-    }
-    if (ctas > 1) cluster_sync_all();
-    if (rank == 0 && tid < 32) {
-        Best other{-1e30f, 0x7FFFFFFF};
-        if (tid > 0 && tid < ctas) {
-            const uint32_t p = cluster_addr(&cta_best, (uint32_t)tid);
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.v) : "r"(p) : "memory");
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(other.i) : "r"(p + 4) : "memory");
-        }
-        if (tid == 0) other = best;
-#pragma unroll
-        for (int off = 4; off > 0; off >>= 1)
-            other.take(__shfl_xor_sync(0xffffffffu, other.v, off), __shfl_xor_sync(0xffffffffu, other.i, off));
-        if (tid == 0) {
-            // nothing above -1e30: index 0, as mgpu_argmax starts
-            a.best[2 * row] = other.v > -1e30f ? other.i : 0;
-            a.best[2 * row + 1] = __float_as_int(other.v);
+    if (tid < 32) best = warp_best_of(tid < kRulesThreads / 32 ? warp_best[tid] : Best{-1e30f, 0x7FFFFFFF});
+    // every CTA's result goes to the first one, which alone waits for the others
+    if (ctas > 1) cluster_wait();  // it runs
+    if (tid == 0) {
+        if (ctas > 1) {
+            const uint32_t p = cluster_addr(&cta_best[rank], 0);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(p), "f"(best.v) : "memory");
+            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(p + 4), "r"(best.i) : "memory");
+        } else {
+            cta_best[0] = best;
         }
     }
-    if (ctas > 1) cluster_sync_all();  // no CTA leaves while another reads its result
+    __syncwarp();
+    if (ctas > 1) cluster_arrive();
+    if (rank != 0) return;
+    if (ctas > 1) cluster_wait();
+    if (tid == 0) {
+        for (int r = 1; r < ctas; ++r) best.take(cta_best[r].v, cta_best[r].i);
+        // nothing above -1e30: index 0, as mgpu_argmax starts
+        a.best[2 * row] = best.v > -1e30f ? best.i : 0;
+        a.best[2 * row + 1] = __float_as_int(best.v);
+    }
 }
+
+template <typename T> constexpr int rules_smem(int slots) { return slots * ((int)sizeof(T) + 4 + 2) + 4 * (kPiece / 32 + 2); }
 
 template <typename T>
 cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a) {
@@ -253,7 +280,7 @@ cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a)
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (ordinal & 63);
     if (ordinal >= 64 || !(configured.load(std::memory_order_acquire) & bit)) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 * (kPiece + 8));
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, rules_smem<T>(kPiece + 8));
         if (e != cudaSuccess) return e;
         configured.fetch_or(bit, std::memory_order_acq_rel);
     }
@@ -265,7 +292,7 @@ cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas * (unsigned)a.rows);
     cfg.blockDim = dim3(kRulesThreads);
-    cfg.dynamicSmemBytes = (size_t)slots * 8;
+    cfg.dynamicSmemBytes = rules_smem<T>(slots);
     cfg.stream = c.stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -361,13 +361,14 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* cache, const mgpu_paged_ba
 /* ---------------------------------------------------------------- logit rules ------ */
 /* What is done to each row of logits before a token is chosen, in this order, in fp32:
  *   history      ids the row's sequence holds, the prompt's first (int32 [rows][history_ld], the
- *                first history_lens[r] of them, prompt_lens[r] of these the prompt's);
- *                ids outside [0, n) are skipped
+ *                first history_lens[r] of them, prompt_lens[r] of these the prompt's;
+ *                history_ld below 2^20); ids outside [0, n) are skipped
  *   penalties    {repetition, frequency, presence} of each row (fp32 [rows][3]): a token in the
  *                history has x > 0 ? x / repetition : x * repetition; one that is c > 0 times in
  *                the history after the prompt loses frequency * c, then presence
  *   bias         row r's entries bias_offsets[r] .. bias_offsets[r+1]-1 of bias_tokens /
- *                bias_values: x += value (of entries with one token, the last one's)
+ *                bias_values: x += value (of entries with one token, the last one's); at most
+ *                2047 entries a row, more are skipped and reported like a batch's contents above
  *   allowed      bit t % 32 of word t / 32 of row r (uint32 [rows][(n + 31) / 32]) clear: x = -inf
  * Each group may be NULL: history (with its lens and penalties), prompt_lens alone (no prompt),
  * bias_* together, allowed. */

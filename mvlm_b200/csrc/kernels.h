@@ -161,7 +161,12 @@ struct RulesArgs {
     const float* bias_values;
     int bias_entries;
     const uint32_t* allowed;
+    int* status;
+    int2* partials;         // rules_scratch_bytes
+    unsigned int* tickets;  // rules_max_rows, zero between calls (the kernel leaves them so)
 };
+int rules_max_rows();
+size_t rules_scratch_bytes();
 cudaError_t logits_process(const LaunchCtx& c, const RulesArgs& a);
 
 // ---------------------------------------------------------------- GEMM (gemm_tc.cu) --

@@ -1,11 +1,12 @@
 // logits.cu - penalties, biases and grammar masks on rows of logits, and the first maximum of
 // what they leave, in one pass.
 //
-// A cluster of CTAs shares a row; each CTA owns a contiguous range of the vocabulary and keeps one
-// word per token of it in shared memory (how often the history holds the token).  It scans the
-// row's history for tokens of its range, then streams its logits once.  Bound: the logits in and
-// out at HBM rate.  Counts are integers and a bias is picked by its entry's index, so the order in
-// which threads reach a word cannot change a result.
+// Up to eight CTAs share a row; each owns a contiguous range of the vocabulary and keeps one word per
+// token of it in shared memory (how often the history holds the token, which bias it has).  It scans
+// the row's history and biases for tokens of its range, then streams its logits once.  Bound: the
+// logits in and out at HBM rate.  Counts are integers and a bias is picked by its entry's index, so
+// the order in which threads reach a word cannot change a result.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -20,7 +21,11 @@ namespace {
 constexpr int kRulesThreads = 256;
 constexpr int kPiece = 8192;  // tokens of a CTA's round: at most 32 KB of logits, 32 KB of words, 16 KB of places
 constexpr int kIds = 8;        // entries of the history that a thread keeps
-constexpr uint32_t kUsed = 1u << 31, kBiased = 1u << 30, kCount = kBiased - 1;
+constexpr int kListed = 1024;  // marked tokens that a round lists
+// A token's word: how often the history after the prompt holds it, whether the prompt does, and its
+// last bias entry + 1.
+constexpr int kBiasShift = 21, kBiases = (1 << (32 - kBiasShift)) - 1;
+constexpr uint32_t kUsed = 1u << 20, kCount = kUsed - 1;
 
 // A logit as mgpu_argmax compares it: exponent field zero -> 0, all ones -> +-1e30 by the sign.
 template <typename T> __device__ __forceinline__ float compared(T v) {
@@ -37,9 +42,6 @@ template <typename T> __device__ __forceinline__ float compared(T v) {
         return __uint_as_float(b);
     }
 }
-
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Values below the type's smallest normal one as 0.
 template <typename T> __device__ __forceinline__ float flush(float v) {
@@ -92,12 +94,10 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
     T* vals = reinterpret_cast<T*>(smem);                                                // [slots] the piece's logits
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + (size_t)slots * sizeof(T));     // [slots] marks and counts
     uint32_t* mask = words + slots;                                                      // [kPiece / 32 + 2] allowed tokens
-    uint16_t* marked = reinterpret_cast<uint16_t*>(mask + kPiece / 32 + 2);              // [slots] places of marked tokens
+    uint16_t* marked = reinterpret_cast<uint16_t*>(mask + kPiece / 32 + 2);              // [kListed] places of marked tokens
     __shared__ Best warp_best[kRulesThreads / 32];
-    __shared__ Best cta_best[8];  // the first CTA's: all CTAs' results
     __shared__ int n_marked;
     const int tid = threadIdx.x, row = blockIdx.x / ctas, rank = blockIdx.x % ctas;
-    if (a.best && ctas > 1) cluster_arrive();  // this CTA runs: the others may write to it
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx;
@@ -137,9 +137,15 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
             often = a.penalties[3 * row + 1];
             present = a.penalties[3 * row + 2];
         }
+        int bias_t = -1;
         if (a.bias_offsets) {
             b0 = min(max(a.bias_offsets[row], 0), a.bias_entries);
             b1 = min(a.bias_offsets[row + 1], a.bias_entries);
+            if (b1 - b0 > kBiases) {
+                if (tid == 0) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                b1 = b0 + kBiases;
+            }
+            if (b0 + tid < b1) bias_t = __ldg(a.bias_tokens + b0 + tid);
         }
         if (a.history || a.bias_offsets) {
             const int used = (p1 - base + 3) / 4;  // slots are a multiple of 4
@@ -148,36 +154,48 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
             __syncthreads();
             // The few tokens that have a mark: the first to mark one lists it, and then each is changed once
             // where it lies, so that the pass over all tokens knows nothing of penalties and biases.
-            auto mark = [&](int t, uint32_t add, uint32_t set) {
-                if (t < p0 || t >= p1) return;
-                uint32_t* w = &words[t - base];
-                if ((set ? atomicOr(w, set) : atomicAdd(w, add)) == 0) marked[atomicAdd(&n_marked, 1)] = (uint16_t)(t - base);
+            auto listed = [&](int at) {
+                const int k = atomicAdd(&n_marked, 1);
+                if (k < kListed) marked[k] = (uint16_t)at;
             };
-            // a token of the prompt is used but not counted
-#pragma unroll
-            for (int k = 0; k < kIds; ++k) {
-                const int i = tid + k * kRulesThreads;
-                if (i < hist) mark(id[k], 1, i < prompt ? kUsed : 0);
+            auto in = [&](int t) { return (unsigned)(t - p0) < (unsigned)(p1 - p0); };
+            if (b1 > b0) {  // of entries with one token, the last
+                auto bias = [&](int i, int t) {
+                    if (in(t) && atomicMax(&words[t - base], (uint32_t)i << kBiasShift) == 0) listed(t - base);
+                };
+                if (tid < b1 - b0) bias(tid + 1, bias_t);
+                for (int i = tid + kRulesThreads; i < b1 - b0; i += kRulesThreads) bias(i + 1, __ldg(a.bias_tokens + b0 + i));
+                __syncthreads();
             }
-            for (int i = tid + kIds * kRulesThreads; i < hist; i += kRulesThreads) mark(__ldg(ids + i), 1, i < prompt ? kUsed : 0);
-            for (int i = b0 + tid; i < b1; i += kRulesThreads) mark(__ldg(a.bias_tokens + i), 0, kBiased);
+            // a token of the prompt is used but not counted
+            auto mark = [&](int i, int t) {
+                if (!in(t)) return;
+                uint32_t* w = &words[t - base];
+                if ((i < prompt ? atomicOr(w, kUsed) : atomicAdd(w, 1u)) == 0) listed(t - base);
+            };
+#pragma unroll
+            for (int k = 0; k < kIds; ++k)
+                if (tid + k * kRulesThreads < hist) mark(tid + k * kRulesThreads, id[k]);
+            for (int i = tid + kIds * kRulesThreads; i < hist; i += kRulesThreads) mark(i, __ldg(ids + i));
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncthreads();
         if (a.history || a.bias_offsets) {
             // multiplication, division, subtraction and addition each rounded once, in the documented order
-            for (int i = tid; i < n_marked; i += kRulesThreads) {
-                const int at = marked[i];
-                const uint32_t w = words[at];
+            auto change = [&](int at) {
+                const uint32_t w = words[at], entry = w >> kBiasShift;
+                const float bias = entry ? __ldg(a.bias_values + b0 + entry - 1) : 0.0f;
                 float v = to_f32<T>(vals[at]);
                 if (w & (kUsed | kCount)) v = v > 0.0f ? __fdiv_rn(v, again) : __fmul_rn(v, again);
                 if (w & kCount) v = __fsub_rn(__fsub_rn(v, __fmul_rn(often, (float)(w & kCount))), present);
-                if (w & kBiased) {  // of entries with one token, the last
-                    int e = b1 - 1;
-                    while (__ldg(a.bias_tokens + e) != at + base) --e;
-                    v = __fadd_rn(v, __ldg(a.bias_values + e));
-                }
+                if (entry) v = __fadd_rn(v, bias);
                 vals[at] = from_f32<T>(v);
+            };
+            if (n_marked <= kListed) {
+                for (int i = tid; i < n_marked; i += kRulesThreads) change(marked[i]);
+            } else {  // more than the list holds
+                for (int at = tid; at < p1 - base; at += kRulesThreads)
+                    if (words[at]) change(at);
             }
             __syncthreads();
         }
@@ -246,30 +264,27 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
     if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
     if (tid < 32) best = warp_best_of(tid < kRulesThreads / 32 ? warp_best[tid] : Best{-1e30f, 0x7FFFFFFF});
-    // every CTA's result goes to the first one, which alone waits for the others
-    if (ctas > 1) cluster_wait();  // it runs
-    if (tid == 0) {
-        if (ctas > 1) {
-            const uint32_t p = cluster_addr(&cta_best[rank], 0);
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(p), "f"(best.v) : "memory");
-            asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(p + 4), "r"(best.i) : "memory");
-        } else {
-            cta_best[0] = best;
-        }
+    if (tid != 0) return;
+    // The row's last CTA to come joins their results.  (A cluster would hold its CTAs until the slowest:
+    // 11 us more for 256 rows of 51200.)
+    if (ctas > 1) {
+        __stcg(a.partials + (int64_t)row * 8 + rank, make_int2(best.i, __float_as_int(best.v)));
+        __threadfence();
+        if (atomicAdd(a.tickets + row, 1u) != (unsigned)(ctas - 1)) return;
+        a.tickets[row] = 0;
+        __threadfence();
+        int2 other[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) other[r] = r < ctas ? __ldcg(a.partials + (int64_t)row * 8 + r) : make_int2(0x7FFFFFFF, __float_as_int(-1e30f));
+#pragma unroll
+        for (int r = 0; r < 8; ++r) best.take(__int_as_float(other[r].y), other[r].x);
     }
-    __syncwarp();
-    if (ctas > 1) cluster_arrive();
-    if (rank != 0) return;
-    if (ctas > 1) cluster_wait();
-    if (tid == 0) {
-        for (int r = 1; r < ctas; ++r) best.take(cta_best[r].v, cta_best[r].i);
-        // nothing above -1e30: index 0, as mgpu_argmax starts
-        a.best[2 * row] = best.v > -1e30f ? best.i : 0;
-        a.best[2 * row + 1] = __float_as_int(best.v);
-    }
+    // nothing above -1e30: index 0, as mgpu_argmax starts
+    a.best[2 * (int64_t)row] = best.v > -1e30f ? best.i : 0;
+    a.best[2 * (int64_t)row + 1] = __float_as_int(best.v);
 }
 
-template <typename T> constexpr int rules_smem(int slots) { return slots * ((int)sizeof(T) + 4 + 2) + 4 * (kPiece / 32 + 2); }
+template <typename T> constexpr int rules_smem(int slots) { return slots * ((int)sizeof(T) + 4) + 4 * (kPiece / 32 + 2) + 2 * kListed; }
 
 template <typename T>
 cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a) {
@@ -294,15 +309,11 @@ cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a)
     cfg.blockDim = dim3(kRulesThreads);
     cfg.dynamicSmemBytes = rules_smem<T>(slots);
     cfg.stream = c.stream;
-    cudaLaunchAttribute attr[2];
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)ctas;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, a, ctas, range, slots);
 }
 
@@ -310,10 +321,31 @@ cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a)
 
 namespace mgpu_k {
 
-cudaError_t logits_process(const LaunchCtx& c, const RulesArgs& a) {
-    if (a.type == MGPU_F32) return launch_rules<float>(c, a);
-    if (a.type == MGPU_F16) return launch_rules<__half>(c, a);
-    return launch_rules<__nv_bfloat16>(c, a);
+cudaError_t logits_process(const LaunchCtx& c, const RulesArgs& in) {
+    // launches of at most rules_max_rows() rows, for which there are tickets
+    for (int64_t r0 = 0; r0 < in.rows; r0 += rules_max_rows()) {
+        RulesArgs a = in;
+        a.rows = (int)std::min<int64_t>(in.rows - r0, rules_max_rows());
+        const size_t es = a.type == MGPU_F32 ? 4 : 2;
+        a.x = static_cast<const char*>(in.x) + r0 * in.ldx * es;
+        if (in.out) a.out = static_cast<char*>(in.out) + r0 * in.ldo * es;
+        if (in.best) a.best = in.best + 2 * r0;
+        if (in.history) {
+            a.history = in.history + r0 * in.history_ld;
+            a.history_lens = in.history_lens + r0;
+            if (in.prompt_lens) a.prompt_lens = in.prompt_lens + r0;
+            a.penalties = in.penalties + 3 * r0;
+        }
+        if (in.bias_offsets) a.bias_offsets = in.bias_offsets + r0;
+        if (in.allowed) a.allowed = in.allowed + r0 * ((in.n + 31) / 32);
+        const cudaError_t e = a.type == MGPU_F32 ? launch_rules<float>(c, a)
+                              : a.type == MGPU_F16 ? launch_rules<__half>(c, a) : launch_rules<__nv_bfloat16>(c, a);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
+
+int rules_max_rows() { return 8192; }
+size_t rules_scratch_bytes() { return (size_t)rules_max_rows() * 8 * sizeof(int2); }
 
 }  // namespace mgpu_k

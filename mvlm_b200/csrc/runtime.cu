@@ -107,14 +107,15 @@ size_t quant_row_bytes(int t, int64_t k) { return (size_t)((k + 31) / 32) * (t =
 
 // Scratch arena layout: [0, 64 KB) holds the split-K tickets of gemv_kn, [64 KB, 128 KB) those of
 // the split-K GEMM and [128 KB, 136 KB) those of the paged attention's shares (eight per CTA of a
-// one-wave grid); all must stay zero between launches (the kernels reset them).
+// one-wave grid) and [136 KB, 168 KB) those of the logit rules' rows; all must stay zero between launches (the kernels reset them).
 // Everything from kScratchOffset on is free for per-call use (split-K partials, im2col
 // patches, staged operands), in stream order.
 constexpr size_t kGemvTicketBytes = 64 * 1024;
 constexpr size_t kGemmTicketOffset = 64 * 1024;
 constexpr size_t kGemmTicketBytes = 64 * 1024;
 constexpr size_t kAttendTicketOffset = 128 * 1024;
-constexpr size_t kScratchOffset = 136 * 1024;
+constexpr size_t kRulesTicketOffset = 136 * 1024;
+constexpr size_t kScratchOffset = 168 * 1024;
 
 mgpu_k::LaunchCtx ctx_of(const mgpu_device* d) {
     mgpu_k::LaunchCtx c;
@@ -190,7 +191,8 @@ bool check_status(mgpu_device* d) {
         if (st == MGPU_ERR_DEVICE_TIMEOUT && d->workspace_bytes >= kScratchOffset)
             cudaMemsetAsync((char*)d->workspace + kAttendTicketOffset, 0, kScratchOffset - kAttendTicketOffset, d->stream);
         if (st == MGPU_ERR_INVALID_ARG)
-            set_error(st, "a kernel skipped sequences whose lengths, pages or positions do not fit their buffers");
+            set_error(st, "a kernel skipped what does not fit its buffers: sequences by their lengths, pages or positions, "
+                      "or bias entries of a row beyond 2047");
         else
             set_error(st, "a kernel's bounded wait expired (device status %d); its output is invalid", st);
         return false;
@@ -1295,7 +1297,7 @@ mgpu_event* mgpu_logits_process(const mgpu_device* cd, mgpu_buf* logits, mgpu_bu
     REQUIRE(cd && logits && r, "logits_process: null argument");
     REQUIRE(out || best, "logits_process: neither out nor best");
     REQUIRE(rows > 0 && n > 0, "logits_process: rows=%d n=%d", rows, n);
-    REQUIRE((int64_t)rows * 8 <= INT32_MAX && n <= (1 << 30), "logits_process: rows=%d or n=%d too large", rows, n);
+    REQUIRE(n <= (1 << 30), "logits_process: n=%d too large", n);
     mgpu_k::RulesArgs a = {};
     if (!rows_ok(logits, rows, n, "logits_process", "logits", &a.ldx)) return nullptr;
     if (out) {
@@ -1347,8 +1349,18 @@ mgpu_event* mgpu_logits_process(const mgpu_device* cd, mgpu_buf* logits, mgpu_bu
     a.type = logits->type;
     a.rows = rows;
     a.n = n;
+    if (a.history && a.history_ld >= 1 << 20) {  // what a token's word counts
+        set_error(MGPU_ERR_UNSUPPORTED, "logits_process: history_ld=%d is not below 2^20", a.history_ld);
+        return nullptr;
+    }
     mgpu_device* d = const_cast<mgpu_device*>(cd);
     DeviceGuard g(d->ordinal);
+    a.status = d->d_status;
+    if (best) {
+        if (!ensure_workspace(d, kScratchOffset + mgpu_k::rules_scratch_bytes())) return nullptr;
+        a.tickets = (unsigned int*)((char*)d->workspace + kRulesTicketOffset);
+        a.partials = (int2*)((char*)d->workspace + kScratchOffset);
+    }
     mgpu_event* ev = event_begin(d);
     if (!cuda_ok(mgpu_k::logits_process(ctx_of(d), a), "logits_process")) {
         if (ev) d->event_pool.push_back(ev);

@@ -634,7 +634,7 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
 // 4 D operations to a row and key, and by one exponential to a row and key.  A CTA takes two tiles of
 // up to 128 rows (whole tokens: 128 / G of them) over the same blocks of 128 keys.  A warp to
 // each tile issues S_t = Q_t K^T and O_t += P_t V, so that one tile's products run while the other's
-// softmax does; scores, weights and O stay in TMEM, weights in the place of half the scores.  Each
+// softmax does; scores, weights and O stay in TMEM, weights in the place of their scores.  Each
 // tile has four warps, a thread to a row, which needs no exchange for its maximum and sum.  O is
 // rescaled only when a row's maximum has grown by more than 2^8 since its reference was taken: weights
 // stay below 2^8, and most blocks then leave O alone.  All blocks of all items (sequence, key head,
@@ -651,30 +651,6 @@ constexpr float kGrowth = 8.0f;    // log2 of how far a weight may exceed 1
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
 // K on even and V on odd stages: two blocks of 128 dims, four of 64
 template <int DP> constexpr int tile_stages() { return 128 * 1024 / tile_stage_bytes<DP>(); }
-// mbar_wait for the waits of the loop between products and softmax: asks again at once, where
-// try_wait may put the warp to sleep and wake it some 300 clocks late.
-__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, int* status) {
-    const uint32_t addr = smem_u32(bar);
-    uint64_t t0 = 0;
-    for (uint32_t i = 0;; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done)
-            : "r"(addr), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((i & 1023u) == 1023u) {
-            const uint64_t t = globaltimer();
-            if (t0 == 0) t0 = t;
-            if (t - t0 > kWaitLimitNs) {
-                if (status) atomicExch(status, (int)MGPU_ERR_DEVICE_TIMEOUT);
-                return false;
-            }
-        }
-    }
-}
-
 template <int DP> constexpr int tile_smem() {
     return 1024 + 2 * kTileRows * DP * 2 + tile_stages<DP>() * tile_stage_bytes<DP>() + 4 * (kTileSeqs + 1 + kTileEntries + 1);
 }
@@ -793,7 +769,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t* ring = qs + 2 * QB;
     int* seq_first = reinterpret_cast<int*>(ring + S * SB);  // [n + 1] pairs before a sequence
     int* cum = seq_first + kTileSeqs + 1;                    // [entries + 1] blocks before an entry
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2], p_bar[2][2], o_bar[2], turn_bar[2], drain_bar,
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2][2], p_bar[2][2], o_bar[2][2], drain_bar,
         seg_full[kSegments], seg_empty[kSegments];
     __shared__ Segment segs[kSegments];
     __shared__ uint32_t tmem_slot;
@@ -809,11 +785,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_bar[t], 4);
-            mbar_init(&s_bar[t], 1);
-            mbar_init(&p_bar[t][0], 4);
-            mbar_init(&p_bar[t][1], 4);
-            mbar_init(&o_bar[t], 1);
-            mbar_init(&turn_bar[t], 1);
+            for (int half = 0; half < 2; ++half) {
+                mbar_init(&s_bar[t][half], 1);
+                mbar_init(&p_bar[t][half], 4);
+                mbar_init(&o_bar[t][half], 1);
+            }
         }
         mbar_init(&drain_bar, 2);
         for (int i = 0; i < kSegments; ++i) {
@@ -905,7 +881,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, a.status)); };
-    auto poll = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_poll(bar, phase & 1u, a.status)); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
@@ -1075,19 +1050,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 for (uint32_t it = 2 * n > S ? 2 * n - S : 0; it < 2 * n; ++it) wait(&full_bar[it % S], it / S);
         } else {
             // ------------------------------------------------------------ products: a warp to a tile
+            // A block's keys are taken in halves, each with its own 64 columns of scores: the scores of a
+            // half of block kb + 1 are asked for as soon as the weights of that half of kb have been used,
+            // while the softmax is at the other half, so that it finds its next scores there.
             // Descriptors of the tile's Q, of stage 0 as keys and as values; steps and stages are added to
-            // their address fields, in units of 16 bytes.  All waits but the one for the weights come before
-            // it: from there to the commit of the next scores is what the tile's softmax waits for.  The
-            // tiles take turns: left alone they fall into step, and then products and softmax alternate
-            // instead of running side by side.
+            // their address fields, in units of 16 bytes.
             const int t = warp == 8 ? 0 : 1;
-            uint32_t q_phase = 0, p_phase = 0, turn = 0;
+            uint32_t q_phase = 0, p_phase = 0;
             const uint64_t q_desc = smem_desc(smem_u32(qs + t * QB), 16, 1024, kSwizzle128B);
             const uint64_t k_desc = smem_desc(smem_u32(ring), 16, 1024, kSwizzle128B);
             const uint64_t v_desc = smem_desc(smem_u32(ring), SLAB, 1024, kSwizzle128B);
-            const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys);
+            const uint32_t id_s = idesc_f16(kBf16, false, false, kTileRows, kTileKeys / 2);
             const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
-            const uint32_t d_s = tmem + t * kTileKeys, d_p = d_s + 64, d_o = tmem + 256 + t * 128;
+            const uint32_t d_s = tmem + t * kTileKeys, d_o = tmem + 256 + t * 128;
             const int dims = (a.D + 15) / 16;
             for (int i = 0; ok && more; ++i) {
                 ok = wait(&seg_full[i % kSegments], i / kSegments);
@@ -1105,38 +1080,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         ok = ok && wait(&clean_bar[vs], (2 * n - 1) / S);
                     }
                     if (score && kb + 1 == lo) ok = ok && wait(&q_bar[t], q_phase++);
-                    ok = ok && poll(&turn_bar[t], turn++ ^ (t == 0));
-                    const uint64_t vd = v_desc + vs * (SB >> 4);
-                    // the upper half of the keys has its weights first
+                    const uint64_t vd = v_desc + vs * (SB >> 4), kd = k_desc + ks * (SB >> 4);
 #pragma unroll 1
-                    for (int half = 1; weigh && half >= 0; --half) {
-                        ok = ok && poll(&p_bar[t][half], p_phase);
+                    for (int half = 0; half < 2; ++half) {
+                        if (weigh) ok = ok && wait(&p_bar[t][half], p_phase);
                         if (!ok) break;
                         tc_fence_after();
                         if (elect_one()) {
+                            if (weigh) {
+                                const uint64_t vh = vd + half * (kTileKeys / 2 * 128 >> 4);
 #pragma unroll
-                            for (int d = 0; d < kTileKeys / 32; ++d) {
-                                const int step = d + half * (kTileKeys / 32);
-                                umma_f16_ts(d_o, d_p + step * 8, vd + step * (2048 >> 4), id_o, kb > lo || half == 0 || d != 0);
+                                for (int d = 0; d < kTileKeys / 32; ++d)
+                                    umma_f16_ts(d_o, d_s + half * 64 + d * 8, vh + d * (2048 >> 4), id_o, kb > lo || half != 0 || d != 0);
+                                umma_commit(&o_bar[t][half]);
+                            }
+                            if (score) {
+                                const uint64_t kh = kd + half * (kTileKeys / 2 * 128 >> 4);
+#pragma unroll
+                                for (int d = 0; d < DP / 16; ++d) {
+                                    const int step = (d >> 2) * (SLAB >> 4) + (d & 3) * 2;  // Q and K have the same slabs
+                                    if (d < dims) umma_f16(d_s + half * 64, q_desc + step, kh + step, id_s, d != 0);
+                                }
+                                umma_commit(&s_bar[t][half]);
                             }
                         }
                         __syncwarp();
                     }
-                    p_phase ^= weigh;
                     if (!ok) break;
-                    tc_fence_after();
+                    p_phase ^= weigh;
                     if (elect_one()) {
-                        if (weigh && (kb + 1 >= hi || !scores)) umma_commit(&o_bar[t]);
-                        if (score) {
-                            const uint64_t kd = k_desc + ks * (SB >> 4);
-#pragma unroll
-                            for (int d = 0; d < DP / 16; ++d) {
-                                const int step = (d >> 2) * (SLAB >> 4) + (d & 3) * 2;  // Q and K have the same slabs
-                                if (d < dims) umma_f16(d_s, q_desc + step, kd + step, id_s, d != 0);
-                            }
-                            umma_commit(&s_bar[t]);
-                        }
-                        mbar_arrive(&turn_bar[1 - t]);
                         if (kb >= kb0) umma_commit(&empty_bar[vs]);
                         if (scores) umma_commit(&empty_bar[ks]);
                     }
@@ -1202,58 +1174,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const bool valid = row < g.rows[t];
             const Seen sr = valid ? seen_at(a, g.kv, g.index[t] + row / G) : Seen{0, 0};
             float m = -INFINITY, l = 0.0f;  // the reference (log2 units) and the sum of 2^(s - m)
-            for (int kb = kb0; kb < kb1; ++kb) {
-                ok = poll(&s_bar[t], s_phase++);
+            for (int j0 = kb0 * kTileKeys; j0 < kb1 * kTileKeys; j0 += kTileKeys / 2) {
+                const int half = (j0 / (kTileKeys / 2)) & 1;
+                ok = wait(&s_bar[t][half], s_phase);
                 if (!ok) break;
+                s_phase ^= half;
                 tc_fence_after();
-                // The scores are read twice in part: all 128 and the state beside them do not fit the
-                // registers.  Columns 64 .. 127 stay from the search for the maximum; the weights go to
-                // their place, 64 + key / 2, so that columns 0 .. 63 can be read again.
-                const bool all = g.whole(t, kb);
-                const int c0 = sr.lo - kb * kTileKeys, c1 = sr.hi - kb * kTileKeys;
-                auto mask = [&](uint32_t (&s)[32], int at) {
-                    if (all) return;
-#pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (at + e < c0 || at + e >= c1) s[e] = 0xFF800000u;
-                };
-                float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
-                auto search = [&](const uint32_t (&s)[32]) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        x0 = fmaxf(x0, __uint_as_float(s[e]));
-                        x1 = fmaxf(x1, __uint_as_float(s[e + 1]));
-                        x2 = fmaxf(x2, __uint_as_float(s[e + 2]));
-                        x3 = fmaxf(x3, __uint_as_float(s[e + 3]));
-                    }
-                };
+                const uint32_t cols = s_tm + half * (kTileKeys / 2);
                 uint32_t sa[32], sb[32];
-                tmem_ld32(s_tm, sa);
-                tmem_ld32(s_tm + 32, sb);
+                tmem_ld32(cols, sa);
+                tmem_ld32(cols + 32, sb);
                 tmem_ld_wait();
                 tmem_use(sa);
                 tmem_use(sb);
-                mask(sa, 0);
-                mask(sb, 32);
-                search(sa);
-                search(sb);
-                tmem_ld32(s_tm + 64, sa);
-                tmem_ld32(s_tm + 96, sb);
-                tmem_ld_wait();
-                tmem_use(sa);
-                tmem_use(sb);
-                mask(sa, 64);
-                mask(sb, 96);
-                search(sa);
-                search(sb);
+                if (j0 < g.whole_lo[t] || j0 + kTileKeys / 2 > g.whole_hi[t]) {
+                    const int c0 = sr.lo - j0, c1 = sr.hi - j0;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        if (e < c0 || e >= c1) sa[e] = 0xFF800000u;
+                        if (e + 32 < c0 || e + 32 >= c1) sb[e] = 0xFF800000u;
+                    }
+                }
+                float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    x0 = fmaxf(x0, __uint_as_float(sa[e]));
+                    x1 = fmaxf(x1, __uint_as_float(sa[e + 1]));
+                    x2 = fmaxf(x2, __uint_as_float(sb[e]));
+                    x3 = fmaxf(x3, __uint_as_float(sb[e + 1]));
+                }
                 const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2;
                 const bool grown = top > m + kGrowth;
                 if (__any_sync(0xffffffffu, grown)) {
                     const float f = grown ? ex2(m - top) : 1.0f;
                     if (grown) m = top;
                     l *= f;
-                    // the product of the block before has ended: this block's scores were issued after it
-                    if (kb > kb0) {
+                    if (j0 > kb0 * kTileKeys) {
+                        // O as the half before left it.  A barrier to each half: the phases before that one's
+                        // are then over for certain, and a parity tells only one phase from the next.
+                        ok = wait(&o_bar[t][half ^ 1], half ? o_phase : o_phase - 1);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DP; c += 16) {
                             uint32_t o[16];
@@ -1274,42 +1235,28 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, neg2);
-                        // the exponential unit takes 4 values a clock and quarter of an SM, two tiles' 256 a row more
-                        // than the products take: every kPoly-th pair goes to the FMA pipe
+                        // the exponential unit takes 4 values a clock and quarter of an SM, two tiles' 256 a row
+                        // as long as the products take: every kPoly-th pair goes to the FMA pipe
                         const float2 w2 = e % kPoly == kPoly - 1 ? ex2_poly<T>(z) : make_float2(ex2(z.x), ex2(z.y));
                         sum = __fadd2_rn(sum, w2);
                         w[e] = pack2<T>(w2.x, w2.y);
                     }
-                    tmem_st16(s_tm + 64 + at / 2, w);
+                    tmem_st16(cols + at / 2, w);
                 };
-                auto given = [&](int half) {  // the weights of half the keys are in place
-                    tmem_st_wait();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_bar[t][half]);
-                    __syncwarp();
-                };
-                uint32_t sc[32];
-                tmem_ld32(s_tm, sc);
-                weigh(sa, 64);
-                tmem_ld_wait();
-                tmem_use(sc);
-                mask(sc, 0);
-                tmem_ld32(s_tm + 32, sa);
-                weigh(sb, 96);
-                given(1);
-                weigh(sc, 0);
-                tmem_ld_wait();
-                tmem_use(sa);
-                mask(sa, 32);
-                weigh(sa, 32);
-                given(0);
+                weigh(sa, 0);
+                weigh(sb, 32);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_bar[t][half]);
+                __syncwarp();
+                o_phase += half;  // blocks so far
                 l += sum.x + sum.y;
             }
             if (!ok) break;
             const bool took = kb0 < kb1;
             if (took) {
-                ok = wait(&o_bar[t], o_phase++);
+                ok = wait(&o_bar[t][1], o_phase - 1);
                 if (!ok) break;
                 tc_fence_after();
             }

@@ -759,7 +759,7 @@ __device__ __forceinline__ bool elect_one() {
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attend_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                       const mgpu_k::AttendArgs a, int seq0) {
+                       const __grid_constant__ CUtensorMap tmQ, const mgpu_k::AttendArgs a, int seq0) {
     constexpr int SLABS = DP / 64, QB = kTileRows * DP * 2, SB = tile_stage_bytes<DP>(), SLAB = kTileKeys * 128;
     constexpr int S = tile_stages<DP>();
     constexpr int PIECE = kTileRows * (DP + 2);
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t* ring = qs + 2 * QB;
     int* seq_first = reinterpret_cast<int*>(ring + S * SB);  // [n + 1] pairs before a sequence
     int* cum = seq_first + kTileSeqs + 1;                    // [entries + 1] blocks before an entry
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2][2], p_bar[2][2], o_bar[2][2], drain_bar,
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], clean_bar[S], q_bar[2], s_bar[2][2], p_bar[2][2], o_bar[2][2], q_free[2], drain_bar,
         seg_full[kSegments], seg_empty[kSegments];
     __shared__ Segment segs[kSegments];
     __shared__ uint32_t tmem_slot;
@@ -784,7 +784,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             mbar_init(&clean_bar[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&q_bar[t], 4);
+            mbar_init(&q_bar[t], a.q_tma ? 1 : 4);
+            mbar_init(&q_free[t], 1);
             for (int half = 0; half < 2; ++half) {
                 mbar_init(&s_bar[t][half], 1);
                 mbar_init(&p_bar[t][half], 4);
@@ -799,6 +800,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         fence_mbar_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
+        if (a.q_tma) prefetch_tensormap(&tmQ);
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1064,12 +1066,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
             const uint32_t d_s = tmem + t * kTileKeys, d_o = tmem + 256 + t * 128;
             const int dims = (a.D + 15) / 16;
+            uint32_t free_phase = 0;
+            // A tile's queries: whole tokens of the key head's query heads, which lie in its rows' order.
+            // Rows beyond the tile's hold other tokens' or old values; nothing of theirs is written.
+            auto load_q = [&](const Segment& g) {
+                if (!a.q_tma || g.lo[t] >= g.hi[t]) return;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&q_bar[t], (uint32_t)(SLABS * 128 * G * per_tile));
+                    for (int slab = 0; slab < SLABS; ++slab)
+                        tma_load_3d(qs + t * QB + slab * SLAB, &tmQ, slab * 64, g.h * G, g.row0[t], &q_bar[t]);
+                }
+                __syncwarp();
+            };
             for (int i = 0; ok && more; ++i) {
                 ok = wait(&seg_full[i % kSegments], i / kSegments);
                 if (!ok) break;
                 const Segment& g = segs[i % kSegments];
                 more = g.more;
                 const int kb0 = g.kb0, kb1 = g.kb1, lo = g.lo[t], hi = g.hi[t];
+                if (i == 0) load_q(g);
                 // kb0 - 1 stands for the scores of the first block alone
                 for (int kb = kb0 - 1; kb < kb1; ++kb) {
                     const uint32_t ks = (2 * n) % S, vs = (2 * n + S - 1) % S;  // keys of kb + 1, values of kb
@@ -1102,6 +1117,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                     if (d < dims) umma_f16(d_s + half * 64, q_desc + step, kh + step, id_s, d != 0);
                                 }
                                 umma_commit(&s_bar[t][half]);
+                                if (half == 1 && kb + 2 >= hi) umma_commit(&q_free[t]);
                             }
                         }
                         __syncwarp();
@@ -1114,6 +1130,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                     __syncwarp();
                     if (scores) ++n;
+                    if (!scores && more) {
+                        // the next segment's queries, while this one's rows are written
+                        ok = (lo >= hi || wait(&q_free[t], free_phase++)) && wait(&seg_full[(i + 1) % kSegments], (i + 1) / kSegments);
+                        if (ok) load_q(segs[(i + 1) % kSegments]);
+                    }
                 }
                 if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
                 __syncwarp();
@@ -1128,30 +1149,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 lanes of TMEM
         const uint32_t s_tm = tmem + t * kTileKeys + lanes, o_tm = tmem + 256 + t * 128 + lanes;
-        // this warp's 32 rows of Q into the swizzled slabs, zeros beyond the tile's rows and the head's dims
+        // Where TMA cannot read the queries: this warp's 32 rows of Q into the swizzled slabs, zeros beyond
+        // the tile's rows and the head's dims.
         auto stage_q = [&](const Segment& g) {
-            if (g.lo[t] >= g.hi[t]) return;
+            if (a.q_tma || g.lo[t] >= g.hi[t]) return;
             constexpr int PER = DP / 8, ROWS = 32 / PER;  // 16-byte chunks of a row; rows of one access
             const int c = lane % PER, rows = g.rows[t];
             const uint32_t dst = smem_u32(qs + t * QB + (c >> 3) * SLAB);
             const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)g.row0[t] * a.ldq + (int64_t)g.h * G * a.D + c * 8;
             int r = (warp & 3) * 32 + lane / PER, token = r / G, head = r % G;
-            // A short loop of asynchronous copies: unrolled loads would wait for their instructions longer
-            // than for their data, as this is run once a segment.
 #pragma unroll 1
             for (int x = 0; x < 32; x += ROWS) {
                 const bool in = r < rows && c * 8 < a.D;
                 const uint16_t* at = in ? q + (int64_t)token * a.ldq + head * a.D : reinterpret_cast<const uint16_t*>(a.q);
                 const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                if (a.q_vec) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(at), "r"(in ? 16 : 0) : "memory");
-                } else {
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    if (in)
+                uint32_t w[4] = {0, 0, 0, 0};
+                if (in)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = (uint32_t)at[2 * e] | ((uint32_t)at[2 * e + 1] << 16);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                }
+                    for (int e = 0; e < 4; ++e) w[e] = (uint32_t)at[2 * e] | ((uint32_t)at[2 * e + 1] << 16);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                 r += ROWS;
                 head += ROWS;
                 while (head >= G) {
@@ -1159,7 +1175,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     ++token;
                 }
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_bar[t]);
@@ -1174,16 +1189,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const bool valid = row < g.rows[t];
             const Seen sr = valid ? seen_at(a, g.kv, g.index[t] + row / G) : Seen{0, 0};
             float m = -INFINITY, l = 0.0f;  // the reference (log2 units) and the sum of 2^(s - m)
-            for (int j0 = kb0 * kTileKeys; j0 < kb1 * kTileKeys; j0 += kTileKeys / 2) {
-                const int half = (j0 / (kTileKeys / 2)) & 1;
+            // The scores of half `half` at keys j0 .. are asked for; they are there after tmem_ld_wait.
+            auto fetch = [&](uint32_t (&sa)[32], uint32_t (&sb)[32], const int half) {
                 ok = wait(&s_bar[t][half], s_phase);
-                if (!ok) break;
+                if (!ok) return;
                 s_phase ^= half;
                 tc_fence_after();
-                const uint32_t cols = s_tm + half * (kTileKeys / 2);
-                uint32_t sa[32], sb[32];
-                tmem_ld32(cols, sa);
-                tmem_ld32(cols + 32, sb);
+                tmem_ld32(s_tm + half * (kTileKeys / 2), sa);
+                tmem_ld32(s_tm + half * (kTileKeys / 2) + 32, sb);
+            };
+            // Masks, the maximum, and with it the reference; O is rescaled where that moves.
+            auto refer = [&](uint32_t (&sa)[32], uint32_t (&sb)[32], const int half, int j0) {
                 tmem_ld_wait();
                 tmem_use(sa);
                 tmem_use(sb);
@@ -1213,7 +1229,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         // O as the half before left it.  A barrier to each half: the phases before that one's
                         // are then over for certain, and a parity tells only one phase from the next.
                         ok = wait(&o_bar[t][half ^ 1], half ? o_phase : o_phase - 1);
-                        if (!ok) break;
+                        if (!ok) return;
                         tc_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < DP; c += 16) {
@@ -1227,10 +1243,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
                 }
+            };
+            // The weights, in place of the scores.
+            auto weigh = [&](const uint32_t (&sa)[32], const uint32_t (&sb)[32], const int half) {
                 const float neg = m == -INFINITY ? 0.0f : -m;
                 float2 sum = make_float2(0.0f, 0.0f);
                 const float2 sc2 = make_float2(a.scale_log2, a.scale_log2), neg2 = make_float2(neg, neg);
-                auto weigh = [&](const uint32_t (&s)[32], int at) {
+                auto part = [&](const uint32_t (&s)[32], int at) {
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -1241,10 +1260,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         sum = __fadd2_rn(sum, w2);
                         w[e] = pack2<T>(w2.x, w2.y);
                     }
-                    tmem_st16(cols + at / 2, w);
+                    tmem_st16(s_tm + half * (kTileKeys / 2) + at / 2, w);
                 };
-                weigh(sa, 0);
-                weigh(sb, 32);
+                part(sa, 0);
+                part(sb, 32);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -1252,6 +1271,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 __syncwarp();
                 o_phase += half;  // blocks so far
                 l += sum.x + sum.y;
+            };
+            for (int j0 = kb0 * kTileKeys; j0 < kb1 * kTileKeys; j0 += kTileKeys / 2) {
+                const int half = (j0 / (kTileKeys / 2)) & 1;
+                uint32_t sa[32], sb[32];
+                fetch(sa, sb, half);
+                if (!ok) break;
+                refer(sa, sb, half, j0);
+                if (!ok) break;
+                weigh(sa, sb, half);
             }
             if (!ok) break;
             const bool took = kb0 < kb1;
@@ -1407,8 +1435,15 @@ cudaError_t launch_tiles(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, cons
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    // [tokens][heads][dims] of q; a box is a tile's tokens, a key head's query heads and 64 dims
+    const int group = a.hq / a.hkv;
+    const int64_t dims[3] = {a.D, a.hq, a.batch.n_tokens}, strides[2] = {(int64_t)a.D * 2, a.ldq * 2};
+    const int box[3] = {64, group, kTileRows / group};
+    CUtensorMap mq = {};
+    mgpu_k::AttendArgs b = a;
+    b.q_tma = a.q_vec && mgpu_k::make_tensor_map_u16_3d(&mq, a.q, dims, strides, box, true);
     for (int seq0 = 0; seq0 < a.batch.n_seqs && e == cudaSuccess; seq0 += kTileSeqs)
-        e = cudaLaunchKernelEx(&cfg, kern, mk, mv, a, seq0);
+        e = cudaLaunchKernelEx(&cfg, kern, mk, mv, mq, b, seq0);
     return e;
 }
 

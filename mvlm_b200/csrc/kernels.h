@@ -136,7 +136,7 @@ struct AttendArgs {
     float* partials;        // attend_scratch_bytes
     unsigned int* tickets;  // eight per CTA, zero between calls (the kernels leave them so)
     // set by paged_attention
-    int box_rows, page_shift, max_rows, q_pairs, out_pairs, q_vec, out_vec, out_wide;
+    int box_rows, page_shift, max_rows, q_pairs, out_pairs, q_vec, q_tma, out_vec, out_wide;
 };
 // Whether some sequence may have more rows (new tokens x query heads of a key head) than the
 // kernel for few rows takes, and the scratch that needs.

@@ -95,6 +95,17 @@ template <> __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A barrier of `threads` threads that says whether any of them brought `p`.
+__device__ __forceinline__ bool named_barrier_or(int id, int threads, bool p) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(r)
+        : "r"((uint32_t)p), "r"(id), "r"(threads)
+        : "memory");
+    return r != 0;
+}
+
 // ------------------------------------------------------------------ few rows --------
 // At most 16 rows to a key head (a decode step): bound by reading K and V once from HBM, 4 G
 // operations to a byte pair.  The blocks of all (sequence, key head) items are laid end to end and
@@ -112,9 +123,18 @@ template <int DP> constexpr int rows_stage_bytes() { return 2 * kBlock * DP * 2;
 // other could when they shared a stage.
 template <int DP> constexpr int rows_stages() { return 128 * 1024 / rows_stage_bytes<DP>(); }
 template <int DP> constexpr int rows_pitch() { return DP + 4; }
+template <int DP> constexpr int rows_q_pitch() { return DP * 2 + 16; }  // bytes; rows start in different banks
+constexpr int kItems = 4;  // handed out ahead
 template <int DP> constexpr int rows_smem() {
-    return 1024 + rows_stages<DP>() * rows_stage_bytes<DP>() + 4 * kRowsMax * rows_pitch<DP>() * 4;
+    return 1024 + rows_stages<DP>() * rows_stage_bytes<DP>() + kRowsWarps * kRowsMax * rows_pitch<DP>() * 4 +
+           kItems * kRowsMax * rows_q_pitch<DP>();
 }
+
+// What a CTA does of one item, handed out by its first loading warp.
+struct Item {
+    SeqView s;
+    int seq, h, base, k0, k1, blocks, begin, more;  // base: the item's first block; begin: its place among all blocks
+};
 
 __device__ __forceinline__ int first_block(const mgpu_k::AttendArgs& a, const SeqView& s) {
     return seen_by(a, s, 0).lo / kBlock;
@@ -141,16 +161,19 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     constexpr int SLABS = DP / 64, SLAB = kBlock * 128;  // 64 dims x 64 keys, 128-byte rows, swizzled
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
     static_assert(S % 2 == 0, "a stage belongs to one group of warps");
+    constexpr int QP = rows_q_pitch<DP>();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     float* scratch = reinterpret_cast<float*>(ring + S * SB);
-    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S];
+    uint8_t* q_smem = reinterpret_cast<uint8_t*>(scratch + kRowsWarps * kRowsMax * PITCH);
+    __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], item_full[kItems], item_empty[kItems];
+    __shared__ Item slots[kItems];
     __shared__ int counts[kSeqCap];
     __shared__ long long warp_sum[kRowsWarps + 2];
     __shared__ bool last;
     __shared__ int start_before;
     __shared__ int start_seq;
-    __shared__ float sm_m[kRowsWarps][kRowsMax], sm_l[kRowsWarps][kRowsMax];
+    __shared__ float sm_m[2][kRowsWarps][kRowsMax], sm_l[2][kRowsWarps][kRowsMax];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.hq / a.hkv;
 
@@ -159,6 +182,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             mbar_init(&full_bar[s], 2);
             mbar_init(&empty_bar[s], kRowsWarps / 2);
         }
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(&item_full[i], 1);
+            mbar_init(&item_empty[i], kRowsWarps + 1);  // the warps that score, and the other loading warp
+        }
         fence_mbar_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
@@ -166,6 +193,9 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     }
     // the step's contents and the cache may be the preceding kernel's
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    // dims beyond the head's stay zero, whatever the rows become
+    for (int x = tid; x < kItems * kRowsMax * QP / 16; x += kRowsThreads) reinterpret_cast<uint4*>(q_smem)[x] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
     // ---- this CTA's share of all blocks
     auto count = [&](int b) {
         bool bad = false;
@@ -188,8 +218,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const int total = (int)(sum_all * a.hkv);  // the host has bounded it
     const int shares = min((int)gridDim.x, total);  // none is empty
     if ((int)blockIdx.x >= shares) return;
-    const int quota = total / shares, more = total % shares;  // the first `more` shares have one block more
-    auto share = [&](int c) { return c * quota + min(c, more); };
+    const int quota = total / shares, extra = total % shares;  // the first `extra` shares have one block more
+    auto share = [&](int c) { return c * quota + min(c, extra); };
     const int begin = share(blockIdx.x), end = share(blockIdx.x + 1);
     if (warp == 0) {
         // the sequence that holds block `begin`, and the blocks of the sequences before it
@@ -228,10 +258,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         w.h = 0;
         w.k = 0;
     };
-    Walk w;
-    enter(w, start_seq);
-    w.h = (begin - start_before) / w.blocks;
-    w.k = (begin - start_before) % w.blocks;
+    auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, a.status)); };
 
     if (warp >= kRowsWarps) {
         // ---------------------------------------------------------------- loads
@@ -240,242 +267,261 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         const bool loads = lane < chunks * SLABS;
         const int first = (lane % chunks) * rows, slab = lane / chunks;
         const CUtensorMap* map = side ? &tmV : &tmK;
-        int base = first_block(a, w.s);
-        // the page of this lane's chunk of block k, asked for one block ahead; chunks past the end are
+        // the page of this lane's chunk of a block, asked for one block ahead; chunks past the end are
         // read from outside the map, which gives zeros
-        auto key = [&] { return (base + w.k) * kBlock + first; };
-        auto page_of = [&](int j) {
-            if (!loads || j >= w.s.kv) return -2;
-            return __ldg(a.batch.page_table + (int64_t)w.b * a.batch.max_pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size));
+        auto page_of = [&](const Item& it, int j) {
+            if (!loads || j >= it.s.kv) return -2;
+            return __ldg(a.batch.page_table + (int64_t)it.seq * a.batch.max_pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size));
         };
-        int j = key(), page = page_of(j);
-        for (int pos = begin, it = 0; pos < end; ++pos, ++it) {
-            const uint32_t st = it % S;
-            if (!__all_sync(0xffffffffu, mbar_wait(&empty_bar[st], ((it / S) & 1u) ^ 1u, a.status))) return;
-            if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB / 2);
-            __syncwarp();
-            if (loads) {
-                const bool in = page >= 0 && page < a.num_pages;
-                if (!in && page != -2) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-                const int z = in ? page * a.hkv + w.h : a.num_pages * a.hkv;
-                const int y = in ? (a.page_shift >= 0 ? j & ((1 << a.page_shift) - 1) : j % a.page_size) : 0;
-                tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);
-            }
-            if (++w.k == w.blocks && pos + 1 < end) {
-                w.k = 0;
-                if (++w.h == a.hkv) {
-                    enter(w, w.b + 1);
-                    base = first_block(a, w.s);
-                }
-            }
-            j = key();
-            if (pos + 1 < end) page = page_of(j);
+        Walk w;
+        if (side == 0) {
+            enter(w, start_seq);
+            w.h = (begin - start_before) / w.blocks;
+            w.k = (begin - start_before) % w.blocks;
         }
+        bool ok = true, more = true;
+        uint32_t n = 0;  // blocks so far
+        int pos = begin;
+        for (int i = 0; ok && more; ++i) {
+            Item& slot = slots[i % kItems];
+            Item it;
+            if (side == 0) {
+                it.s = w.s;
+                it.seq = w.b;
+                it.h = w.h;
+                it.base = first_block(a, w.s);
+                it.k0 = w.k;
+                it.k1 = min(w.blocks, w.k + (end - pos));
+                it.blocks = w.blocks;
+                it.begin = pos - w.k;
+                pos += it.k1 - it.k0;
+                it.more = pos < end;
+                ok = wait(&item_empty[i % kItems], (i / kItems) ^ 1);
+                if (!ok) break;
+                const int R = it.s.n * G;
+                if (lane == 0) {
+                    slot = it;
+                    if (a.q_vec) mbar_arrive_expect_tx(&item_full[i % kItems], (uint32_t)(R * a.D * 2));
+                }
+                __syncwarp();
+                if (!a.q_vec) {  // no 16-byte boundaries
+                    for (int e = lane; e < R * a.D; e += 32) {
+                        const int r = e / a.D, d = e % a.D;
+                        reinterpret_cast<uint16_t*>(q_smem + ((i % kItems) * kRowsMax + r) * QP)[d] =
+                            reinterpret_cast<const uint16_t*>(a.q)[(int64_t)(it.s.q0 + r / G) * a.ldq + (int64_t)(it.h * G + r % G) * a.D + d];
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&item_full[i % kItems]);
+                } else if (lane < R)  // the item's queries, a row to a lane
+                    bulk_g2s(q_smem + ((i % kItems) * kRowsMax + lane) * QP,
+                             reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.s.q0 + lane / G) * a.ldq + (int64_t)(it.h * G + lane % G) * a.D,
+                             (uint32_t)a.D * 2, &item_full[i % kItems]);
+                w.k = 0;
+                if (++w.h == a.hkv && it.more) enter(w, w.b + 1);
+            } else {
+                ok = wait(&item_full[i % kItems], i / kItems);
+                if (!ok) break;
+                it = slot;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
+            }
+            more = it.more;
+            int j = (it.base + it.k0) * kBlock + first, page = page_of(it, j);
+            for (int k = it.k0; k < it.k1; ++k, ++n) {
+                const uint32_t st = n % S;
+                ok = wait(&empty_bar[st], (n / S) ^ 1);
+                if (!ok) break;
+                if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], SB / 2);
+                __syncwarp();
+                if (loads) {
+                    const bool in = page >= 0 && page < a.num_pages;
+                    if (!in && page != -2) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                    const int z = in ? page * a.hkv + it.h : a.num_pages * a.hkv;
+                    const int y = in ? (a.page_shift >= 0 ? j & ((1 << a.page_shift) - 1) : j % a.page_size) : 0;
+                    tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);
+                }
+                j += kBlock;
+                if (k + 1 < it.k1) page = page_of(it, j);
+                __syncwarp();
+            }
+        }
+        // a wait ran out: the copies under way still have to land before the CTA may end
+        if (!ok)
+            for (uint32_t x = n > S ? n - S : 0; x < n; ++x) wait(&full_bar[x % S], x / S);
         return;
     }
 
     // -------------------------------------------------------------------- scores and sums
     const int group = warp >> 2, part = warp & 3;  // blocks of one parity; 16 keys of each
     const int g = lane >> 2, c2 = 2 * (lane & 3);  // this thread's rows g and g + 8, and first column
-    bool dead = false;  // a wait ran out: walk on without data, so that every barrier is still met
+    // Two items' states of up to 8 rows fit the scratch, and the barrier of the item between says that the
+    // last ones have been read.  Where an item may have more rows, each takes both places, and a barrier more.
+    const bool wide = (long long)a.batch.max_q_len * G > 8;
+    const int room = wide ? kRowsMax : 8;
     uint32_t it = 0;
-    for (int pos = begin; pos < end;) {
-        const int k0 = w.k, k1 = min(w.blocks, k0 + (end - pos));
-        const int base = first_block(a, w.s), R = w.s.n * G;
-        // queries: A fragments of every 16 dims
-        uint32_t qf[DP / 16][4];
+    struct {
+        SeqView s;
+        int h, blocks;
+    } w;
+    for (int i = 0, more = 1; more; ++i) {
+        const int slot = i % kItems, turn = i & 1;
+        int k0 = 0, k1 = 0, base = 0, item_begin = 0, R = 0;
         Seen sr[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = g + 8 * i;
-            const int64_t at = r < R ? (int64_t)(w.s.q0 + r / G) * a.ldq + (int64_t)(w.h * G + r % G) * a.D : 0;
-            const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + at;
-            sr[i] = r < R ? seen_by(a, w.s, r / G) : Seen{0, 0};
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int d = 16 * k + 8 * half + c2;
-                    uint32_t v = 0;
-                    if (r < R && d < a.D)
-                        v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(q + d) : (uint32_t)q[d] | ((uint32_t)q[d + 1] << 16);
-                    qf[k][2 * half + i] = v;
-                }
-        }
-        // keys [s1.lo, s0.hi) are seen by every row
-        const Seen s0 = seen_by(a, w.s, 0), s1 = seen_by(a, w.s, w.s.n - 1);
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DP / 8][4];
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][e] = 0.0f;
-
-        for (int k = k0; k < k1; ++k, ++it) {
-            if ((int)(it & 1u) != group || dead) continue;
-            const uint32_t st = it % S;
-            if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[st], (it / S) & 1u, a.status))) {
-                dead = true;
-                continue;
-            }
-            const uint32_t kb = smem_u32(ring + st * SB), vb = kb + SB / 2;
-            const int j0 = (base + k) * kBlock + 16 * part;  // this warp's first key
-            // S = Q K^T: 16 rows x 16 keys
-            float sc[2][4] = {};
+        bool dead = !wait(&item_full[slot], i / kItems);  // a wait ran out: all warps leave at the item's barrier
+        if (!dead) {
+            k0 = slots[slot].k0;
+            k1 = slots[slot].k1;
+            base = slots[slot].base;
+            item_begin = slots[slot].begin;
+            w.s = slots[slot].s;
+            w.h = slots[slot].h;
+            w.blocks = slots[slot].blocks;
+            more = slots[slot].more;
+            R = w.s.n * G;
+            // Queries: A fragments of every 16 dims.  Rows beyond the item's hold older ones; nothing of
+            // theirs is written.
+            uint32_t qf[DP / 16][4];
+            const uint32_t qa = smem_u32(q_smem) + (slot * kRowsMax + (lane & 15)) * QP + (lane >> 4) * 16;
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) {
-                // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step
-                const int row = 16 * part + (lane & 7) + ((lane >> 4) << 3), ch = (2 * d + ((lane >> 3) & 1)) & 7;
-                uint32_t b[4];
-                ldsm4(b, kb + (d / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
-                mma16816<T>(sc[0], qf[d], b[0], b[1]);
-                mma16816<T>(sc[1], qf[d], b[2], b[3]);
-            }
-            const bool whole = j0 >= s1.lo && j0 + 16 <= s0.hi;
+            for (int k = 0; k < DP / 16; ++k) ldsm4(qf[k], qa + 32 * k);
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sc[n][e] *= a.scale_log2;
-                    const int j = j0 + 8 * n + c2 + (e & 1);
-                    if (!whole && (j < sr[e >> 1].lo || j >= sr[e >> 1].hi)) sc[n][e] = -INFINITY;
+            for (int x = 0; x < 2; ++x) sr[x] = g + 8 * x < R ? seen_by(a, w.s, (g + 8 * x) / G) : Seen{0, 0};
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[slot]);
+            // keys [s1.lo, s0.hi) are seen by every row
+            const Seen s0 = seen_by(a, w.s, 0), s1 = seen_by(a, w.s, w.s.n - 1);
+            for (int k = k0; k < k1; ++k, ++it) {
+                if ((int)(it & 1u) != group || dead) continue;
+                const uint32_t st = it % S;
+                if (!__all_sync(0xffffffffu, mbar_wait(&full_bar[st], (it / S) & 1u, a.status))) {
+                    dead = true;
+                    continue;
                 }
-            // running maximum and sum
-            uint32_t pf[4];
+                const uint32_t kb = smem_u32(ring + st * SB), vb = kb + SB / 2;
+                const int j0 = (base + k) * kBlock + 16 * part;  // this warp's first key
+                // S = Q K^T: 16 rows x 16 keys
+                float sc[2][4] = {};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float top = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float mn = fmaxf(m[i], top), mu = mn == -INFINITY ? 0.0f : mn;
-                const float r = ex2(m[i] - mu);
-                m[i] = mn;
-                float p[4];
+                for (int d = 0; d < DP / 16; ++d) {
+                    // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step
+                    const int row = 16 * part + (lane & 7) + ((lane >> 4) << 3), ch = (2 * d + ((lane >> 3) & 1)) & 7;
+                    uint32_t b[4];
+                    ldsm4(b, kb + (d / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
+                    mma16816<T>(sc[0], qf[d], b[0], b[1]);
+                    mma16816<T>(sc[1], qf[d], b[2], b[3]);
+                }
+                const bool whole = j0 >= s1.lo && j0 + 16 <= s0.hi;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[e] = ex2(sc[e >> 1][2 * i + (e & 1)] - mu);
-                l[i] = l[i] * r + ((p[0] + p[1]) + (p[2] + p[3]));
-                pf[i] = pack2<T>(p[0], p[1]);
-                pf[2 + i] = pack2<T>(p[2], p[3]);
-                if (__any_sync(0xffffffffu, r != 1.0f)) {
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int n = 0; n < DP / 8; ++n) {
-                        o[n][2 * i] *= r;
-                        o[n][2 * i + 1] *= r;
+                    for (int e = 0; e < 4; ++e) {
+                        sc[n][e] *= a.scale_log2;
+                        const int j = j0 + 8 * n + c2 + (e & 1);
+                        if (!whole && (j < sr[e >> 1].lo || j >= sr[e >> 1].hi)) sc[n][e] = -INFINITY;
                     }
-                }
-            }
-            if (!whole) {
-                // Values that some row does not see: a weight of 0 times NaN or Inf is not 0, so those
-                // are taken out of the block and added to the rows that see them.
-                const int row = 16 * part + (lane >> 1);
-                bool found = false;
+                // running maximum and sum
+                uint32_t pf[4];
 #pragma unroll
-                for (int i = 0; i < DP / 16; ++i) {
-                    const int ch = (lane & 1) * (DP / 16) + i;
-                    const uint4 v = *reinterpret_cast<const uint4*>(ring + st * SB + SB / 2 + (ch >> 3) * SLAB + row * 128 +
-                                                                    (((ch & 7) ^ (row & 7)) << 4));
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                for (int i = 0; i < 2; ++i) {
+                    float top = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float mn = fmaxf(m[i], top), mu = mn == -INFINITY ? 0.0f : mn;
+                    const float r = ex2(m[i] - mu);
+                    m[i] = mn;
+                    float p[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) found |= odd16(x[e], kBf16) || odd16(x[e] >> 16, kBf16);
-                }
-                if (__any_sync(0xffffffffu, found)) {
-                    for (int j = 0; j < 16; ++j) {
-                        const int r = 16 * part + j;
-                        const bool s_lo = j0 + j >= sr[0].lo && j0 + j < sr[0].hi, s_hi = j0 + j >= sr[1].lo && j0 + j < sr[1].hi;
+                    for (int e = 0; e < 4; ++e) p[e] = ex2(sc[e >> 1][2 * i + (e & 1)] - mu);
+                    l[i] = l[i] * r + ((p[0] + p[1]) + (p[2] + p[3]));
+                    pf[i] = pack2<T>(p[0], p[1]);
+                    pf[2 + i] = pack2<T>(p[2], p[3]);
+                    if (__any_sync(0xffffffffu, r != 1.0f)) {
 #pragma unroll
                         for (int n = 0; n < DP / 8; ++n) {
-                            const uint32_t v = *reinterpret_cast<const uint32_t*>(ring + st * SB + SB / 2 + (n >> 3) * SLAB +
-                                                                                 r * 128 + (((n & 7) ^ (r & 7)) << 4) + 2 * c2);
-                            const float2 f = unpack2<T>(v);
-                            const float x = odd16(v, kBf16) ? f.x : 0.0f, y = odd16(v >> 16, kBf16) ? f.y : 0.0f;
-                            if (s_lo) { o[n][0] += x; o[n][1] += y; }
-                            if (s_hi) { o[n][2] += x; o[n][3] += y; }
+                            o[n][2 * i] *= r;
+                            o[n][2 * i + 1] *= r;
                         }
                     }
-                    __syncwarp();
+                }
+                if (__builtin_expect(!whole, 0)) {
+                    // Values that some row does not see: a weight of 0 times NaN or Inf is not 0, so those
+                    // are taken out of the block and added to the rows that see them.
+                    const int row = 16 * part + (lane >> 1);
+                    bool found = false;
+#pragma unroll
                     for (int i = 0; i < DP / 16; ++i) {
                         const int ch = (lane & 1) * (DP / 16) + i;
-                        uint16_t* v = reinterpret_cast<uint16_t*>(ring + st * SB + SB / 2 + (ch >> 3) * SLAB + row * 128 +
-                                                                  (((ch & 7) ^ (row & 7)) << 4));
-                        for (int e = 0; e < 8; ++e)
-                            if (odd16(v[e], kBf16)) v[e] = 0;
+                        const uint4 v = *reinterpret_cast<const uint4*>(ring + st * SB + SB / 2 + (ch >> 3) * SLAB + row * 128 +
+                                                                        (((ch & 7) ^ (row & 7)) << 4));
+                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) found |= odd16(x[e], kBf16) || odd16(x[e] >> 16, kBf16);
                     }
-                    fence_proxy_async_smem();  // before the ring's next load of this stage
-                    __syncwarp();
+                    if (__builtin_expect(__any_sync(0xffffffffu, found), 0)) {
+                        for (int j = 0; j < 16; ++j) {
+                            const int r = 16 * part + j;
+                            const bool s_lo = j0 + j >= sr[0].lo && j0 + j < sr[0].hi, s_hi = j0 + j >= sr[1].lo && j0 + j < sr[1].hi;
+#pragma unroll
+                            for (int n = 0; n < DP / 8; ++n) {
+                                const uint32_t v = *reinterpret_cast<const uint32_t*>(ring + st * SB + SB / 2 + (n >> 3) * SLAB +
+                                                                                     r * 128 + (((n & 7) ^ (r & 7)) << 4) + 2 * c2);
+                                const float2 f = unpack2<T>(v);
+                                const float x = odd16(v, kBf16) ? f.x : 0.0f, y = odd16(v >> 16, kBf16) ? f.y : 0.0f;
+                                if (s_lo) { o[n][0] += x; o[n][1] += y; }
+                                if (s_hi) { o[n][2] += x; o[n][3] += y; }
+                            }
+                        }
+                        __syncwarp();
+                        for (int i = 0; i < DP / 16; ++i) {
+                            const int ch = (lane & 1) * (DP / 16) + i;
+                            uint16_t* v = reinterpret_cast<uint16_t*>(ring + st * SB + SB / 2 + (ch >> 3) * SLAB + row * 128 +
+                                                                      (((ch & 7) ^ (row & 7)) << 4));
+                            for (int e = 0; e < 8; ++e)
+                                if (odd16(v[e], kBf16)) v[e] = 0;
+                        }
+                        fence_proxy_async_smem();  // before the ring's next load of this stage
+                        __syncwarp();
+                    }
                 }
-            }
-            // O += P V
+                // O += P V
 #pragma unroll
-            for (int n = 0; n < DP / 16; ++n) {
-                // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step, transposed
-                const int row = 16 * part + (lane & 7) + (((lane >> 3) & 1) << 3), ch = (2 * n + (lane >> 4)) & 7;
-                uint32_t b[4];
-                ldsm4_t(b, vb + (n / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
-                mma16816<T>(o[2 * n], pf, b[0], b[1]);
-                mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+                for (int n = 0; n < DP / 16; ++n) {
+                    // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step, transposed
+                    const int row = 16 * part + (lane & 7) + (((lane >> 3) & 1) << 3), ch = (2 * n + (lane >> 4)) & 7;
+                    uint32_t b[4];
+                    ldsm4_t(b, vb + (n / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
+                    mma16816<T>(o[2 * n], pf, b[0], b[1]);
+                    mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty_bar[st]);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty_bar[st]);
         }
-
-        // ---- the eight warps' states join
+        // ---- the eight warps' states join: each leaves its own, and whoever writes a value weighs them
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        for (int x = 0; x < 2; ++x) {
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
             if ((lane & 3) == 0) {
-                sm_m[warp][g + 8 * i] = m[i];
-                sm_l[warp][g + 8 * i] = l[i];
+                sm_m[turn][warp][g + 8 * x] = m[x];
+                sm_l[turn][warp][g + 8 * x] = l[x];
             }
         }
-        named_barrier_sync(1, 32 * kRowsWarps);
+        float* states = scratch + (wide ? 0 : turn * kRowsWarps * 8 * PITCH);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float top = -INFINITY;
+        for (int x = 0; x < 2; ++x)
+            if (g + 8 * x < R)
 #pragma unroll
-            for (int x = 0; x < kRowsWarps; ++x) top = fmaxf(top, sm_m[x][g + 8 * i]);
-            const float f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - top);
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-                o[n][2 * i] *= f;
-                o[n][2 * i + 1] *= f;
-            }
-        }
-        float* mine = scratch + part * kRowsMax * PITCH;
-        auto put = [&] {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (g + 8 * i < R)
-#pragma unroll
-                    for (int n = 0; n < DP / 8; ++n)
-                        *reinterpret_cast<float2*>(mine + (g + 8 * i) * PITCH + 8 * n + c2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-        };
-        if (group == 1) put();
-        named_barrier_sync(1, 32 * kRowsWarps);
-        if (group == 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (g + 8 * i < R)
-#pragma unroll
-                    for (int n = 0; n < DP / 8; ++n) {
-                        const float2 v = *reinterpret_cast<const float2*>(mine + (g + 8 * i) * PITCH + 8 * n + c2);
-                        o[n][2 * i] += v.x;
-                        o[n][2 * i + 1] += v.y;
-                    }
-            put();  // each thread reads and then writes its own places
-        }
-        named_barrier_sync(1, 32 * kRowsWarps);
+                for (int n = 0; n < DP / 8; ++n)
+                    *reinterpret_cast<float2*>(states + (warp * room + g + 8 * x) * PITCH + 8 * n + c2) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
+        if (named_barrier_or(1, 32 * kRowsWarps, dead)) break;
         // ---- rows out, or this share's state of an item that other CTAs have parts of
         const bool complete = k0 == 0 && k1 == w.blocks;
-        auto state = [&](int r, float* top, float* den) {
-            float t = -INFINITY, d = 0.0f;
-#pragma unroll
-            for (int x = 0; x < kRowsWarps; ++x) t = fmaxf(t, sm_m[x][r]);
-            if (t > -INFINITY)
-#pragma unroll
-                for (int x = 0; x < kRowsWarps; ++x) d += sm_l[x][r] * ex2(sm_m[x][r] - t);
-            *top = t;
-            *den = d;
-        };
         auto write = [&](int r, int d, float x, float y) {
             T* out = reinterpret_cast<T*>(a.out) + (int64_t)(w.s.q0 + r / G) * a.ldo + (int64_t)(w.h * G + r % G) * a.D + d;
             if (a.out_pairs) {
@@ -487,20 +533,23 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         };
         // pieces of CTA c: slot 2c for the item its share begins in, 2c + 1 for a later one
         constexpr int PIECE = kRowsMax * (DP + 2);
-        const int item_begin = pos - k0;
         float* piece = a.partials + (2 * (int64_t)blockIdx.x + (item_begin > begin ? 1 : 0)) * PIECE;
         for (int e = tid; e < R * (DP / 2); e += 32 * kRowsWarps) {
             const int r = e / (DP / 2), d = 2 * (e % (DP / 2));
             if (d >= a.D) continue;
-            float2 v = make_float2(0.0f, 0.0f);
+            float top = -INFINITY, den = 0.0f;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const float2 t = *reinterpret_cast<const float2*>(scratch + (x * kRowsMax + r) * PITCH + d);
-                v.x += t.x;
-                v.y += t.y;
+            for (int x = 0; x < kRowsWarps; ++x) top = fmaxf(top, sm_m[turn][x][r]);
+            const float mu = top == -INFINITY ? 0.0f : top;
+            float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll 2
+            for (int x = 0; x < kRowsWarps; ++x) {
+                const float f = ex2(sm_m[turn][x][r] - mu);
+                const float2 t = *reinterpret_cast<const float2*>(states + (x * room + r) * PITCH + d);
+                v.x += t.x * f;
+                v.y += t.y * f;
+                den += sm_l[turn][x][r] * f;
             }
-            float top, den;
-            state(r, &top, &den);
             if (complete) {
                 // a row that saw nothing has den = 0: its zeros stay zeros
                 const float inv = den > 0.0f ? 1.0f / den : 0.0f;
@@ -515,8 +564,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
         if (!complete) {
             // CTAs c0 .. c1 have the item's blocks; the last of them to arrive joins their pieces in order
-            const int cut = more * (quota + 1);
-            auto owner = [&](int x) { return x < cut ? x / (quota + 1) : more + (x - cut) / quota; };
+            const int cut = extra * (quota + 1);
+            auto owner = [&](int x) { return x < cut ? x / (quota + 1) : extra + (x - cut) / quota; };
             const int c0 = owner(item_begin), c1 = owner(item_begin + w.blocks - 1), pieces = c1 - c0 + 1;
             __threadfence();
             named_barrier_sync(1, 32 * kRowsWarps);
@@ -589,10 +638,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 }
             }
         }
-        named_barrier_sync(1, 32 * kRowsWarps);  // scratch and the joined states are free again
-        pos += k1 - k0;
-        w.k = 0;
-        if (++w.h == a.hkv && pos < end) enter(w, w.b + 1);
+        if (wide || !complete) named_barrier_sync(1, 32 * kRowsWarps);  // the places are free again
     }
 }
 

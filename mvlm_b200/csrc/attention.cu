@@ -112,7 +112,7 @@ __device__ __forceinline__ bool named_barrier_or(int id, int threads, bool p) {
 // cut into equal shares, one per CTA, whatever the sequences' lengths; an item cut by a share's end
 // is joined by the last of its CTAs to finish.  One warp feeds a ring of blocks by TMA; eight warps
 // in two groups take every other block, a warp 16 of its keys, each with its own running state.
-constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 2);
+constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 3);  // then: keys, values, items
 constexpr int kRowsMax = 16;
 constexpr int kSeqCap = 1024;  // sequences whose block counts are kept in shared memory
 
@@ -130,7 +130,7 @@ template <int DP> constexpr int rows_smem() {
            kItems * kRowsMax * rows_q_pitch<DP>();
 }
 
-// What a CTA does of one item, handed out by its first loading warp.
+// What a CTA does of one item, handed out by a warp of its own.
 struct Item {
     SeqView s;
     int seq, h, base, k0, k1, blocks, begin, more;  // base: the item's first block; begin: its place among all blocks
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     __shared__ __align__(8) uint64_t full_bar[S], empty_bar[S], item_full[kItems], item_empty[kItems];
     __shared__ Item slots[kItems];
     __shared__ int counts[kSeqCap];
-    __shared__ long long warp_sum[kRowsWarps + 2];
+    __shared__ long long warp_sum[kRowsThreads / 32];
     __shared__ bool last;
     __shared__ int start_before;
     __shared__ int start_seq;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
         for (int i = 0; i < kItems; ++i) {
             mbar_init(&item_full[i], 1);
-            mbar_init(&item_empty[i], kRowsWarps + 1);  // the warps that score, and the other loading warp
+            mbar_init(&item_empty[i], kRowsWarps + 2);  // the warps that score and those that load
         }
         fence_mbar_init();
         prefetch_tensormap(&tmK);
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
     long long sum_all = 0;
-    for (int x = 0; x < kRowsWarps + 2; ++x) sum_all += warp_sum[x];
+    for (int x = 0; x < kRowsThreads / 32; ++x) sum_all += warp_sum[x];
     const int total = (int)(sum_all * a.hkv);  // the host has bounded it
     const int shares = min((int)gridDim.x, total);  // none is empty
     if ((int)blockIdx.x >= shares) return;
@@ -260,6 +260,48 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     };
     auto wait = [&](uint64_t* bar, uint32_t phase) { return __all_sync(0xffffffffu, mbar_wait(bar, phase & 1u, a.status)); };
 
+    if (warp == kRowsWarps + 2) {
+        // ---------------------------------------------------------------- items, and their queries
+        Walk w;
+        enter(w, start_seq);
+        w.h = (begin - start_before) / w.blocks;
+        w.k = (begin - start_before) % w.blocks;
+        for (int i = 0, pos = begin; pos < end; ++i) {
+            const int x = i % kItems, k1 = min(w.blocks, w.k + (end - pos)), R = w.s.n * G;
+            if (!wait(&item_empty[x], (i / kItems) ^ 1)) break;
+            if (lane == 0) {
+                Item& it = slots[x];
+                it.s = w.s;
+                it.seq = w.b;
+                it.h = w.h;
+                it.base = first_block(a, w.s);
+                it.k0 = w.k;
+                it.k1 = k1;
+                it.blocks = w.blocks;
+                it.begin = pos - w.k;
+                it.more = pos + k1 - w.k < end;
+                if (a.q_vec) mbar_arrive_expect_tx(&item_full[x], (uint32_t)(R * a.D * 2));
+            }
+            __syncwarp();
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)w.s.q0 * a.ldq + (int64_t)w.h * G * a.D;
+            uint8_t* to = q_smem + x * kRowsMax * QP;
+            if (a.q_vec) {  // a row to a lane
+                if (lane < R) bulk_g2s(to + lane * QP, q + (int64_t)(lane / G) * a.ldq + (lane % G) * a.D, (uint32_t)a.D * 2, &item_full[x]);
+            } else {  // no 16-byte boundaries
+                for (int e = lane; e < R * a.D; e += 32) {
+                    const int r = e / a.D, d = e % a.D;
+                    reinterpret_cast<uint16_t*>(to + r * QP)[d] = q[(int64_t)(r / G) * a.ldq + (r % G) * a.D + d];
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&item_full[x]);
+            }
+            __syncwarp();
+            pos += k1 - w.k;
+            w.k = 0;
+            if (++w.h == a.hkv && pos < end) enter(w, w.b + 1);
+        }
+        return;
+    }
     if (warp >= kRowsWarps) {
         // ---------------------------------------------------------------- loads
         // one warp for the keys, one for the values; a lane loads one chunk (rows of one page) of a slab
@@ -267,66 +309,22 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         const bool loads = lane < chunks * SLABS;
         const int first = (lane % chunks) * rows, slab = lane / chunks;
         const CUtensorMap* map = side ? &tmV : &tmK;
-        // the page of this lane's chunk of a block, asked for one block ahead; chunks past the end are
-        // read from outside the map, which gives zeros
-        auto page_of = [&](const Item& it, int j) {
-            if (!loads || j >= it.s.kv) return -2;
-            return __ldg(a.batch.page_table + (int64_t)it.seq * a.batch.max_pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size));
-        };
-        Walk w;
-        if (side == 0) {
-            enter(w, start_seq);
-            w.h = (begin - start_before) / w.blocks;
-            w.k = (begin - start_before) % w.blocks;
-        }
         bool ok = true, more = true;
         uint32_t n = 0;  // blocks so far
-        int pos = begin;
         for (int i = 0; ok && more; ++i) {
-            Item& slot = slots[i % kItems];
-            Item it;
-            if (side == 0) {
-                it.s = w.s;
-                it.seq = w.b;
-                it.h = w.h;
-                it.base = first_block(a, w.s);
-                it.k0 = w.k;
-                it.k1 = min(w.blocks, w.k + (end - pos));
-                it.blocks = w.blocks;
-                it.begin = pos - w.k;
-                pos += it.k1 - it.k0;
-                it.more = pos < end;
-                ok = wait(&item_empty[i % kItems], (i / kItems) ^ 1);
-                if (!ok) break;
-                const int R = it.s.n * G;
-                if (lane == 0) {
-                    slot = it;
-                    if (a.q_vec) mbar_arrive_expect_tx(&item_full[i % kItems], (uint32_t)(R * a.D * 2));
-                }
-                __syncwarp();
-                if (!a.q_vec) {  // no 16-byte boundaries
-                    for (int e = lane; e < R * a.D; e += 32) {
-                        const int r = e / a.D, d = e % a.D;
-                        reinterpret_cast<uint16_t*>(q_smem + ((i % kItems) * kRowsMax + r) * QP)[d] =
-                            reinterpret_cast<const uint16_t*>(a.q)[(int64_t)(it.s.q0 + r / G) * a.ldq + (int64_t)(it.h * G + r % G) * a.D + d];
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&item_full[i % kItems]);
-                } else if (lane < R)  // the item's queries, a row to a lane
-                    bulk_g2s(q_smem + ((i % kItems) * kRowsMax + lane) * QP,
-                             reinterpret_cast<const uint16_t*>(a.q) + (int64_t)(it.s.q0 + lane / G) * a.ldq + (int64_t)(it.h * G + lane % G) * a.D,
-                             (uint32_t)a.D * 2, &item_full[i % kItems]);
-                w.k = 0;
-                if (++w.h == a.hkv && it.more) enter(w, w.b + 1);
-            } else {
-                ok = wait(&item_full[i % kItems], i / kItems);
-                if (!ok) break;
-                it = slot;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
-            }
+            ok = wait(&item_full[i % kItems], i / kItems);
+            if (!ok) break;
+            const Item it = slots[i % kItems];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[i % kItems]);
             more = it.more;
-            int j = (it.base + it.k0) * kBlock + first, page = page_of(it, j);
+            // the page of this lane's chunk of a block, asked for one block ahead; chunks past the end are
+            // read from outside the map, which gives zeros
+            const int* pages = a.batch.page_table + (int64_t)it.seq * a.batch.max_pages;
+            auto page_of = [&](int j) {
+                return loads && j < it.s.kv ? __ldg(pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size)) : -2;
+            };
+            int j = (it.base + it.k0) * kBlock + first, page = page_of(j);
             for (int k = it.k0; k < it.k1; ++k, ++n) {
                 const uint32_t st = n % S;
                 ok = wait(&empty_bar[st], (n / S) ^ 1);
@@ -341,7 +339,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);
                 }
                 j += kBlock;
-                if (k + 1 < it.k1) page = page_of(it, j);
+                if (k + 1 < it.k1) page = page_of(j);
                 __syncwarp();
             }
         }

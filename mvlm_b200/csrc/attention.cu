@@ -20,7 +20,8 @@ using namespace mgpu_dev;
 
 namespace {
 
-constexpr int kBlock = 64;  // keys of a block: one row of the TMA boxes' 64-row destination
+constexpr float kGrowth = 8.0f;  // log2 of how far a weight may exceed 1 before its row's reference moves
+constexpr int kBoxRows = 64;  // most rows of a box of the cache's TMA maps
 
 // ------------------------------------------------------------------ masks -----------
 // First and one-past-last key that the row of token i (of n, at the end of kv) sees.
@@ -116,7 +117,10 @@ constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 3);  // then: ke
 constexpr int kRowsMax = 16;
 constexpr int kSeqCap = 1024;  // sequences whose block counts are kept in shared memory
 
-template <int DP> constexpr int rows_stage_bytes() { return 2 * kBlock * DP * 2; }
+// Keys of a block, and of one warp: blocks of 32 KB whatever the head's dims, so that what a block
+// costs beside its products (waits, maxima) falls on as many bytes.
+template <int DP> constexpr int rows_keys() { return DP == 64 ? 128 : 64; }
+template <int DP> constexpr int rows_stage_bytes() { return 2 * rows_keys<DP>() * DP * 2; }
 // 128 KB in flight, some three times what HBM's latency at full rate asks of an SM.  An even number,
 // so that a stage always belongs to one group of warps: a wait on the parity of a barrier's phase
 // must not be able to meet the phase before the last one, which a group two blocks ahead of the
@@ -136,14 +140,14 @@ struct Item {
     int seq, h, base, k0, k1, blocks, begin, more;  // base: the item's first block; begin: its place among all blocks
 };
 
-__device__ __forceinline__ int first_block(const mgpu_k::AttendArgs& a, const SeqView& s) {
-    return seen_by(a, s, 0).lo / kBlock;
+template <int KEYS> __device__ __forceinline__ int first_block(const mgpu_k::AttendArgs& a, const SeqView& s) {
+    return seen_by(a, s, 0).lo / KEYS;
 }
 // Blocks of one item of sequence b; a sequence that sees no key has one, in which nothing is seen,
 // so that its rows are written.
-__device__ __forceinline__ int item_blocks(const mgpu_k::AttendArgs& a, const SeqView& s, int max_rows) {
+template <int KEYS> __device__ __forceinline__ int item_blocks(const mgpu_k::AttendArgs& a, const SeqView& s, int max_rows) {
     if (s.n <= 0 || (long long)s.n * (a.hq / a.hkv) > max_rows) return 0;
-    return max(1, (s.kv + kBlock - 1) / kBlock - first_block(a, s));
+    return max(1, (s.kv + KEYS - 1) / KEYS - first_block<KEYS>(a, s));
 }
 
 // The blocks [k0, k1) of key head h of sequence b.
@@ -158,7 +162,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     attend_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const mgpu_k::AttendArgs a) {
     constexpr int S = rows_stages<DP>(), SB = rows_stage_bytes<DP>(), PITCH = rows_pitch<DP>();
-    constexpr int SLABS = DP / 64, SLAB = kBlock * 128;  // 64 dims x 64 keys, 128-byte rows, swizzled
+    constexpr int KEYS = rows_keys<DP>(), KW = KEYS / 4;   // of a block, of a warp
+    constexpr int SLABS = DP / 64, SLAB = KEYS * 128;      // 64 dims of a block's keys, 128-byte rows, swizzled
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
     static_assert(S % 2 == 0, "a stage belongs to one group of warps");
     constexpr int QP = rows_q_pitch<DP>();
@@ -201,7 +206,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         bool bad = false;
         const SeqView s = seq_view(a.batch, b, a.page_size, &bad);
         if (bad) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
-        return item_blocks(a, s, a.max_rows);
+        return item_blocks<KEYS>(a, s, a.max_rows);
     };
     long long sum = 0;
     for (int b = tid; b < a.batch.n_seqs; b += kRowsThreads) {
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             if (n == 0) continue;
             bool bad = false;
             w.s = seq_view(a.batch, b, a.page_size, &bad);
-            w.blocks = n > 0 ? n : item_blocks(a, w.s, a.max_rows);
+            w.blocks = n > 0 ? n : item_blocks<KEYS>(a, w.s, a.max_rows);
             if (w.blocks > 0) break;
         }
         w.b = b;
@@ -274,7 +279,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 it.s = w.s;
                 it.seq = w.b;
                 it.h = w.h;
-                it.base = first_block(a, w.s);
+                it.base = first_block<KEYS>(a, w.s);
                 it.k0 = w.k;
                 it.k1 = k1;
                 it.blocks = w.blocks;
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     if (warp >= kRowsWarps) {
         // ---------------------------------------------------------------- loads
         // one warp for the keys, one for the values; a lane loads one chunk (rows of one page) of a slab
-        const int rows = a.box_rows, chunks = kBlock / rows, side = warp - kRowsWarps;
+        const int rows = a.box_rows, chunks = KEYS / rows, side = warp - kRowsWarps;
         const bool loads = lane < chunks * SLABS;
         const int first = (lane % chunks) * rows, slab = lane / chunks;
         const CUtensorMap* map = side ? &tmV : &tmK;
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             auto page_of = [&](int j) {
                 return loads && j < it.s.kv ? __ldg(pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size)) : -2;
             };
-            int j = (it.base + it.k0) * kBlock + first, page = page_of(j);
+            int j = (it.base + it.k0) * KEYS + first, page = page_of(j);
             for (int k = it.k0; k < it.k1; ++k, ++n) {
                 const uint32_t st = n % S;
                 ok = wait(&empty_bar[st], (n / S) ^ 1);
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     const int y = in ? (a.page_shift >= 0 ? j & ((1 << a.page_shift) - 1) : j % a.page_size) : 0;
                     tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);
                 }
-                j += kBlock;
+                j += KEYS;
                 if (k + 1 < it.k1) page = page_of(j);
                 __syncwarp();
             }
@@ -350,7 +355,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     }
 
     // -------------------------------------------------------------------- scores and sums
-    const int group = warp >> 2, part = warp & 3;  // blocks of one parity; 16 keys of each
+    const int group = warp >> 2, part = warp & 3;  // blocks of one parity; KW keys of each
     const int g = lane >> 2, c2 = 2 * (lane & 3);  // this thread's rows g and g + 8, and first column
     // Two items' states of up to 8 rows fit the scratch, and the barrier of the item between says that the
     // last ones have been read.  Where an item may have more rows, each takes both places, and a barrier more.
@@ -401,73 +406,95 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     continue;
                 }
                 const uint32_t kb = smem_u32(ring + st * SB), vb = kb + SB / 2;
-                const int j0 = (base + k) * kBlock + 16 * part;  // this warp's first key
-                // S = Q K^T: 16 rows x 16 keys
-                float sc[2][4] = {};
+                const int j0 = (base + k) * KEYS + KW * part;  // this warp's first key
+                // S = Q K^T: 16 rows x KW keys
+                float sc[KW / 8][4];
 #pragma unroll
-                for (int d = 0; d < DP / 16; ++d) {
-                    // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step
-                    const int row = 16 * part + (lane & 7) + ((lane >> 4) << 3), ch = (2 * d + ((lane >> 3) & 1)) & 7;
-                    uint32_t b[4];
-                    ldsm4(b, kb + (d / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
-                    mma16816<T>(sc[0], qf[d], b[0], b[1]);
-                    mma16816<T>(sc[1], qf[d], b[2], b[3]);
-                }
-                const bool whole = j0 >= s1.lo && j0 + 16 <= s0.hi;
+                for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                    for (int e = 0; e < 4; ++e) sc[n][e] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        sc[n][e] *= a.scale_log2;
-                        const int j = j0 + 8 * n + c2 + (e & 1);
-                        if (!whole && (j < sr[e >> 1].lo || j >= sr[e >> 1].hi)) sc[n][e] = -INFINITY;
+                for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                    for (int u = 0; u < KW / 16; ++u) {
+                        // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step
+                        const int row = KW * part + 16 * u + (lane & 7) + ((lane >> 4) << 3), ch = (2 * d + ((lane >> 3) & 1)) & 7;
+                        uint32_t b[4];
+                        ldsm4(b, kb + (d / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
+                        mma16816<T>(sc[2 * u], qf[d], b[0], b[1]);
+                        mma16816<T>(sc[2 * u + 1], qf[d], b[2], b[3]);
                     }
-                // running maximum and sum
-                uint32_t pf[4];
+                const bool whole = j0 >= s1.lo && j0 + KW <= s0.hi;
+                if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+                    for (int n = 0; n < KW / 8; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = j0 + 8 * n + c2 + (e & 1);
+                            if (j < sr[e >> 1].lo || j >= sr[e >> 1].hi) sc[n][e] = -INFINITY;
+                        }
+                }
+                // The reference m, which the maximum may exceed by kGrowth before it moves (weights then stay
+                // below 2^kGrowth, and O mostly as it is), and the sum.
+                uint32_t pf[KW / 16][4];
+                float top[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    float top = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float mn = fmaxf(m[i], top), mu = mn == -INFINITY ? 0.0f : mn;
-                    const float r = ex2(m[i] - mu);
-                    m[i] = mn;
-                    float p[4];
+                    top[i] = fmaxf(sc[0][2 * i], sc[0][2 * i + 1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] = ex2(sc[e >> 1][2 * i + (e & 1)] - mu);
-                    l[i] = l[i] * r + ((p[0] + p[1]) + (p[2] + p[3]));
-                    pf[i] = pack2<T>(p[0], p[1]);
-                    pf[2 + i] = pack2<T>(p[2], p[3]);
-                    if (__any_sync(0xffffffffu, r != 1.0f)) {
+                    for (int n = 1; n < KW / 8; ++n) top[i] = fmaxf(top[i], fmaxf(sc[n][2 * i], sc[n][2 * i + 1]));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                    top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2)) * a.scale_log2;
+                }
+                if (__any_sync(0xffffffffu, top[0] > m[0] + kGrowth || top[1] > m[1] + kGrowth)) {
+                    float r[2];
 #pragma unroll
-                        for (int n = 0; n < DP / 8; ++n) {
-                            o[n][2 * i] *= r;
-                            o[n][2 * i + 1] *= r;
-                        }
+                    for (int i = 0; i < 2; ++i) {
+                        const float mn = fmaxf(m[i], top[i]);
+                        r[i] = mn == -INFINITY ? 1.0f : ex2(m[i] - mn);
+                        m[i] = mn;
+                        l[i] *= r[i];
+                    }
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][e] *= r[e >> 1];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float neg = m[i] == -INFINITY ? 0.0f : -m[i];
+#pragma unroll
+                    for (int u = 0; u < KW / 16; ++u) {
+                        float p[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(sc[2 * u + (e >> 1)][2 * i + (e & 1)], a.scale_log2, neg));
+                        l[i] += (p[0] + p[1]) + (p[2] + p[3]);
+                        pf[u][i] = pack2<T>(p[0], p[1]);
+                        pf[u][2 + i] = pack2<T>(p[2], p[3]);
                     }
                 }
                 if (__builtin_expect(!whole, 0)) {
                     // Values that some row does not see: a weight of 0 times NaN or Inf is not 0, so those
                     // are taken out of the block and added to the rows that see them.
-                    const int row = 16 * part + (lane >> 1);
+                    uint8_t* vs = ring + st * SB + SB / 2;
                     bool found = false;
+#pragma unroll 4
+                    for (int x = lane; x < KW * DP / 8; x += 32) {
+                        const int row = KW * part + x / (DP / 8), ch = x % (DP / 8);
+                        const uint4 v = *reinterpret_cast<const uint4*>(vs + (ch >> 3) * SLAB + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+                        const uint32_t y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int i = 0; i < DP / 16; ++i) {
-                        const int ch = (lane & 1) * (DP / 16) + i;
-                        const uint4 v = *reinterpret_cast<const uint4*>(ring + st * SB + SB / 2 + (ch >> 3) * SLAB + row * 128 +
-                                                                        (((ch & 7) ^ (row & 7)) << 4));
-                        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) found |= odd16(x[e], kBf16) || odd16(x[e] >> 16, kBf16);
+                        for (int e = 0; e < 4; ++e) found |= odd16(y[e], kBf16) || odd16(y[e] >> 16, kBf16);
                     }
                     if (__builtin_expect(__any_sync(0xffffffffu, found), 0)) {
-                        for (int j = 0; j < 16; ++j) {
-                            const int r = 16 * part + j;
+#pragma unroll 1
+                        for (int j = 0; j < KW; ++j) {
+                            const int r = KW * part + j;
                             const bool s_lo = j0 + j >= sr[0].lo && j0 + j < sr[0].hi, s_hi = j0 + j >= sr[1].lo && j0 + j < sr[1].hi;
 #pragma unroll
                             for (int n = 0; n < DP / 8; ++n) {
-                                const uint32_t v = *reinterpret_cast<const uint32_t*>(ring + st * SB + SB / 2 + (n >> 3) * SLAB +
-                                                                                     r * 128 + (((n & 7) ^ (r & 7)) << 4) + 2 * c2);
+                                const uint32_t v = *reinterpret_cast<const uint32_t*>(vs + (n >> 3) * SLAB + r * 128 +
+                                                                                     (((n & 7) ^ (r & 7)) << 4) + 2 * c2);
                                 const float2 f = unpack2<T>(v);
                                 const float x = odd16(v, kBf16) ? f.x : 0.0f, y = odd16(v >> 16, kBf16) ? f.y : 0.0f;
                                 if (s_lo) { o[n][0] += x; o[n][1] += y; }
@@ -475,12 +502,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                             }
                         }
                         __syncwarp();
-                        for (int i = 0; i < DP / 16; ++i) {
-                            const int ch = (lane & 1) * (DP / 16) + i;
-                            uint16_t* v = reinterpret_cast<uint16_t*>(ring + st * SB + SB / 2 + (ch >> 3) * SLAB + row * 128 +
-                                                                      (((ch & 7) ^ (row & 7)) << 4));
-                            for (int e = 0; e < 8; ++e)
-                                if (odd16(v[e], kBf16)) v[e] = 0;
+#pragma unroll 1
+                        for (int x = lane; x < KW * DP; x += 32) {
+                            const int row = KW * part + x / DP, d = x % DP;
+                            uint16_t* v = reinterpret_cast<uint16_t*>(vs + (d >> 6) * SLAB + row * 128 + ((((d >> 3) & 7) ^ (row & 7)) << 4)) + (d & 7);
+                            if (odd16(*v, kBf16)) *v = 0;
                         }
                         fence_proxy_async_smem();  // before the ring's next load of this stage
                         __syncwarp();
@@ -488,14 +514,16 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 }
                 // O += P V
 #pragma unroll
-                for (int n = 0; n < DP / 16; ++n) {
-                    // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step, transposed
-                    const int row = 16 * part + (lane & 7) + (((lane >> 3) & 1) << 3), ch = (2 * n + (lane >> 4)) & 7;
-                    uint32_t b[4];
-                    ldsm4_t(b, vb + (n / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
-                    mma16816<T>(o[2 * n], pf, b[0], b[1]);
-                    mma16816<T>(o[2 * n + 1], pf, b[2], b[3]);
-                }
+                for (int u = 0; u < KW / 16; ++u)
+#pragma unroll
+                    for (int n = 0; n < DP / 16; ++n) {
+                        // matrices: keys 0-7 / 8-15 x dims 0-7 / 8-15 of this step, transposed
+                        const int row = KW * part + 16 * u + (lane & 7) + (((lane >> 3) & 1) << 3), ch = (2 * n + (lane >> 4)) & 7;
+                        uint32_t b[4];
+                        ldsm4_t(b, vb + (n / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
+                        mma16816<T>(o[2 * n], pf[u], b[0], b[1]);
+                        mma16816<T>(o[2 * n + 1], pf[u], b[2], b[3]);
+                    }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty_bar[st]);
             }
@@ -690,7 +718,6 @@ constexpr int kTileSeqs = 1024;    // sequences of one launch
 constexpr int kTileEntries = 2048; // entries of the table of items
 constexpr int kJoinBlocks = 6;     // what a join costs, in blocks
 constexpr int kPoly = 4;
-constexpr float kGrowth = 8.0f;    // log2 of how far a weight may exceed 1
 
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
 // K on even and V on odd stages: two blocks of 128 dims, four of 64
@@ -1509,7 +1536,7 @@ size_t attend_scratch_bytes(int sm_count, bool many_rows) {
 bool attend_many_rows(const AttendArgs& a) { return a.batch.max_q_len * (int64_t)(a.hq / a.hkv) > kRowsMax; }
 
 bool make_cache_map(CUtensorMap* m, const void* side, int type, int num_pages, int page_size, int kv_heads, int head_dim) {
-    int rows = kBlock;
+    int rows = kBoxRows;
     while (page_size % rows) rows /= 2;
     const int64_t dims[3] = {head_dim, page_size, (int64_t)num_pages * kv_heads};
     const int64_t strides[2] = {(int64_t)head_dim * 2, (int64_t)page_size * head_dim * 2};
@@ -1519,7 +1546,7 @@ bool make_cache_map(CUtensorMap* m, const void* side, int type, int num_pages, i
 
 cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const AttendArgs& in) {
     AttendArgs a = in;
-    a.box_rows = kBlock;
+    a.box_rows = kBoxRows;
     while (a.page_size % a.box_rows) a.box_rows /= 2;
     // one sequence of a chunk: the kernel for many rows alone, however few it turns out to have
     a.max_rows = a.batch.n_seqs == 1 && attend_many_rows(a) ? 0 : kRowsMax;
@@ -1529,7 +1556,6 @@ cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUt
     a.q_vec = ((uintptr_t)a.q & 15) == 0 && a.ldq % 8 == 0;
     a.out_vec = ((uintptr_t)a.out & 15) == 0 && a.ldo % 8 == 0;
     a.out_wide = ((uintptr_t)a.out & 31) == 0 && a.ldo % 16 == 0 && a.D % 16 == 0;
-    a.q_pairs = ((uintptr_t)a.q & 3) == 0 && a.ldq % 2 == 0;
     a.out_pairs = ((uintptr_t)a.out & 3) == 0 && a.ldo % 2 == 0;
     return a.type == MGPU_F16 ? launch_attend<__half>(c, mk, mv, a) : launch_attend<__nv_bfloat16>(c, mk, mv, a);
 }

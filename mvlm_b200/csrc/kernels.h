@@ -136,14 +136,14 @@ struct AttendArgs {
     float* partials;        // attend_scratch_bytes
     unsigned int* tickets;  // eight per CTA, zero between calls (the kernels leave them so)
     // set by paged_attention
-    int box_rows, page_shift, max_rows, q_pairs, out_pairs, q_vec, q_tma, out_vec, out_wide;
+    int box_rows, page_shift, max_rows, out_pairs, q_vec, q_tma, out_vec, out_wide;
 };
 // Whether some sequence may have more rows (new tokens x query heads of a key head) than the
 // kernel for few rows takes, and the scratch that needs.
 bool attend_many_rows(const AttendArgs& a);
 size_t attend_scratch_bytes(int sm_count, bool many_rows);
 // The TMA map of one side of a cache: [num_pages * kv_heads][page_size][head_dim], boxes of 64
-// dims x the most rows that divide both a page and a block of keys.
+// dims x the most rows, at most 64, that divide a page.
 bool make_cache_map(CUtensorMap* m, const void* side, int type, int num_pages, int page_size, int kv_heads, int head_dim);
 cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const AttendArgs& a);
 

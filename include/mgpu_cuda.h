@@ -17,7 +17,8 @@
  *     reading their weight operand (W / B) before that kernel has finished, and read
  *     activations and write outputs only after it.  A weight buffer must therefore not be
  *     written by the GEMV or GEMM call enqueued directly before the call that reads it as
- *     weights (uploads, copies, conversions and any other enqueued work may precede it).
+ *     weights (uploads, copies, conversions and any other enqueued work may precede it).  The
+ *     same holds for what mgpu_kv_append, mgpu_paged_attention and mgpu_logits_process write.
  */
 #ifndef MGPU_CUDA_H
 #define MGPU_CUDA_H

@@ -49,32 +49,6 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// 2^z for two values on the FMA pipe: z = n + f with n the nearest integer, a polynomial in f on
-// [-1/2, 1/2] (least largest relative error; 2^-13.7 of degree 3, 2^-18.5 of degree 4, each below
-// the rounding of the weight that follows, 2^-9 of bf16 and 2^-12 of fp16), n added to the exponent.
-// Below 2^-126 it is 0, as ex2 has it.
-template <typename T> __device__ __forceinline__ float2 ex2_poly(float2 z) {
-    constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: the sum's last bits are n
-    const float2 zc = make_float2(fmaxf(z.x, -126.0f), fmaxf(z.y, -126.0f));
-    const float2 t = __fadd2_rn(zc, make_float2(kRound, kRound));
-    const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
-    const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), zc);
-    float2 p;
-    if constexpr (std::is_same<T, __half>::value) {
-        p = __ffma2_rn(make_float2(9.5700979e-3f, 9.5700979e-3f), f, make_float2(5.5917859e-2f, 5.5917859e-2f));
-        p = __ffma2_rn(p, f, make_float2(2.4024744e-1f, 2.4024744e-1f));
-        p = __ffma2_rn(p, f, make_float2(6.9312179e-1f, 6.9312179e-1f));
-        p = __ffma2_rn(p, f, make_float2(9.9999928e-1f, 9.9999928e-1f));
-    } else {
-        p = __ffma2_rn(make_float2(5.5171665e-2f, 5.5171665e-2f), f, make_float2(2.4261113e-1f, 2.4261113e-1f));
-        p = __ffma2_rn(p, f, make_float2(6.9326097e-1f, 6.9326097e-1f));
-        p = __ffma2_rn(p, f, make_float2(9.9992806e-1f, 9.9992806e-1f));
-    }
-    const float x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
-    const float y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
-    return make_float2(z.x < -126.0f ? 0.0f : x, z.y < -126.0f ? 0.0f : y);
-}
-
 // ------------------------------------------------------------------ tensor cores ----
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -194,10 +168,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         fence_mbar_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
     // the step's contents and the cache may be the preceding kernel's
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
     // dims beyond the head's stay zero, whatever the rows become
     for (int x = tid; x < kItems * kRowsMax * QP / 16; x += kRowsThreads) reinterpret_cast<uint4*>(q_smem)[x] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
@@ -717,7 +691,6 @@ constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, pr
 constexpr int kTileSeqs = 1024;    // sequences of one launch
 constexpr int kTileEntries = 2048; // entries of the table of items
 constexpr int kJoinBlocks = 6;     // what a join costs, in blocks
-constexpr int kPoly = 4;
 
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
 // K on even and V on odd stages: two blocks of 128 dims, four of 64
@@ -872,9 +845,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
         if (a.q_tma) prefetch_tensormap(&tmQ);
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
     // ---- the table of items: pairs before each sequence, blocks before each run of pairs
     const int seqs = min(a.batch.n_seqs - seq0, kTileSeqs);
     auto view = [&](int b) {
@@ -1325,9 +1298,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float2 z = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), sc2, neg2);
-                        // the exponential unit takes 4 values a clock and quarter of an SM, two tiles' 256 a row
-                        // as long as the products take: every kPoly-th pair goes to the FMA pipe
-                        const float2 w2 = e % kPoly == kPoly - 1 ? ex2_poly<T>(z) : make_float2(ex2(z.x), ex2(z.y));
+                        const float2 w2 = make_float2(ex2(z.x), ex2(z.y));
                         sum = __fadd2_rn(sum, w2);
                         w[e] = pack2<T>(w2.x, w2.y);
                     }

@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const mgpu_k:
     const bool paired = u < pair_units;
     const int d = paired ? u * 8 : a.rot + (u - pair_units) * 8;
     const int step = (int)gridDim.y * abreast, heads = h0 < abreast ? a.hq + 2 * a.hkv : 0;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
     Raw8 x[kAhead], y[kAhead];
     auto src_type = [&](const Head& s) { return ST >= 0 ? ST : s.stype; };
     auto dst_type = [&](const Head& s) { return DT >= 0 ? DT : s.dtype; };

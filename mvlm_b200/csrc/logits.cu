@@ -98,8 +98,8 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
     __shared__ Best warp_best[kRulesThreads / 32];
     __shared__ int n_marked;
     const int tid = threadIdx.x, row = blockIdx.x / ctas, rank = blockIdx.x % ctas;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
     const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.ldx;
     T* out = a.out ? reinterpret_cast<T*>(a.out) + (int64_t)row * a.ldo : nullptr;
     const int first = (int)min((int64_t)a.n, (int64_t)rank * range), last = (int)min((int64_t)a.n, (int64_t)first + range);

@@ -5,6 +5,7 @@
 // (dispatch_rope_apply and kv_cache_append, src/models/moondream2.cpp:406-420): three passes over
 // the activations.  Here each value is read once and written once: the bound is
 // T (Hq + 2 Hkv) D (source + cache bytes) at HBM rate.
+#include <climits>
 #include <type_traits>
 
 #include "common.cuh"
@@ -134,77 +135,88 @@ __device__ __forceinline__ void store8(void* p, int type, int64_t i, const float
 // One CTA per (token, share of its heads), rows and halves of pairs on 16-byte boundaries.  A head is
 // cut into units of one thread: 8 dims and their partners rot/2 further on, or, with adjacent pairs,
 // 8 dims that hold their own partners; and 8 dims of the rest.  A thread keeps its unit over its
-// heads, so that it reads its angles once, and asks for its first kAhead heads before it looks up
-// where they go: five dependent reads (sequence, length, page, position, angle) that would otherwise
-// come before the first byte of data.
-constexpr int kAhead = 3;
+// heads, so that it reads its angles once, and asks for its first heads of q, k and v before it looks
+// up where they go: five dependent reads (sequence, length, page, position, angle) that would
+// otherwise come before the first byte of data.
 // ST, DT: the type of q, k and v, and that of q_out and the cache; -1 where they are not one.
 template <bool ADJ, int ST, int DT>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const mgpu_k::AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, ADJ ? 7 : ST == MGPU_F32 || ST < 0 ? 4 : 6) kv_append_kernel(const mgpu_k::AppendArgs a) {
     constexpr int NP = ADJ ? 4 : 8;  // pairs of a unit
+    constexpr int AHEAD = ADJ && ST != MGPU_F32 && ST >= 0 ? 4 : 2;  // heads of q on their way: 16 to 64 registers
     const int t = blockIdx.x, half = a.rot / 2;
     const int pair_units = a.rot / (ADJ ? 8 : 16), units = pair_units + (a.D - a.rot) / 8, abreast = kAppendThreads / units;
     const int u = threadIdx.x % units, h0 = threadIdx.x / units;
     const bool paired = u < pair_units;
     const int d = paired ? u * 8 : a.rot + (u - pair_units) * 8;
-    const int step = (int)gridDim.y * abreast, heads = h0 < abreast ? a.hq + 2 * a.hkv : 0;
+    const int first = h0 < abreast ? (int)blockIdx.y * abreast + h0 : INT_MAX, step = (int)gridDim.y * abreast;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
-    Raw8 x[kAhead], y[kAhead];
-    auto src_type = [&](const Head& s) { return ST >= 0 ? ST : s.stype; };
-    auto dst_type = [&](const Head& s) { return DT >= 0 ? DT : s.dtype; };
-    auto fetch = [&](int h) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i)
-            if (h + i * step < heads) {
-                const Head s = head_of(a, t, h + i * step);
-                x[i] = load_raw(s.src, src_type(s), s.in + d);
-                if (!ADJ && paired) y[i] = load_raw(s.src, src_type(s), s.in + d + half);
-            }
+    struct Unit {
+        Raw8 x, y;
     };
-    int h = (int)blockIdx.y * abreast + h0;
-    fetch(h);
+    auto load = [&](Unit& r, const void* src, int type, int64_t at) {
+        const int st = ST >= 0 ? ST : type;
+        r.x = load_raw(src, st, at);
+        if (!ADJ && paired) r.y = load_raw(src, st, at + half);
+    };
+    Unit q[AHEAD], k, v;
+    const int64_t row_q = (int64_t)t * a.ldq + d, row_k = (int64_t)t * a.ldk + d, row_v = (int64_t)t * a.ldv + d;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (first < a.hq - i * step) load(q[i], a.q, a.qt, row_q + (int64_t)(first + i * step) * a.D);
+    if (first < a.hkv) {
+        load(k, a.k, a.kt, row_k + (int64_t)first * a.D);
+        load(v, a.v, a.vt, row_v + (int64_t)first * a.D);
+    }
     Place place;
     if (!place_of(a, t, place)) return;
     float2 cs[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) cs[i] = paired ? angle_of(a, place, (ADJ ? d / 2 : d) + i) : make_float2(1.0f, 0.0f);
-    for (; h < heads; h += kAhead * step) {
+    auto store = [&](const Unit& r, int src_type, void* dst, int dst_type, int64_t at, bool turns) {
+        const int st = ST >= 0 ? ST : src_type, dt = DT >= 0 ? DT : dst_type;
+        float x[8];
+        values_of(r.x, st, x);
+        if constexpr (ADJ) {
+            if (paired && turns) {
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (h + i * step >= heads) break;
-            const Head s = head_of(a, t, h + i * step);
-            const int64_t out = s.out + d + (h + i * step < a.hq ? 0 : place.slot);
-            float v[8];
-            values_of(x[i], src_type(s), v);
-            if (!paired) {
-                store8(s.dst, dst_type(s), out, v);
-            } else if constexpr (ADJ) {
-                if (s.turns) {
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) {
-                        const float b = v[2 * p];
-                        v[2 * p] = b * cs[p].x - v[2 * p + 1] * cs[p].y;
-                        v[2 * p + 1] = b * cs[p].y + v[2 * p + 1] * cs[p].x;
-                    }
+                for (int p = 0; p < NP; ++p) {
+                    const float b = x[2 * p];
+                    x[2 * p] = b * cs[p].x - x[2 * p + 1] * cs[p].y;
+                    x[2 * p + 1] = b * cs[p].y + x[2 * p + 1] * cs[p].x;
                 }
-                store8(s.dst, dst_type(s), out, v);
-            } else {
-                float w[8];
-                values_of(y[i], src_type(s), w);
-                if (s.turns) {
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) {
-                        const float b = v[p];
-                        v[p] = b * cs[p].x - w[p] * cs[p].y;
-                        w[p] = b * cs[p].y + w[p] * cs[p].x;
-                    }
-                }
-                store8(s.dst, dst_type(s), out, v);
-                store8(s.dst, dst_type(s), out + half, w);
             }
+        } else if (paired) {
+            float y[8];
+            values_of(r.y, st, y);
+            if (turns) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    const float b = x[p];
+                    x[p] = b * cs[p].x - y[p] * cs[p].y;
+                    y[p] = b * cs[p].y + y[p] * cs[p].x;
+                }
+            }
+            store8(dst, dt, at + half, y);
         }
-        fetch(h + kAhead * step);
+        store8(dst, dt, at, x);
+    };
+    const int64_t row_qo = (int64_t)t * a.ldqo + d, slot = place.slot + d, head = (int64_t)a.page_size * a.D;
+    for (int h = first; h < a.hkv; h += step) {
+        store(k, a.kt, a.kc, a.ctype, slot + h * head, true);
+        store(v, a.vt, a.vc, a.ctype, slot + h * head, false);
+        if (h + step < a.hkv) {
+            load(k, a.k, a.kt, row_k + (int64_t)(h + step) * a.D);
+            load(v, a.v, a.vt, row_v + (int64_t)(h + step) * a.D);
+        }
+    }
+    for (int h = first; h < a.hq; h += AHEAD * step) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (h < a.hq - i * step) store(q[i], a.qt, a.qo, a.qot, row_qo + (int64_t)(h + i * step) * a.D, true);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (h < a.hq - (AHEAD + i) * step) load(q[i], a.q, a.qt, row_q + (int64_t)(h + (AHEAD + i) * step) * a.D);
     }
 }
 
@@ -261,13 +273,12 @@ cudaError_t kv_append(const LaunchCtx& c, const AppendArgs& a) {
     };
     const bool vec = ok(a.q, a.qt, a.ldq) && ok(a.k, a.kt, a.ldk) && ok(a.v, a.vt, a.ldv) && ok(a.qo, a.qot, a.ldqo) &&
                      a.rot % (a.interleaved ? 8 : 16) == 0;
-    const int heads = a.hq + 2 * a.hkv;
     int passes;  // of a CTA over a token's heads
     if (vec) {
         const int units = a.rot / (a.interleaved ? 8 : 16) + (a.D - a.rot) / 8, abreast = kAppendThreads / units;
-        passes = (heads + abreast - 1) / abreast;
+        passes = ((a.hq > a.hkv ? a.hq : a.hkv) + abreast - 1) / abreast;
     } else {
-        passes = (int)(((int64_t)heads * (a.D - a.rot / 2) + kAppendThreads - 1) / kAppendThreads);
+        passes = (int)(((int64_t)(a.hq + 2 * a.hkv) * (a.D - a.rot / 2) + kAppendThreads - 1) / kAppendThreads);
     }
     // Few tokens: one pass of heads per CTA, so that a decode step's launch is one round of loads.
     // Many: a CTA keeps its token's heads, so that the look-ups are paid once.

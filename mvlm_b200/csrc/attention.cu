@@ -82,17 +82,24 @@ __device__ __forceinline__ bool named_barrier_or(int id, int threads, bool p) {
 }
 
 // ------------------------------------------------------------------ few rows --------
-// At most 16 rows to a key head (a decode step): bound by reading K and V once from HBM, 4 G
-// operations to a byte pair.  The blocks of all (sequence, key head) items are laid end to end and
-// cut into equal shares, one per CTA, whatever the sequences' lengths; an item cut by a share's end
-// is joined by the last of its CTAs to finish.  One warp feeds a ring of blocks by TMA; eight warps
-// in two groups take every other block, a warp 16 of its keys, each with its own running state.
+// At most 16 rows to a key head (a decode step): bound by reading K and V once from HBM, some G
+// operations to a byte.  The blocks of all (sequence, key head) items are laid end to end and cut into
+// equal shares, one per CTA, whatever the sequences' lengths; an item cut by a share's end is joined
+// by the last of its CTAs to finish, in the pieces' order.  A warp hands the items out ahead, with
+// their queries; one each feeds keys and values to a ring of 32 KB blocks by TMA; eight warps in two
+// groups take every other block, each a quarter of its keys, with a running state of its own, and
+// leave it in shared memory at an item's end.  Code that runs once an item is kept short: at some
+// 15 clocks an instruction (it has left the instruction caches by then) 600 of them cost as much as
+// five blocks.
+// Measured (bf16, 8 key heads of 128, 4 rows): 64 sequences of 2150 tokens on average, 559 MB, in
+// 102 us, 5.46 TB/s, 83 % of a copy's; one of 131,002 tokens, 537 MB, in 91 us, 90 %.  256 sequences of
+// 540 reach 68 %: what an item costs is then seen.
 constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 3);  // then: keys, values, items
 constexpr int kRowsMax = 16;
 constexpr int kSeqCap = 1024;  // sequences whose block counts are kept in shared memory
 
-// Keys of a block, and of one warp: blocks of 32 KB whatever the head's dims, so that what a block
-// costs beside its products (waits, maxima) falls on as many bytes.
+// Keys of a block: 32 KB whatever the head's dims, so that what a block costs beside its products
+// (waits, maxima) falls on as many bytes (64 sequences of 64 dims: 77 us with 64 keys, 60 with 128).
 template <int DP> constexpr int rows_keys() { return DP == 64 ? 128 : 64; }
 template <int DP> constexpr int rows_stage_bytes() { return 2 * rows_keys<DP>() * DP * 2; }
 // 128 KB in flight, some three times what HBM's latency at full rate asks of an SM.  An even number,
@@ -676,21 +683,31 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
 }
 
 // ------------------------------------------------------------------ many rows -------
-// More than 16 rows to a key head (a chunk of a prompt): bound by the tensor cores' two products,
-// 4 D operations to a row and key, and by one exponential to a row and key.  A CTA takes two tiles of
-// up to 128 rows (whole tokens: 128 / G of them) over the same blocks of 128 keys.  A warp to
-// each tile issues S_t = Q_t K^T and O_t += P_t V, so that one tile's products run while the other's
-// softmax does; scores, weights and O stay in TMEM, weights in the place of their scores.  Each
-// tile has four warps, a thread to a row, which needs no exchange for its maximum and sum.  O is
-// rescaled only when a row's maximum has grown by more than 2^8 since its reference was taken: weights
-// stay below 2^8, and most blocks then leave O alone.  All blocks of all items (sequence, key head,
-// pair of tiles) are cut into equal shares as above; where whole items are few and short, a CTA takes
-// one item instead, which saves the join.
+// More than 16 rows to a key head (a chunk of a prompt): bound by the two products, 4 D operations to a
+// row and key, and beside them one exponential.  A CTA takes two tiles of up to 128 rows (whole
+// tokens: 128 / G of them) over the same blocks of 128 keys.  A warp to each tile issues
+// S_t = Q_t K^T and O_t += P_t V; scores, weights and O stay in TMEM (its 512 columns are full at 128
+// dims), weights in the place of their scores.  Each tile has four softmax warps, a thread to a row,
+// which needs no exchange for its maximum and sum.  O is rescaled only when a row's maximum has grown
+// by more than 2^kGrowth since its reference was taken, and most blocks leave it alone.  All blocks
+// of all items (sequence, key head, pair of tiles) are cut into equal shares as above.
+// Measured (bf16, 32 query and 8 key heads of 128): 4096 new tokens over 4096 in 441 us, 935 TFLOP/s,
+// 56 % of a library product's rate.  A block of 128 keys takes 3300 clocks for both tiles, of which the
+// tensor cores' arithmetic is 2048, their reads of shared memory 2560 (all of Q for every 64 keys), the
+// exponentials 2048.  Scores come in halves of 64 keys: next to whole blocks 24.0 -> 20.7 us for 761
+// tokens and 137 -> 129 for a mixed batch, at 452 -> 461 for 4096 tokens over 4096.  Tried and slower: a
+// quarter of the exponentials as polynomials (+4 %), two threads to a row (453 us), the next scores in
+// registers a half ahead (517 us).
+//
+// Which kernel: at most 16 rows go to the one above (64 sequences of 2150 tokens, 4 rows: 102 us there,
+// 150 here; 16 rows: 125 and 151; sequences of 250 tokens and 16 rows are the exception, 56 and 48).
+// A call with one sequence that may have more rows launches this kernel alone (761 tokens: 20.2 us, and
+// 22.6 with the other beside it).
 constexpr int kTileKeys = 128, kTileRows = 128;
 constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, products, scheduling
 constexpr int kTileSeqs = 1024;    // sequences of one launch
 constexpr int kTileEntries = 2048; // entries of the table of items
-constexpr int kJoinBlocks = 6;     // what a join costs, in blocks
+constexpr int kJoinBlocks = 6;     // what a join costs, in blocks (some 10 us)
 
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
 // K on even and V on odd stages: two blocks of 128 dims, four of 64
@@ -914,7 +931,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     for (int w = 0; w < kTileThreads / 32; ++w) most = max(most, warp_part[w]);
     const int head_blocks = cum[entries], total = head_blocks * a.hkv, items = pairs * a.hkv;
-    // whole items, one to a CTA, unless cutting them saves more than a join costs
+    // Whole items, one to a CTA, unless cutting them saves more than a join costs (32 heads of 64 dims: 257
+    // new tokens 12.9 us whole and 20.6 cut, 761 tokens 20.3 and 22.2; 2000 tokens have too many items).
     const bool by_item = items <= (int)gridDim.x && most <= (total + (int)gridDim.x - 1) / (int)gridDim.x + kJoinBlocks;
     const int shares = by_item ? items : min((int)gridDim.x, total);
     if ((int)blockIdx.x >= shares) return;

@@ -4,7 +4,11 @@
 // Up to eight CTAs share a row; each owns a contiguous range of the vocabulary and keeps one word per
 // token of it in shared memory (how often the history holds the token, which bias it has).  It scans
 // the row's history and biases for tokens of its range, then streams its logits once.  Bound: the
-// logits in and out at HBM rate.  Counts are integers and a bias is picked by its entry's index, so
+// logits in and out at HBM rate.  Measured: 256 rows of 51200 fp32 logits, 108 MB, with histories of
+// up to 2048 tokens, 16 biases, masks and the maximum in 37 us (44 % of a copy's rate), 17.5 us without
+// any of them: the history costs 6.6, the maximum 5.5, the biases 4 to 5, the masks 1.5, nearly all of it
+// waits one after another in a CTA (lengths, ids, words, logits), with four CTAs to an SM to fill them.
+// Counts are integers and a bias is picked by its entry's index, so
 // the order in which threads reach a word cannot change a result.
 #include <algorithm>
 #include <atomic>
@@ -299,7 +303,8 @@ cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a)
         if (e != cudaSuccess) return e;
         configured.fetch_or(bit, std::memory_order_acq_rel);
     }
-    // CTAs to a row: enough of them to fill the device, and no more than a cluster holds
+    // CTAs to a row: enough of them to fill the device, and short ranges (a range's waits come one after
+    // another).  One row of 51200: 20 us by one CTA, 13 by 2, 8.6 by 4, 8.0 by 8; 256 rows: 48, 48, 42, 37.
     int ctas = 1;
     while (ctas < 8 && ((int64_t)a.rows * ctas < 4 * c.sm_count || (a.n + ctas - 1) / ctas > kPiece)) ctas *= 2;
     const int range = ((a.n + ctas - 1) / ctas + 31) / 32 * 32;

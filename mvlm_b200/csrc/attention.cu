@@ -49,6 +49,13 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The maximum of three; a NaN loses, as in fmaxf.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
 // ------------------------------------------------------------------ tensor cores ----
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -691,13 +698,16 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
 // which needs no exchange for its maximum and sum.  O is rescaled only when a row's maximum has grown
 // by more than 2^kGrowth since its reference was taken, and most blocks leave it alone.  All blocks
 // of all items (sequence, key head, pair of tiles) are cut into equal shares as above.
-// Measured (bf16, 32 query and 8 key heads of 128): 4096 new tokens over 4096 in 441 us, 935 TFLOP/s,
-// 56 % of a library product's rate.  A block of 128 keys takes 3300 clocks for both tiles, of which the
-// tensor cores' arithmetic is 2048, their reads of shared memory 2560 (all of Q for every 64 keys), the
-// exponentials 2048.  Scores come in halves of 64 keys: next to whole blocks 24.0 -> 20.7 us for 761
-// tokens and 137 -> 129 for a mixed batch, at 452 -> 461 for 4096 tokens over 4096.  Tried and slower: a
-// quarter of the exponentials as polynomials (+4 %), two threads to a row (453 us), the next scores in
-// registers a half ahead (517 us).
+// Measured (bf16, 32 query and 8 key heads of 128): 4096 new tokens over 4096 in 392 us at 1965 MHz, 1052
+// TFLOP/s, 63 % of a library product's rate; calls in a row reach the power limit after 50 ms and settle
+// at 437 us (1.75 GHz), 68 % of what the library then holds.  A block of 128 keys takes 4150 clocks for
+// both tiles, of which the tensor cores' arithmetic is 2048, their reads of shared memory 2560 (all of Q
+// for every 64 keys), the exponentials 2048.  A softmax warp's half block: 1050 clocks of exponentials,
+// which the two warps of a scheduler mostly do at the same time, 380 of masks and maxima, 300 of waiting
+// for scores, 350 of the rest.  Scores come in halves of 64 keys: next to whole blocks 24.0 -> 20.7 us for
+// 761 tokens and 137 -> 129 for a mixed batch, at 452 -> 461 for 4096 tokens over 4096.  Tried and slower:
+// a quarter of the exponentials as polynomials (+4 %), turns at the exponentials (a lock to each scheduler:
+// +14 %), two threads to a row (453 us), the next scores in registers a half ahead (517 us).
 //
 // Which kernel: at most 16 rows go to the one above (64 sequences of 2150 tokens, 4 rows: 102 us there,
 // 150 here; 16 rows: 125 and 151; sequences of 250 tokens and 16 rows are the exception, 56 and 48).
@@ -1151,16 +1161,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 for (int kb = kb0 - 1; kb < kb1; ++kb) {
                     const uint32_t ks = (2 * n) % S, vs = (2 * n + S - 1) % S;  // keys of kb + 1, values of kb
                     const bool scores = kb + 1 < kb1, score = scores && kb + 1 >= lo && kb + 1 < hi, weigh = kb >= lo && kb < hi;
-                    if (scores) ok = wait(&full_bar[ks], 2 * n / S);
-                    if (kb >= kb0) {
-                        ok = ok && wait(&full_bar[vs], (2 * n - 1) / S);
-                        ok = ok && wait(&clean_bar[vs], (2 * n - 1) / S);
-                    }
-                    if (score && kb + 1 == lo) ok = ok && wait(&q_bar[t], q_phase++);
+                    // Keys, values (looked over, and so there), weights of half 0 and queries: a lane waits for
+                    // each.  Beside the products' reads of shared memory a wait takes some 250 clocks even when
+                    // its phase is over (a mixed batch: 119.9 us one after another, 118.1 so).
+                    const bool first = score && kb + 1 == lo;
+                    const bool mine = lane == 0 ? scores : lane == 1 ? kb >= kb0 : lane == 2 ? weigh : lane == 3 && first;
+                    uint64_t* const bar = lane == 0 ? &full_bar[ks] : lane == 1 ? &clean_bar[vs] : lane == 2 ? &p_bar[t][0] : &q_bar[t];
+                    const uint32_t phase = lane == 0 ? 2 * n / S : lane == 1 ? (2 * n - 1) / S : lane == 2 ? p_phase : q_phase;
+                    ok = __all_sync(0xffffffffu, !mine || mbar_wait(bar, phase & 1u, a.status));
+                    q_phase += first;
                     const uint64_t vd = v_desc + vs * (SB >> 4), kd = k_desc + ks * (SB >> 4);
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
-                        if (weigh) ok = ok && wait(&p_bar[t][half], p_phase);
+                        if (half && weigh) ok = wait(&p_bar[t][1], p_phase);
                         if (!ok) break;
                         tc_fence_after();
                         if (elect_one()) {
@@ -1275,11 +1288,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 float x0 = -INFINITY, x1 = -INFINITY, x2 = -INFINITY, x3 = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    x0 = fmaxf(x0, __uint_as_float(sa[e]));
-                    x1 = fmaxf(x1, __uint_as_float(sa[e + 1]));
-                    x2 = fmaxf(x2, __uint_as_float(sb[e]));
-                    x3 = fmaxf(x3, __uint_as_float(sb[e + 1]));
+                for (int e = 0; e < 32; e += 4) {
+                    x0 = max3(x0, __uint_as_float(sa[e]), __uint_as_float(sa[e + 1]));
+                    x1 = max3(x1, __uint_as_float(sa[e + 2]), __uint_as_float(sa[e + 3]));
+                    x2 = max3(x2, __uint_as_float(sb[e]), __uint_as_float(sb[e + 1]));
+                    x3 = max3(x3, __uint_as_float(sb[e + 2]), __uint_as_float(sb[e + 3]));
                 }
                 const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2;
                 const bool grown = top > m + kGrowth;

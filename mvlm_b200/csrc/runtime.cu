@@ -31,6 +31,7 @@ struct mgpu_device {
     int event_mode;
     void* workspace;
     size_t workspace_bytes;
+    std::vector<void*> old_workspaces;
     bool capturing;
     int saved_event_mode;
     std::vector<mgpu_event*> event_pool;
@@ -127,7 +128,9 @@ mgpu_k::LaunchCtx ctx_of(const mgpu_device* d) {
     return c;
 }
 
-// Grow the per-device scratch arena (zero-filled).  Synchronises the stream when it grows.
+// Grow the per-device scratch arena (zero-filled).  Synchronises the stream when it grows.  A captured
+// graph holds the address of the arena of its time (tickets and partials), whoever captured it, so earlier
+// arenas stay until the device goes; an arena at least doubles, so together they are smaller than the last.
 bool ensure_workspace(mgpu_device* d, size_t bytes) {
     if (bytes <= d->workspace_bytes) return true;
     if (d->capturing) {
@@ -148,7 +151,7 @@ bool ensure_workspace(mgpu_device* d, size_t bytes) {
         cudaFree(fresh);
         return false;
     }
-    if (d->workspace) cudaFree(d->workspace);
+    if (d->workspace) d->old_workspaces.push_back(d->workspace);
     d->workspace = fresh;
     d->workspace_bytes = want;
     return true;
@@ -188,8 +191,12 @@ bool check_status(mgpu_device* d) {
     if (st != 0) {
         cudaMemsetAsync(d->d_status, 0, sizeof(int), d->stream);
         // CTAs that gave up have not counted themselves
-        if (st == MGPU_ERR_DEVICE_TIMEOUT && d->workspace_bytes >= kScratchOffset)
-            cudaMemsetAsync((char*)d->workspace + kAttendTicketOffset, 0, kScratchOffset - kAttendTicketOffset, d->stream);
+        if (st == MGPU_ERR_DEVICE_TIMEOUT) {
+            std::vector<void*> arenas = d->old_workspaces;
+            if (d->workspace) arenas.push_back(d->workspace);
+            for (void* w : arenas)  // each holds at least the tickets
+                cudaMemsetAsync((char*)w + kAttendTicketOffset, 0, kScratchOffset - kAttendTicketOffset, d->stream);
+        }
         if (st == MGPU_ERR_INVALID_ARG)
             set_error(st, "a kernel skipped what does not fit its buffers: sequences by their lengths, pages or positions, "
                       "or bias entries of a row beyond 2047");
@@ -403,6 +410,7 @@ void mgpu_release_device(mgpu_device* d) {
         cudaEventDestroy(ev->end);
         delete ev;
     }
+    for (void* w : d->old_workspaces) cudaFree(w);
     if (d->workspace) cudaFree(d->workspace);
     cudaFree(d->d_status);
     cudaStreamDestroy(d->own_stream);

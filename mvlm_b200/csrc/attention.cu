@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     auto count = [&](int b) {
         bool bad = false;
         const SeqView s = seq_view(a.batch, b, a.page_size, &bad);
-        if (bad) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+        if (bad) report_contents(a.status);
         return item_blocks<KEYS>(a, s, a.max_rows);
     };
     long long sum = 0;
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 __syncwarp();
                 if (loads) {
                     const bool in = page >= 0 && page < a.num_pages;
-                    if (!in && page != -2) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                    if (!in && page != -2) report_contents(a.status);
                     const int z = in ? page * a.hkv + it.h : a.num_pages * a.hkv;
                     const int y = in ? (a.page_shift >= 0 ? j & ((1 << a.page_shift) - 1) : j % a.page_size) : 0;
                     tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);
@@ -880,7 +880,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     auto view = [&](int b) {
         bool bad = false;
         SeqView s = seq_view(a.batch, seq0 + b, a.page_size, &bad);
-        if (bad) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+        if (bad) report_contents(a.status);
         if ((long long)s.n * G <= a.max_rows) s.n = 0;  // the rows kernel's
         return s;
     };
@@ -1096,7 +1096,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             z = page * a.hkv + g.h;
                             y = j - at * a.page_size;
                         } else {
-                            atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                            report_contents(a.status);
                         }
                     }
 #pragma unroll

@@ -54,7 +54,7 @@ __device__ __forceinline__ bool place_of(const mgpu_k::AppendArgs& a, int t, Pla
         }
     }
     if (bad) {
-        if (threadIdx.x == 0) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+        if (threadIdx.x == 0) report_contents(a.status);
         return false;
     }
     p.slot = ((int64_t)page * a.hkv * a.page_size + index % a.page_size) * a.D;

@@ -86,6 +86,7 @@ cudaError_t fill_normal(const LaunchCtx& c, int otype, void* out, int64_t n, uin
 cudaError_t convert(const LaunchCtx& c, int itype, const void* in, int otype, void* out, int64_t n);
 // One CTA waits on an mbarrier that never completes, bounded by limit_ns.
 cudaError_t selftest_bounded_wait(const LaunchCtx& c, uint64_t limit_ns);
+cudaError_t clear_status(const LaunchCtx& c, int seen);  // 0 into the status word if it holds `seen`
 // out[0] = argmax index, out[1] = the value (fp32 bits), reference argmax semantics; n >= 1.
 cudaError_t argmax(const LaunchCtx& c, int type, const void* logits, int n, int* out);
 // The same for `rows` rows of n values, row r at element r * ld: pair r at out[2r], out[2r+1].

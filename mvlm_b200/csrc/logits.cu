@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
             b0 = min(max(a.bias_offsets[row], 0), a.bias_entries);
             b1 = min(a.bias_offsets[row + 1], a.bias_entries);
             if (b1 - b0 > kBiases) {
-                if (tid == 0) atomicExch(a.status, (int)MGPU_ERR_INVALID_ARG);
+                if (tid == 0) report_contents(a.status);
                 b1 = b0 + kBiases;
             }
             if (b0 + tid < b1) bias_t = __ldg(a.bias_tokens + b0 + tid);

@@ -146,6 +146,9 @@ __global__ void selftest_wait_kernel(int* status, uint64_t limit_ns) {
     if (threadIdx.x == 0) mbar_wait(&bar, 0, status, limit_ns);
 }
 
+// What has been read leaves the status word; what a kernel has recorded over it since stays.
+__global__ void clear_status_kernel(int* status, int seen) { atomicCAS(status, seen, 0); }
+
 // A logit as the reference's argmax compares it (moondream2.cpp:567-582, written there for
 // fp16): exponent field zero (zero or subnormal) -> 0, all ones (Inf or NaN) -> +-1e30 by the
 // sign bit, else the value.  bf16 and fp32 logits follow the same rule on their own fields.
@@ -366,6 +369,11 @@ cudaError_t rms_norm(const LaunchCtx& c, int type, const void* in, void* out, in
 
 cudaError_t argmax_combine(const LaunchCtx& c, const int* pairs, int n_ranks, int n_total, int* out) {
     argmax_combine_kernel<<<1, 32, 0, c.stream>>>(pairs, n_ranks, n_total, out);
+    return cudaGetLastError();
+}
+
+cudaError_t clear_status(const LaunchCtx& c, int seen) {
+    clear_status_kernel<<<1, 1, 0, c.stream>>>(c.status, seen);
     return cudaGetLastError();
 }
 

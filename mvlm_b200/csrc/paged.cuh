@@ -5,6 +5,10 @@
 
 namespace mgpu_dev {
 
+// Contents that a kernel skipped.  An expired wait, already recorded or still to come, has the word: its
+// output is invalid, and its tickets are not all counted.
+__device__ __forceinline__ void report_contents(int* status) { atomicCAS(status, 0, (int)MGPU_ERR_INVALID_ARG); }
+
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));

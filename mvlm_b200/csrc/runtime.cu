@@ -189,14 +189,12 @@ bool check_status(mgpu_device* d) {
     int st = 0;
     if (!cuda_ok(cudaMemcpy(&st, d->d_status, sizeof(int), cudaMemcpyDeviceToHost), "read status")) return false;
     if (st != 0) {
-        cudaMemsetAsync(d->d_status, 0, sizeof(int), d->stream);
-        // CTAs that gave up have not counted themselves
-        if (st == MGPU_ERR_DEVICE_TIMEOUT) {
-            std::vector<void*> arenas = d->old_workspaces;
-            if (d->workspace) arenas.push_back(d->workspace);
-            for (void* w : arenas)  // each holds at least the tickets
-                cudaMemsetAsync((char*)w + kAttendTicketOffset, 0, kScratchOffset - kAttendTicketOffset, d->stream);
-        }
+        mgpu_k::clear_status(ctx_of(d), st);
+        // CTAs that gave up have not counted themselves.  Work enqueued since the wait comes before this, and
+        // no kernel is at its tickets here, so they are zero but for that.
+        std::vector<void*> arenas = d->old_workspaces;
+        if (d->workspace) arenas.push_back(d->workspace);
+        for (void* w : arenas) cudaMemsetAsync(w, 0, kScratchOffset, d->stream);
         if (st == MGPU_ERR_INVALID_ARG)
             set_error(st, "a kernel skipped what does not fit its buffers: sequences by their lengths, pages or positions, "
                       "or bias entries of a row beyond 2047");

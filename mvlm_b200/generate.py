@@ -130,6 +130,8 @@ class Session:
     """Sequences in the decoder's cache; ``step`` advances each by a chunk of its prompt or one token."""
 
     def __init__(self, decoder: Decoder, chunk: int = 128, penalties=(1.1, 0.1, 0.0), allowed: np.ndarray | None = None):
+        if chunk < 1:
+            raise mg.MgpuError(mg.ERR_INVALID_ARG, f"generate: chunks of {chunk} tokens")
         self.d, self.chunk, self.penalties, self.sequences = decoder, chunk, penalties, []
         self.free = list(range(decoder.cfg.num_pages))[::-1]
         self.allowed = None if allowed is None else np.packbits(
@@ -137,9 +139,17 @@ class Session:
 
     def add(self, ids, positions=None) -> Sequence:
         """A prompt; positions [3][len(ids)] (time, height, width), by default 0, 1, 2, ... on every axis."""
+        c, ids = self.d.cfg, [int(i) for i in ids]
+        if not ids or min(ids) < 0 or max(ids) >= c.vocab:
+            raise mg.MgpuError(mg.ERR_INVALID_ARG, "generate: an empty prompt, or ids outside the vocabulary")
+        if len(self.sequences) >= c.max_tokens:
+            raise mg.MgpuError(mg.ERR_INVALID_ARG, f"generate: more sequences than a step's {c.max_tokens} rows")
         if positions is None:
             positions = np.tile(np.arange(len(ids), dtype=np.int32), (3, 1))
-        s = Sequence(list(ids), np.asarray(positions, np.int32), prompt=len(ids))
+        positions = np.asarray(positions, np.int32)
+        if positions.shape != (3, len(ids)):
+            raise mg.MgpuError(mg.ERR_INVALID_ARG, f"generate: positions {positions.shape} of {len(ids)} ids")
+        s = Sequence(ids, positions, prompt=len(ids))
         self.sequences.append(s)
         return s
 
@@ -147,53 +157,68 @@ class Session:
         self.free += s.pages
         self.sequences.remove(s)
 
-    def step(self):
-        """One step over all sequences; [(sequence, its next token, its logits' row)] for those whose
-        prompts are done, and the processed logits."""
-        c, dev = self.d.cfg, self.d.dev
+    def _plan(self):
+        """[(sequence, its tokens of this step, its pages with them)] and the pages then left."""
+        c, free, plan = self.d.cfg, list(self.free), []
         room = c.max_tokens - len(self.sequences)
-        ids, positions, starts, lens, done = [], [], [0], [], []
         for s in self.sequences:
             n = min(len(s.ids) - s.cached, self.chunk, 1 + room)
             room -= n - 1
-            need = -(-(s.cached + n) // c.page_size)
-            if need - len(s.pages) > len(self.free):
+            more = -(-(s.cached + n) // c.page_size) - len(s.pages)
+            if more > len(free):
                 raise mg.MgpuError(mg.ERR_OUT_OF_MEMORY, "generate: no free page")
-            while len(s.pages) < need:
-                s.pages.append(self.free.pop())
+            plan.append((s, n, s.pages + [free.pop() for _ in range(more)]))
+        return plan, free
+
+    def step(self):
+        """One step over all sequences; [(sequence, its next token)] for those whose prompts are done, and
+        the processed logits, a row for each of them (None where there is none).  An error leaves the
+        session as it was: the step may be taken again, for instance after a sequence was released."""
+        if not self.sequences:
+            return [], None
+        c, dev = self.d.cfg, self.d.dev
+        plan, free = self._plan()
+        ids, positions, starts, lens, done = [], [], [0], [], []
+        for s, n, _ in plan:
             ids += s.ids[s.cached:s.cached + n]
             positions.append(s.positions[:, s.cached:s.cached + n])
-            s.cached += n
             starts.append(starts[-1] + n)
-            lens.append(s.cached)
-            if s.cached == len(s.ids):
+            lens.append(s.cached + n)
+            if lens[-1] == len(s.ids):
                 done.append((s, starts[-1] - 1))
-        width = max(len(s.pages) for s in self.sequences)
-        table = np.zeros((len(self.sequences), width), np.int32)
-        for i, s in enumerate(self.sequences):
-            table[i, :len(s.pages)] = s.pages
+        width = max(len(pages) for _, _, pages in plan)
+        table = np.zeros((len(plan), width), np.int32)
+        for i, (_, _, pages) in enumerate(plan):
+            table[i, :len(pages)] = pages
         batch = mg.PagedBatch(*(dev.array(np.asarray(a, np.int32), mg.F32) for a in (starts, lens, table)), len(lens), len(ids),
-                              max(np.diff(starts)), width)
-        if not done:
-            self.d.step(ids, np.concatenate(positions, 1), batch, [len(ids) - 1])
-            return [], None
-        logits = self.d.step(ids, np.concatenate(positions, 1), batch, [r for _, r in done])
-        rows = len(done)
-        most = max(len(s.ids) for s, _ in done)
+                              int(max(np.diff(starts))), width)
+        logits = self.d.step(ids, np.concatenate(positions, 1), batch, [r for _, r in done] or [len(ids) - 1])
+        out = [(s, t) for (s, _), t in zip(done, self._tokens([s for s, _ in done], logits))]
+        # everything is in the cache, and nothing failed
+        self.free = free
+        for s, n, pages in plan:
+            s.cached += n
+            s.pages = pages
+        for s, t in out:
+            s.append(t)
+        return out, logits if done else None
+
+    def _tokens(self, sequences, logits):
+        """The sequences' greedy tokens, from their rows of the logits, which the rules change in place."""
+        rows, c, dev = len(sequences), self.d.cfg, self.d.dev
+        if not rows:
+            return []
+        most = max(len(s.ids) for s in sequences)
         history = np.full((rows, most), -1, np.int32)
-        for i, (s, _) in enumerate(done):
+        for i, s in enumerate(sequences):
             history[i, :len(s.ids)] = s.ids
-        ints = [dev.array(np.asarray(a, np.int32), mg.F32) for a in (history, [len(s.ids) for s, _ in done], [s.prompt for s, _ in done])]
+        ints = [dev.array(np.asarray(a, np.int32), mg.F32) for a in (history, [len(s.ids) for s in sequences], [s.prompt for s in sequences])]
         rules = mg.LogitRules(history=ints[0], history_lens=ints[1], prompt_lens=ints[2], history_ld=most,
                               penalties=dev.array(np.tile(np.asarray(self.penalties, np.float32), (rows, 1)), mg.F32),
                               allowed=None if self.allowed is None else dev.array(np.tile(self.allowed, (rows, 1)), mg.F32))
         best = dev.create_buffer(8 * rows)
         mg.logits_process(dev, logits, logits, rows, c.vocab, rules, best)
-        tokens = best.read(np.int32).reshape(rows, 2)[:, 0]
-        out = [(s, int(t)) for (s, _), t in zip(done, tokens)]
-        for s, t in out:
-            s.append(t)
-        return out, logits
+        return [int(t) for t in best.read(np.int32).reshape(rows, 2)[:, 0]]
 
 
 def image_positions(rows: int, cols: int, text: int) -> np.ndarray:

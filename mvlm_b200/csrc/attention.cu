@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             // read from outside the map, which gives zeros
             const int* pages = a.batch.page_table + (int64_t)it.seq * a.batch.max_pages;
             auto page_of = [&](int j) {
-                return loads && j < it.s.kv ? __ldg(pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size)) : -2;
+                return loads && j < it.s.kv ? __ldg(pages + (a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size)) : -1;
             };
             int j = (it.base + it.k0) * KEYS + first, page = page_of(j);
             for (int k = it.k0; k < it.k1; ++k, ++n) {
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 __syncwarp();
                 if (loads) {
                     const bool in = page >= 0 && page < a.num_pages;
-                    if (!in && page != -2) report_contents(a.status);
+                    if (!in && j < it.s.kv) report_contents(a.status);
                     const int z = in ? page * a.hkv + it.h : a.num_pages * a.hkv;
                     const int y = in ? (a.page_shift >= 0 ? j & ((1 << a.page_shift) - 1) : j % a.page_size) : 0;
                     tma_load_3d(ring + st * SB + side * (SB / 2) + slab * SLAB + first * 128, map, slab * 64, y, z, &full_bar[st]);

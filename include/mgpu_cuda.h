@@ -369,7 +369,8 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* cache, const mgpu_paged_ba
  *                the history after the prompt loses frequency * c, then presence
  *   bias         row r's entries bias_offsets[r] .. bias_offsets[r+1]-1 of bias_tokens /
  *                bias_values: x += value (of entries with one token, the last one's); at most
- *                2047 entries a row, more are skipped and reported like a batch's contents above
+ *                2047 entries a row, more are skipped and reported like a batch's contents above;
+ *                offsets are taken into the buffers, and a row whose end is before its start has none
  *   allowed      bit t % 32 of word t / 32 of row r (uint32 [rows][(n + 31) / 32]) clear: x = -inf
  * Each group may be NULL: history (with its lens and penalties), prompt_lens alone (no prompt),
  * bias_* together, allowed. */

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kRulesThreads) rules_kernel(const mgpu_k::Rule
         int bias_t = -1;
         if (a.bias_offsets) {
             b0 = min(max(a.bias_offsets[row], 0), a.bias_entries);
-            b1 = min(a.bias_offsets[row + 1], a.bias_entries);
+            b1 = max(b0, min(a.bias_offsets[row + 1], a.bias_entries));  // not below: the difference must hold
             if (b1 - b0 > kBiases) {
                 if (tid == 0) report_contents(a.status);
                 b1 = b0 + kBiases;

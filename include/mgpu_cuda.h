@@ -343,7 +343,8 @@ mgpu_event* mgpu_rope_table(const mgpu_device* dev, mgpu_buf* table, int max_pos
  * in one launch.  q [n_tokens][q_heads * head_dim], k and v [n_tokens][kv_heads * head_dim], f32 /
  * f16 / bf16 each, rows at their tag's pitch (so they may be views into one qkv projection);
  * q_out f32 / f16 / bf16, may be q itself.  q and q_out NULL: only the cache.  rope NULL: no
- * rotation.  fp32 arithmetic, one rounding.  Two tokens of a step must not share a slot. */
+ * rotation.  fp32 arithmetic, one rounding.  Two tokens of a step must not share a slot.  Neither the cache
+ * nor q_out may hold what the call reads, but for q itself. */
 mgpu_event* mgpu_kv_append(const mgpu_kv_cache* cache, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* k,
                            mgpu_buf* v, mgpu_buf* q_out, int q_heads, const mgpu_rope* rope);
 /* Attention of the step's tokens over the cache (their own keys and values appended before):
@@ -387,7 +388,8 @@ typedef struct mgpu_logit_rules {
 } mgpu_logit_rules;
 /* out = rules(logits) for `rows` rows of n logits (f32 / f16 / bf16, each buffer's rows at its
  * tag's pitch, default n); out of logits' type, may be logits itself, or NULL.  best (>= 8 bytes a
- * row, or NULL) receives each row's {int32 index, fp32 value} as mgpu_argmax_rows(out) would. */
+ * row, or NULL) receives each row's {int32 index, fp32 value} as mgpu_argmax_rows(out) would.  Neither
+ * out nor best may overlap anything else of the call. */
 mgpu_event* mgpu_logits_process(const mgpu_device* dev, mgpu_buf* logits, mgpu_buf* out, int rows, int n,
                                 const mgpu_logit_rules* rules, mgpu_buf* best);
 

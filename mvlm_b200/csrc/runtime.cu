@@ -1078,6 +1078,16 @@ Range rows_range(const mgpu_buf* b, int64_t rows, int64_t width, int64_t ld) {
     return range_of(b, ((size_t)(rows - 1) * ld + width) * elem_size(b->type));
 }
 
+// n 4-byte entries; none of a buffer that is not given.
+constexpr Range kNoRange{nullptr, nullptr};
+Range words_range(const mgpu_buf* b, int64_t n) { return b ? range_of(b, (size_t)n * 4) : kNoRange; }
+
+// Whether something that is written lies in what describes the step, which other CTAs may still read.
+bool in_batch(const Range& w, const mgpu_paged_batch* b) {
+    return w.overlaps(words_range(b->cu_q, (int64_t)b->n_seqs + 1)) || w.overlaps(words_range(b->kv_lens, b->n_seqs)) ||
+           w.overlaps(words_range(b->page_table, (int64_t)b->n_seqs * b->max_pages));
+}
+
 }  // namespace
 
 mgpu_kv_cache* mgpu_kv_cache_create(const mgpu_device* cd, int num_pages, int page_size, int kv_heads, int head_dim,
@@ -1168,10 +1178,18 @@ mgpu_event* mgpu_kv_append(const mgpu_kv_cache* c, const mgpu_paged_batch* batch
         if (!rows_ok(q, rows, qw, "kv_append", "q", &a.ldq) || !rows_ok(q_out, rows, qw, "kv_append", "q_out", &a.ldqo))
             return nullptr;
         const Range out = rows_range(q_out, rows, qw, a.ldqo);
-        // interleaved rows (views into one projection) share a range without sharing a value: only
-        // q_out's own rows are checked against them, as whole views
+        // interleaved rows (views into one projection) share a range without sharing a value, if their
+        // columns of the common pitch are apart
+        auto apart = [&](const mgpu_buf* x, int64_t ld) {
+            if (!out.overlaps(rows_range(x, rows, kw, ld))) return true;
+            const int64_t es = (int64_t)elem_size(q->type), delta = (const char*)x->ptr - (const char*)q->ptr;
+            if (x->type != q->type || ld != a.ldq || delta % es) return false;
+            const int64_t column = (delta / es % ld + ld) % ld;
+            return column >= qw && column + kw <= ld;
+        };
         if (q_out->ptr == q->ptr)
-            REQUIRE(q_out->type == q->type && a.ldqo == a.ldq, "kv_append: q_out in place must have q's type and pitch");
+            REQUIRE(q_out->type == q->type && a.ldqo == a.ldq && apart(k, a.ldk) && apart(v, a.ldv),
+                    "kv_append: q_out in place must have q's type and pitch, and columns apart from k and v");
         else
             REQUIRE(!out.overlaps(rows_range(q, rows, qw, a.ldq)), "kv_append: q_out overlaps q without being q");
         for (const Range& r : caches) REQUIRE(!out.overlaps(r), "kv_append: q_out overlaps the cache");
@@ -1213,6 +1231,14 @@ mgpu_event* mgpu_kv_append(const mgpu_kv_cache* c, const mgpu_paged_batch* batch
         a.n_axes = rope->n_axes;
         a.end0 = rope->sections[0];
         a.end1 = a.end0 + (rope->n_axes > 1 ? rope->sections[1] : 0);
+    }
+    const Range written[3] = {caches[0], caches[1], q ? rows_range(q_out, rows, (int64_t)q_heads * c->head_dim, a.ldqo) : kNoRange};
+    for (const Range& w : written) {
+        REQUIRE(!in_batch(w, batch), "kv_append: cu_q, kv_lens or page_table in the cache or q_out");
+        if (rope)
+            REQUIRE(!w.overlaps(words_range(rope->table, (int64_t)rope->max_pos * rope->rot_dim)) &&
+                        !w.overlaps(words_range(rope->positions, (int64_t)rope->n_axes * rows)),
+                    "kv_append: the rope table or positions in the cache or q_out");
     }
     mgpu_device* d = c->dev;
     DeviceGuard g(d->ordinal);
@@ -1260,6 +1286,7 @@ mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* c, const mgpu_paged_batch*
     REQUIRE(!ro.overlaps(rows_range(q, rows, width, a.ldq)), "paged_attention: out overlaps q");
     REQUIRE(!ro.overlaps(range_of(c->k, c->k->bytes)) && !ro.overlaps(range_of(c->v, c->v->bytes)),
             "paged_attention: out overlaps the cache");
+    REQUIRE(!in_batch(ro, batch), "paged_attention: cu_q, kv_lens or page_table in out");
     // the kernels count blocks of 64 or 128 keys, and pairs of tiles over them, in 32 bits
     const int64_t most_kv = (int64_t)batch->max_pages * c->page_size, group = q_heads / c->kv_heads;
     const int64_t pairs = rows / (2 * (kMaxGroup / group)) + batch->n_seqs;
@@ -1351,6 +1378,17 @@ mgpu_event* mgpu_logits_process(const mgpu_device* cd, mgpu_buf* logits, mgpu_bu
                 "words", rows, (n + 31) / 32);
         a.allowed = (const uint32_t*)r->allowed->ptr;
     }
+    // other CTAs may still read these when a row's results are written
+    const Range read[] = {words_range(r->history, (int64_t)rows * r->history_ld), words_range(r->history_lens, rows),
+                          words_range(r->prompt_lens, rows), words_range(r->penalties, (int64_t)rows * 3),
+                          words_range(r->bias_offsets, (int64_t)rows + 1), words_range(r->bias_tokens, a.bias_entries),
+                          words_range(r->bias_values, a.bias_entries), words_range(r->allowed, (int64_t)rows * ((n + 31) / 32))};
+    const Range written = out ? rows_range(out, rows, n, a.ldo) : kNoRange;
+    const Range pairs = best ? range_of(best, (size_t)rows * 8) : kNoRange;
+    for (const Range& w : read)
+        REQUIRE(!w.overlaps(written) && !w.overlaps(pairs), "logits_process: out or best overlaps what the rules are read from");
+    REQUIRE(!pairs.overlaps(rows_range(logits, rows, n, a.ldx)) && !pairs.overlaps(written),
+            "logits_process: best overlaps logits or out");
     a.x = logits->ptr;
     a.type = logits->type;
     a.rows = rows;

@@ -310,8 +310,11 @@ void mgpu_kv_cache_release(mgpu_kv_cache* cache);
  * the counts below are the host's: n_tokens activation rows (rows of no sequence are left alone),
  * max_q_len the most new tokens of a sequence, max_pages the row pitch of page_table.  Contents
  * that do not fit (pages outside the cache, more new tokens than max_q_len, lengths beyond
- * max_pages * page_size, a new token before index 0) are skipped, and the next mgpu_finish or
- * mgpu_buf_read reports MGPU_ERR_INVALID_ARG; no access leaves the buffers. */
+ * max_pages * page_size) are skipped, and the next mgpu_finish or mgpu_buf_read reports
+ * MGPU_ERR_INVALID_ARG; no access leaves the buffers.  A sequence may be shorter than its new tokens:
+ * the first of them then stand before index 0.  They have no place in the cache, so mgpu_kv_append
+ * skips and reports them; to mgpu_paged_attention they are tokens before the first key, which see
+ * nothing under a causal mask and every key without one. */
 typedef struct mgpu_paged_batch {
     mgpu_buf* cu_q;       /* int32 [n_seqs + 1] */
     mgpu_buf* kv_lens;    /* int32 [n_seqs] */

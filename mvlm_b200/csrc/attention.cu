@@ -259,7 +259,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         enter(w, start_seq);
         w.h = (begin - start_before) / w.blocks;
         w.k = (begin - start_before) % w.blocks;
-        for (int i = 0, pos = begin; pos < end; ++i) {
+        int i = 0;
+        for (int pos = begin; pos < end; ++i) {
             const int x = i % kItems, k1 = min(w.blocks, w.k + (end - pos)), R = w.s.n * G;
             if (!wait(&item_empty[x], (i / kItems) ^ 1)) break;
             if (lane == 0) {
@@ -293,6 +294,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
             w.k = 0;
             if (++w.h == a.hkv && pos < end) enter(w, w.b + 1);
         }
+        // the copies under way land before the CTA may end, also where other warps gave up
+        for (int x = max(0, i - kItems); x < i; ++x) wait(&item_full[x % kItems], x / kItems);
         return;
     }
     if (warp >= kRowsWarps) {
@@ -1138,11 +1141,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const uint32_t id_o = idesc_f16(kBf16, false, true, kTileRows, (a.D + 15) / 16 * 16);
             const uint32_t d_s = tmem + t * kTileKeys, d_o = tmem + 256 + t * 128;
             const int dims = (a.D + 15) / 16;
-            uint32_t free_phase = 0;
+            uint32_t free_phase = 0, q_loads = 0;
             // A tile's queries: whole tokens of the key head's query heads, which lie in its rows' order.
             // Rows beyond the tile's hold other tokens' or old values; nothing of theirs is written.
             auto load_q = [&](const Segment& g) {
                 if (!a.q_tma || g.lo[t] >= g.hi[t]) return;
+                ++q_loads;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(&q_bar[t], (uint32_t)(SLABS * 128 * G * per_tile));
                     for (int slab = 0; slab < SLABS; ++slab)
@@ -1214,6 +1218,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (lane == 0) mbar_arrive(&seg_empty[i % kSegments]);
                 __syncwarp();
             }
+            // a wait ran out: queries under way still have to land before the CTA may end
+            if (q_loads > q_phase) wait(&q_bar[t], q_phase);
             if (elect_one()) umma_commit(&drain_bar);  // all products have ended before TMEM is given back
             __syncwarp();
             wait(&drain_bar, 0);

@@ -39,12 +39,12 @@ struct Place {
 __device__ __forceinline__ bool place_of(const mgpu_k::AppendArgs& a, int t, Place& p) {
     const int seq = seq_of_token(a.batch, t);
     if (seq < 0) return false;
-    const int q0 = a.batch.cu_q[seq], q1 = a.batch.cu_q[seq + 1];
-    const int index = a.batch.kv_lens[seq] - (q1 - t);  // of this token in its sequence
+    const int q0 = a.batch.cu_q[seq], q1 = a.batch.cu_q[seq + 1], kv = a.batch.kv_lens[seq];
+    const int index = max(kv, 0) - (q1 - t);  // of this token in its sequence
     int page = -1;
     if (index >= 0 && index / a.page_size < a.batch.max_pages)
         page = a.batch.page_table[(int64_t)seq * a.batch.max_pages + index / a.page_size];
-    bool bad = page < 0 || page >= a.num_pages || q1 > a.batch.n_tokens || q1 - q0 > a.batch.max_q_len;
+    bool bad = page < 0 || page >= a.num_pages || q0 < 0 || q1 > a.batch.n_tokens || q1 - q0 > a.batch.max_q_len;
 #pragma unroll
     for (int x = 0; x < 3; ++x) {
         p.pos[x] = index;

@@ -32,3 +32,33 @@ def test_every_page_outside_the_cache_is_reported(dev, n, page):
         reported(dev)
         got = from_bits(dst.read(np.uint16), mg.F16).view(-1, 4, 64)
         assert_within(got[n:], want[n:], tol[n:], f"page {page} at {at}")
+
+
+def test_append_reports_a_start_before_the_rows(dev):
+    pool = Pool(dev, [2, 3], [10, 20], 2, 64, 16, mg.F16, max_q_len=2 ** 31 - 1)
+    x = dev.array(np.ones((5, 128), np.float32), mg.F32)
+    for start in (-1, -2 ** 31, -2 ** 31 + 1):
+        pool.buffers[0].write(np.array([start, 2, 5], np.int32))
+        mg.kv_append(pool.cache, pool.batch, None, x, x, None, 0)
+        reported(dev)
+        k = from_bits(pool.cache.k.read(np.uint16), mg.F16).view(pool.k.shape)
+        want = pool.k.clone()
+        for p in range(17, 20):
+            want[pool.table[1, p // 16], :, p % 16] = 1.0
+        assert torch.equal(k, want), start
+
+
+def test_append_reports_negative_lengths_under_a_wide_table(dev):
+    # 2.2e9 places in the table: an index that wrapped around would find a page there
+    page, wide = 1000, 2_200_000
+    cache = mg.KVCache(dev, 2, page, 1, 8, mg.F16)
+    x = dev.array(np.ones((2, 8), np.float32), mg.F32)
+    lens = dev.array(np.array([0], np.int32), mg.F32)
+    batch = mg.PagedBatch(dev.array(np.array([0, 2], np.int32), mg.F32), lens, dev.array(np.zeros(wide, np.int32), mg.F32), 1, 2, 2, wide)
+    for kv in (-2 ** 31, -2 ** 31 + 1, -1, 0, 1):
+        lens.write(np.array([kv], np.int32))
+        mg.kv_append(cache, batch, None, x, x, None, 0)
+        reported(dev)
+        k = from_bits(cache.k.read(np.uint16), mg.F16).view(2, page, 8)
+        assert bool((k[:, 1:] == 0).all()) and bool((k[1] == 0).all()), kv
+        assert bool((k[0, 0] == (1.0 if kv == 1 else 0.0)).all()), kv  # of two tokens, the second has a place

@@ -314,7 +314,8 @@ void mgpu_kv_cache_release(mgpu_kv_cache* cache);
  * MGPU_ERR_INVALID_ARG; no access leaves the buffers.  A sequence may be shorter than its new tokens:
  * the first of them then stand before index 0.  They have no place in the cache, so mgpu_kv_append
  * skips and reports them; to mgpu_paged_attention they are tokens before the first key, which see
- * nothing under a causal mask and every key without one. */
+ * nothing under a causal mask and every key without one.  Rows that sequences share, as where cu_q
+ * descends, are undefined. */
 typedef struct mgpu_paged_batch {
     mgpu_buf* cu_q;       /* int32 [n_seqs + 1] */
     mgpu_buf* kv_lens;    /* int32 [n_seqs] */

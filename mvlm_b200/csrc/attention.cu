@@ -880,8 +880,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
     // ---- the table of items: pairs before each sequence, blocks before each run of pairs
     const int seqs = min(a.batch.n_seqs - seq0, kTileSeqs);
+    bool bad = false;
     auto view = [&](int b) {
-        bool bad = false;
         SeqView s = seq_view(a.batch, seq0 + b, a.page_size, &bad);
         if (bad) report_contents(a.status);
         if ((long long)s.n * G <= a.max_rows) s.n = 0;  // the rows kernel's
@@ -911,7 +911,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncthreads();
     };
     for (int b = tid; b < seqs; b += kTileThreads) seq_first[b] = (view(b).n + 2 * per_tile - 1) / (2 * per_tile);
-    __syncthreads();
+    if (__syncthreads_or(bad)) {
+        // Sequences that share rows, between which cu_q descends, could have more items than the host's bound
+        // on the 32-bit counts below allows for.
+        long long rows = 0;
+        for (int b = 0; b < seqs; ++b) rows += view(b).n;
+        if (rows > a.batch.n_tokens) return;
+    }
     scan(seq_first, seqs);
     const int pairs = seq_first[seqs];
     if (pairs == 0) return;

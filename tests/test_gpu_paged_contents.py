@@ -62,3 +62,15 @@ def test_append_reports_negative_lengths_under_a_wide_table(dev):
         k = from_bits(cache.k.read(np.uint16), mg.F16).view(2, page, 8)
         assert bool((k[:, 1:] == 0).all()) and bool((k[1] == 0).all()), kv
         assert bool((k[0, 0] == (1.0 if kv == 1 else 0.0)).all()), kv  # of two tokens, the second has a place
+
+
+def test_sequences_that_share_rows(dev):
+    # cu_q descends: more new tokens in all than there are rows, which the counts of items do not allow for
+    n = 300
+    pool = Pool(dev, [n, 0, n], [400, 400, 500], 2, 64, 16, mg.F16)
+    pool.tokens = pool.batch.c.n_tokens = n
+    pool.buffers[0].write(np.array([0, n, 0, n], np.int32))
+    src, dst = dev.array(np.zeros(n * 256, np.uint16), mg.F16), dev.array(np.full(n * 256, 0x4000, np.uint16), mg.F16)
+    mg.paged_attention(pool.cache, pool.batch, src, dst, 4)
+    reported(dev)
+    assert bool((dst.read(np.uint16) == 0x4000).all())

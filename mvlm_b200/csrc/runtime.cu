@@ -1170,6 +1170,11 @@ mgpu_event* mgpu_kv_append(const mgpu_kv_cache* c, const mgpu_paged_batch* batch
     if (!batch_ok(batch, "kv_append", &a.batch)) return nullptr;
     const int64_t rows = batch->n_tokens, kw = (int64_t)c->kv_heads * c->head_dim;
     if (!rows_ok(k, rows, kw, "kv_append", "k", &a.ldk) || !rows_ok(v, rows, kw, "kv_append", "v", &a.ldv)) return nullptr;
+    // the kernels count a token's values in 32 bits
+    if (((q ? (int64_t)q_heads : 0) + 2 * (int64_t)c->kv_heads) * c->head_dim > 1 << 30) {
+        set_error(MGPU_ERR_UNSUPPORTED, "kv_append: more than 2^30 values of a token");
+        return nullptr;
+    }
     const size_t bytes = c->k->bytes;
     Range caches[2] = {range_of(c->k, bytes), range_of(c->v, bytes)};
     if (q) {

@@ -48,6 +48,16 @@ def test_append_reports_a_start_before_the_rows(dev):
         assert torch.equal(k, want), start
 
 
+def test_more_values_of_a_token_than_are_counted(dev):
+    pool = Pool(dev, [1], [10], 2, 64, 16, mg.F16)
+    x, q = dev.array(np.ones((1, 128), np.float32), mg.F32), dev.empty(256, mg.F16)
+    for heads, code in ((2 ** 24 - 3, mg.ERR_UNSUPPORTED), (2 ** 31 - 1, mg.ERR_UNSUPPORTED), (2 ** 24 - 4, mg.ERR_INVALID_ARG), (5, mg.ERR_INVALID_ARG)):
+        with pytest.raises(mg.MgpuError) as e:  # the last two fit, but q does not hold them
+            mg.kv_append(pool.cache, pool.batch, q, x, x, dev.empty(256, mg.F16), heads)
+        assert e.value.code == code, heads
+    dev.finish()
+
+
 def test_append_reports_negative_lengths_under_a_wide_table(dev):
     # 2.2e9 places in the table: an index that wrapped around would find a page there
     page, wide = 1000, 2_200_000

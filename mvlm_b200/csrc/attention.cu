@@ -880,8 +880,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // not before: what came before us is then over
     // ---- the table of items: pairs before each sequence, blocks before each run of pairs
     const int seqs = min(a.batch.n_seqs - seq0, kTileSeqs);
-    bool bad = false;
     auto view = [&](int b) {
+        bool bad = false;
         SeqView s = seq_view(a.batch, seq0 + b, a.page_size, &bad);
         if (bad) report_contents(a.status);
         if ((long long)s.n * G <= a.max_rows) s.n = 0;  // the rows kernel's
@@ -910,8 +910,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (tid == kTileThreads - 1) v[n] = before;
         __syncthreads();
     };
-    for (int b = tid; b < seqs; b += kTileThreads) seq_first[b] = (view(b).n + 2 * per_tile - 1) / (2 * per_tile);
-    if (__syncthreads_or(bad)) {
+    bool descends = false;
+    for (int b = tid; b < seqs; b += kTileThreads) {
+        descends |= a.batch.cu_q[seq0 + b + 1] < a.batch.cu_q[seq0 + b];
+        seq_first[b] = (view(b).n + 2 * per_tile - 1) / (2 * per_tile);
+    }
+    if (__syncthreads_or(descends)) {
         // Sequences that share rows, between which cu_q descends, could have more items than the host's bound
         // on the 32-bit counts below allows for.
         long long rows = 0;

@@ -21,6 +21,10 @@ using namespace mgpu_dev;
 namespace {
 
 constexpr float kGrowth = 8.0f;  // log2 of how far a weight may exceed 1 before its row's reference moves
+// log2 of what a weight of 1 is in fp16, whose values are 2^-24 apart at least: with kGrowth weights stay below
+// 2^16, and those down to 2^-32 count, not only in the sums l.  (What the tensor cores' fp32 sums drop, in either
+// type, are products below some 2^-24 of the sum that they are added to.)
+template <typename T> __host__ __device__ constexpr float weight_log2() { return std::is_same<T, __half>::value ? 7.0f : 0.0f; }
 constexpr int kBoxRows = 64;  // most rows of a box of the cache's TMA maps
 
 // ------------------------------------------------------------------ masks -----------
@@ -153,6 +157,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     constexpr int KEYS = rows_keys<DP>(), KW = KEYS / 4;   // of a block, of a warp
     constexpr int SLABS = DP / 64, SLAB = KEYS * 128;      // 64 dims of a block's keys, 128-byte rows, swizzled
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
+    constexpr float LOG2_1 = weight_log2<T>();
     static_assert(S % 2 == 0, "a stage belongs to one group of warps");
     constexpr int QP = rows_q_pitch<DP>();
     extern __shared__ uint8_t smem_raw[];
@@ -425,8 +430,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                             if (j < sr[e >> 1].lo || j >= sr[e >> 1].hi) sc[n][e] = -INFINITY;
                         }
                 }
-                // The reference m, which the maximum may exceed by kGrowth before it moves (weights then stay
-                // below 2^kGrowth, and O mostly as it is), and the sum.
+                // The reference m, which the maximum may exceed by kGrowth (and LOG2_1, as a weight of 1 counts)
+                // before it moves, so that O mostly stays as it is, and the sum.
                 uint32_t pf[KW / 16][4];
                 float top[2];
 #pragma unroll
@@ -437,11 +442,11 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2)) * a.scale_log2;
                 }
-                if (__any_sync(0xffffffffu, top[0] > m[0] + kGrowth || top[1] > m[1] + kGrowth)) {
+                if (__any_sync(0xffffffffu, top[0] > m[0] + (LOG2_1 + kGrowth) || top[1] > m[1] + (LOG2_1 + kGrowth))) {
                     float r[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float mn = fmaxf(m[i], top[i]);
+                        const float mn = fmaxf(m[i], top[i] - LOG2_1);
                         r[i] = mn == -INFINITY ? 1.0f : ex2(m[i] - mn);
                         m[i] = mn;
                         l[i] *= r[i];
@@ -838,6 +843,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int S = tile_stages<DP>();
     constexpr int PIECE = kTileRows * (DP + 2);
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
+    constexpr float LOG2_1 = weight_log2<T>();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* ring = qs + 2 * QB;
@@ -1279,7 +1285,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const int kb0 = g.lo[t], kb1 = g.hi[t];
             const bool valid = row < g.rows[t];
             const Seen sr = valid ? seen_at(a, g.kv, g.index[t] + row / G) : Seen{0, 0};
-            float m = -INFINITY, l = 0.0f;  // the reference (log2 units) and the sum of 2^(s - m)
+            float m = -INFINITY, l = 0.0f;  // the reference (log2 units, less LOG2_1) and the sum of 2^(s - m)
             // The scores of half `half` at keys j0 .. are asked for; they are there after tmem_ld_wait.
             auto fetch = [&](uint32_t (&sa)[32], uint32_t (&sb)[32], const int half) {
                 ok = wait(&s_bar[t][half], s_phase);
@@ -1311,10 +1317,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     x3 = max3(x3, __uint_as_float(sb[e + 2]), __uint_as_float(sb[e + 3]));
                 }
                 const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3)) * a.scale_log2;
-                const bool grown = top > m + kGrowth;
+                const bool grown = top > m + (LOG2_1 + kGrowth);
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float f = grown ? ex2(m - top) : 1.0f;
-                    if (grown) m = top;
+                    const float f = grown ? ex2(m - (top - LOG2_1)) : 1.0f;
+                    if (grown) m = top - LOG2_1;
                     l *= f;
                     if (j0 > kb0 * kTileKeys) {
                         // O as the half before left it.  A barrier to each half: the phases before that one's

@@ -161,21 +161,36 @@ struct Walk {
 };
 
 // The sums of the NaN and Inf that row r sees in dims d and d + 1 of V.  (The products of a weight and its rest
-// with Inf can be Inf and -Inf; such a value is rare, and looked up in the cache again.)
+// with Inf can be Inf and -Inf; such a value is rare, and looked up in the cache again: eight keys of a page at a
+// time, so that a million of them take a thread some 0.1 s and not a second, within which loads wait for a stage.)
 template <typename T>
 __device__ __noinline__ float2 odd_values(const mgpu_k::AttendArgs& a, SeqView s, int seq, int h, int r, int d) {
     constexpr bool kBf16 = !std::is_same<T, __half>::value;
     const Seen seen = seen_by(a, s, r / (a.hq / a.hkv));
     float2 odd = make_float2(0.0f, 0.0f);
+    constexpr int ABREAST = 8;  // a page's places are a multiple of it
 #pragma unroll 1
-    for (int j = seen.lo; j < seen.hi; ++j) {
-        const int page = __ldg(a.batch.page_table + (int64_t)seq * a.batch.max_pages + j / a.page_size);
-        if (page < 0 || page >= a.num_pages) continue;
-        const uint32_t y = *reinterpret_cast<const uint32_t*>(
-            reinterpret_cast<const T*>(a.vc) + (((int64_t)page * a.hkv + h) * a.page_size + j % a.page_size) * a.D + d);
-        const float2 f = unpack2<T>(y);
-        if (odd16(y, kBf16)) odd.x += f.x;
-        if (odd16(y >> 16, kBf16)) odd.y += f.y;
+    for (int j0 = seen.lo / ABREAST * ABREAST, at = j0 / a.page_size, place = j0 % a.page_size, page = -1; j0 < seen.hi; j0 += ABREAST) {
+        if (place == a.page_size) {
+            place = 0;
+            ++at;
+            page = -1;
+        }
+        if (page < 0) page = __ldg(a.batch.page_table + (int64_t)seq * a.batch.max_pages + at);
+        if (page >= 0 && page < a.num_pages) {
+            const T* v = reinterpret_cast<const T*>(a.vc) + (((int64_t)page * a.hkv + h) * a.page_size + place) * a.D + d;
+            uint32_t y[ABREAST];
+#pragma unroll
+            for (int x = 0; x < ABREAST; ++x) y[x] = *reinterpret_cast<const uint32_t*>(v + (int64_t)x * a.D);
+#pragma unroll
+            for (int x = 0; x < ABREAST; ++x) {
+                if (j0 + x < seen.lo || j0 + x >= seen.hi) continue;
+                const float2 f = unpack2<T>(y[x]);
+                if (odd16(y[x], kBf16)) odd.x += f.x;
+                if (odd16(y[x] >> 16, kBf16)) odd.y += f.y;
+            }
+        }
+        place += ABREAST;
     }
     return odd;
 }

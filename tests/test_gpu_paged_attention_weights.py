@@ -78,3 +78,27 @@ def test_odd_values_that_are_seen(dev, t, new, kv, hq, window):
     want, _ = pool.attention(q, hq, 0.125, window=window)
     # (scores of some hundred: their fp32 error is in every weight)
     assert_within(got, want, 4 * bound(pool, q, hq, 0.125, want, window=window), f"{new} {kv}")
+
+
+def test_odd_values_among_a_million_keys(dev):
+    # 16 rows, each of whose values is looked up again, by one CTA or another; the two pages hold all keys there are
+    kv, page, n, hq = 1000000, 16, 2, 8
+    g = torch.Generator().manual_seed(3)
+    k, v = torch.randn(2, 1, page, 64, generator=g).half(), torch.randn(2, 1, page, 64, generator=g).half()
+    v[1, 0, 5, ::2], v[1, 0, 6, 3], v[1, 0, 7, 7] = float("inf"), -float("inf"), float("nan")
+    v[1, 0, 8, 0] = -float("inf")
+    cache = mg.KVCache(dev, 2, page, 1, 64, mg.F16, k=dev.array(to_bits(k, mg.F16), mg.F16), v=dev.array(to_bits(v, mg.F16), mg.F16))
+    table = np.zeros((3, kv // page), np.int32)
+    table[:, 7] = table[1, -1] = 1
+    lens = np.array([kv, kv - 3, kv], np.int32)
+    batch = mg.PagedBatch(ints(dev, np.arange(4) * n), ints(dev, lens), ints(dev, table), 3, 3 * n, n, table.shape[1])
+    q = torch.randn(3 * n, hq, 64, generator=g).half()
+    out = dev.empty(3 * n * hq * 64, mg.F16)
+    mg.paged_attention(cache, batch, dev.array(to_bits(q, mg.F16), mg.F16), out, hq)
+    dev.finish()
+    got = from_bits(out.read(np.uint16), mg.F16).view(3 * n, hq, 64)
+    want = torch.zeros(64)
+    want[::2], want[3], want[7], want[0] = float("inf"), -float("inf"), float("nan"), float("nan")
+    odd = ~torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), (~odd).expand(got.shape))
+    torch.testing.assert_close(got[..., odd].float(), want[odd].expand(3 * n, hq, -1), equal_nan=True)

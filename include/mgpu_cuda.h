@@ -360,8 +360,8 @@ mgpu_event* mgpu_kv_append(const mgpu_kv_cache* cache, const mgpu_paged_batch* b
  * per sequence, mixed in one call.  q and out of the cache's type, [n_tokens][q_heads * head_dim]
  * at their tag's pitch; q_heads a multiple of kv_heads, at most 128 to a key head.  scale 0 means
  * 1 / sqrt(head_dim).  fp32 scores, softmax and sums.  The tensor cores take a weight in the cache's
- * type: in two parts, 16 to 22 bits, where a sequence's new tokens times the query heads of a key head are
- * at most 16 (but for a call with one sequence whose max_q_len allows for more), else rounded to it.  Uses the device's scratch (run once before a graph capture). */
+ * type: in two parts, 16 to 22 bits, for single tokens and other few rows (a sequence's new tokens times the
+ * query heads of a key head, up to 8 or 16), else rounded to it.  Uses the device's scratch (run once before a graph capture). */
 mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* cache, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* out,
                                  int q_heads, float scale, int causal, int window);
 

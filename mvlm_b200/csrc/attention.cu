@@ -54,10 +54,11 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // Two weights in the products' 16 bits, and what that leaves of them: together 16 bits of bf16, 22 of fp16.
-// With few rows to a key head both are multiplied, so that the result is rounded once.  The second product
-// costs 64 sequences of 128 dims 102.6 -> 105.1 us, a long context 90.9 -> 92.3, one sequence 9.9 -> 10.1; without it
-// errors against 64 bits are up to 1.26 times those of one rounding (in mean squares; 1.4 at their greatest).
-// Many rows are bound by their products, and their weights are rounded.
+// With few rows to a key head both are multiplied, so that the result is rounded once: without the rests errors
+// against 64 bits are up to 1.26 times those of one rounding (in mean squares; 1.4 at their greatest).  Up to 8
+// rows leave 8 of the products' 16 free, and these take the rests (64 sequences of 4 rows: 102.5 us without, 102.0
+// with).  9 to 16 rows take a second product (64 sequences of 16 rows: 125 us without, 128 with).  Many rows are
+// bound by their products, and their weights are rounded.
 template <typename T> __device__ __forceinline__ void split2(float x, float y, uint32_t& w, uint32_t& rest) {
     w = pack2<T>(x, y);
     const float2 f = unpack2<T>(w);
@@ -195,7 +196,8 @@ __device__ __noinline__ float2 odd_values(const mgpu_k::AttendArgs& a, SeqView s
     return odd;
 }
 
-template <typename T, int DP>
+// NARROW: at most 8 rows, and the products' other 8 take the rests of their weights.
+template <typename T, int DP, bool NARROW>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     attend_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const __grid_constant__ mgpu_k::AttendArgs a) {
@@ -401,8 +403,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const int g = lane >> 2, c2 = 2 * (lane & 3);  // this thread's rows g and g + 8, and first column
     // Two items' states of up to 8 rows fit the scratch, and the barrier of the item between says that the
     // last ones have been read.  Where an item may have more rows, each takes both places, and a barrier more.
-    const bool wide = (long long)a.batch.max_q_len * G > 8;
-    const int room = wide ? kRowsMax : 8;
+    constexpr int HALVES = NARROW ? 1 : 2, room = 8 * HALVES;  // of 8 rows: this thread's are g + 8 x, x < HALVES
     uint32_t it = 0;
     struct {
         SeqView s;
@@ -411,8 +412,13 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     for (int i = 0, more = 1; more; ++i) {
         const int slot = i % kItems, turn = i & 1;
         int k0 = 0, k1 = 0, base = 0, item_begin = 0, R = 0;
-        Seen sr[2];
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[DP / 8][4];
+        Seen sr[HALVES];
+        float m[HALVES], l[HALVES], o[DP / 8][4];
+#pragma unroll
+        for (int x = 0; x < HALVES; ++x) {
+            m[x] = -INFINITY;
+            l[x] = 0.0f;
+        }
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) ldsm4(qf[k], qa + 32 * k);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) sr[x] = g + 8 * x < R ? seen_by(a, w.s, (g + 8 * x) / G) : Seen{0, 0};
+            for (int x = 0; x < HALVES; ++x) sr[x] = g + 8 * x < R ? seen_by(a, w.s, (g + 8 * x) / G) : Seen{0, 0};
             __syncwarp();
             if (lane == 0) mbar_arrive(&item_empty[slot]);
             // keys [s1.lo, s0.hi) are seen by every row
@@ -472,7 +478,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
                     for (int n = 0; n < KW / 8; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
+                        for (int e = 0; e < 2 * HALVES; ++e) {
                             const int j = j0 + 8 * n + c2 + (e & 1);
                             if (j < sr[e >> 1].lo || j >= sr[e >> 1].hi) sc[n][e] = -INFINITY;
                         }
@@ -480,19 +486,21 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 // The reference m, which the maximum may exceed by kGrowth (and LOG2_1, as a weight of 1 counts)
                 // before it moves, so that O mostly stays as it is, and the sum.
                 uint32_t pf[KW / 16][4], rest[KW / 16][4];
-                float top[2];
+                float top[HALVES];
+                bool grown = false;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < HALVES; ++i) {
                     top[i] = fmaxf(sc[0][2 * i], sc[0][2 * i + 1]);
 #pragma unroll
                     for (int n = 1; n < KW / 8; ++n) top[i] = fmaxf(top[i], fmaxf(sc[n][2 * i], sc[n][2 * i + 1]));
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
                     top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2)) * a.scale_log2;
+                    grown |= top[i] > m[i] + (LOG2_1 + kGrowth);
                 }
-                if (__any_sync(0xffffffffu, top[0] > m[0] + (LOG2_1 + kGrowth) || top[1] > m[1] + (LOG2_1 + kGrowth))) {
-                    float r[2];
+                if (__any_sync(0xffffffffu, grown)) {
+                    float r[HALVES];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < HALVES; ++i) {
                         const float mn = fmaxf(m[i], top[i] - LOG2_1);
                         r[i] = mn == -INFINITY ? 1.0f : ex2(m[i] - mn);
                         m[i] = mn;
@@ -501,10 +509,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
                     for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[n][e] *= r[e >> 1];
+                        for (int e = 0; e < 4; ++e) o[n][e] *= r[NARROW ? 0 : e >> 1];
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < HALVES; ++i) {
                     const float neg = m[i] == -INFINITY ? 0.0f : -m[i];
 #pragma unroll
                     for (int u = 0; u < KW / 16; ++u) {
@@ -512,8 +520,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) p[e] = ex2(fmaf(sc[2 * u + (e >> 1)][2 * i + (e & 1)], a.scale_log2, neg));
                         l[i] += (p[0] + p[1]) + (p[2] + p[3]);
-                        split2<T>(p[0], p[1], pf[u][i], rest[u][i]);
-                        split2<T>(p[2], p[3], pf[u][2 + i], rest[u][2 + i]);
+                        split2<T>(p[0], p[1], pf[u][i], NARROW ? pf[u][1] : rest[u][i]);
+                        split2<T>(p[2], p[3], pf[u][2 + i], NARROW ? pf[u][3] : rest[u][2 + i]);
                     }
                 }
                 if (__builtin_expect(!whole, 0)) {
@@ -533,7 +541,8 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 #pragma unroll 1
                         for (int j = 0; j < KW; ++j) {
                             const int r = KW * part + j;
-                            const bool s_lo = j0 + j >= sr[0].lo && j0 + j < sr[0].hi, s_hi = j0 + j >= sr[1].lo && j0 + j < sr[1].hi;
+                            const bool s_lo = j0 + j >= sr[0].lo && j0 + j < sr[0].hi;
+                            const bool s_hi = !NARROW && j0 + j >= sr[HALVES - 1].lo && j0 + j < sr[HALVES - 1].hi;
 #pragma unroll
                             for (int n = 0; n < DP / 8; ++n) {
                                 const uint32_t v = *reinterpret_cast<const uint32_t*>(vs + (n >> 3) * SLAB + r * 128 +
@@ -566,8 +575,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                         ldsm4_t(b, vb + (n / 4) * SLAB + row * 128 + ((ch ^ (row & 7)) << 4));
                         mma16816<T>(o[2 * n], pf[u], b[0], b[1]);
                         mma16816<T>(o[2 * n + 1], pf[u], b[2], b[3]);
-                        mma16816<T>(o[2 * n], rest[u], b[0], b[1]);
-                        mma16816<T>(o[2 * n + 1], rest[u], b[2], b[3]);
+                        if constexpr (!NARROW) {
+                            mma16816<T>(o[2 * n], rest[u], b[0], b[1]);
+                            mma16816<T>(o[2 * n + 1], rest[u], b[2], b[3]);
+                        }
                     }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty_bar[st]);
@@ -575,7 +586,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
         }
         // ---- the eight warps' states join: each leaves its own, and whoever writes a value weighs them
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < HALVES; ++x) {
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
             l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
             if ((lane & 3) == 0) {
@@ -583,13 +594,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 sm_l[turn][warp][g + 8 * x] = l[x];
             }
         }
-        float* states = scratch + (wide ? 0 : turn * kRowsWarps * 8 * PITCH);
+        float* states = scratch + (NARROW ? turn * kRowsWarps * 8 * PITCH : 0);
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < HALVES; ++x)
             if (g + 8 * x < R)
 #pragma unroll
                 for (int n = 0; n < DP / 8; ++n)
-                    *reinterpret_cast<float2*>(states + (warp * room + g + 8 * x) * PITCH + 8 * n + c2) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
+                    *reinterpret_cast<float2*>(states + (warp * room + g + 8 * x) * PITCH + 8 * n + c2) =
+                        NARROW ? make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]) : make_float2(o[n][2 * x], o[n][2 * x + 1]);
         if (named_barrier_or(1, 32 * kRowsWarps, dead)) break;
         // ---- rows out, or this share's state of an item that other CTAs have parts of
         const bool complete = k0 == 0 && k1 == w.blocks;
@@ -712,7 +724,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
                 }
             }
         }
-        if (wide || !complete) named_barrier_sync(1, 32 * kRowsWarps);  // the places are free again
+        if (!NARROW || !complete) named_barrier_sync(1, 32 * kRowsWarps);  // the places are free again
     }
 }
 
@@ -730,9 +742,9 @@ cudaError_t allow_smem(K kern, int smem, std::atomic<uint64_t>& configured) {
     return cudaSuccess;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool NARROW>
 cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const mgpu_k::AttendArgs& a) {
-    auto kern = attend_rows_kernel<T, DP>;
+    auto kern = attend_rows_kernel<T, DP, NARROW>;
     static std::atomic<uint64_t> configured{0};
     const cudaError_t e = allow_smem(kern, rows_smem<DP>(), configured);
     if (e != cudaSuccess) return e;
@@ -1600,7 +1612,9 @@ cudaError_t launch_tiles(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, cons
 template <typename T>
 cudaError_t launch_attend(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const CUtensorMap& mv, const mgpu_k::AttendArgs& a) {
     cudaError_t e = cudaSuccess;
-    if (a.max_rows > 0) e = a.D <= 64 ? launch_rows<T, 64>(c, mk, mv, a) : launch_rows<T, 128>(c, mk, mv, a);
+    const bool narrow = a.max_rows <= 8;
+    if (a.max_rows > 0 && narrow) e = a.D <= 64 ? launch_rows<T, 64, true>(c, mk, mv, a) : launch_rows<T, 128, true>(c, mk, mv, a);
+    else if (a.max_rows > 0) e = a.D <= 64 ? launch_rows<T, 64, false>(c, mk, mv, a) : launch_rows<T, 128, false>(c, mk, mv, a);
     if (e != cudaSuccess || !mgpu_k::attend_many_rows(a)) return e;
     return a.D <= 64 ? launch_tiles<T, 64>(c, mk, mv, a) : launch_tiles<T, 128>(c, mk, mv, a);
 }
@@ -1627,8 +1641,13 @@ cudaError_t paged_attention(const LaunchCtx& c, const CUtensorMap& mk, const CUt
     AttendArgs a = in;
     a.box_rows = kBoxRows;
     while (a.page_size % a.box_rows) a.box_rows /= 2;
-    // one sequence of a chunk: the kernel for many rows alone, however few it turns out to have
-    a.max_rows = a.batch.n_seqs == 1 && attend_many_rows(a) ? 0 : kRowsMax;
+    // The most rows that go to the kernel for few.  One sequence of a chunk: none, however few it turns out to
+    // have.  Where no sequence has more than 8: those, whose weights' rests are then free.  Beside chunks the same,
+    // if single tokens have no more than 8 (4 chunks of 300 and 20 single tokens of 4 rows: 117.7 us, 119.3 with
+    // 16; 20 times 3 tokens, which are then tiles: 110 and 128; 60 times 4 tokens: 204 and 202).
+    const int64_t group = a.hq / a.hkv;
+    const bool many = attend_many_rows(a);
+    a.max_rows = many && a.batch.n_seqs == 1 ? 0 : a.batch.max_q_len * group <= 8 || (many && group <= 8) ? 8 : kRowsMax;
     a.page_shift = -1;
     for (int i = 3; i < 31; ++i)
         if (a.page_size == 1 << i) a.page_shift = i;

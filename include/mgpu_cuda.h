@@ -88,7 +88,8 @@ int mgpu_device_ordinal(const mgpu_device* dev);
 int mgpu_device_sm_count(const mgpu_device* dev);
 size_t mgpu_device_l2_bytes(const mgpu_device* dev);
 /* The cudaStream_t all dispatches are enqueued on.  mgpu_set_stream replaces it (the caller
- * keeps ownership of a stream it passes in; NULL restores the device's own stream). */
+ * keeps ownership of a stream it passes in; NULL restores the device's own stream).  The dispatches
+ * share the device's scratch: finish what runs on the stream before, or order the new one after it. */
 void* mgpu_device_stream(const mgpu_device* dev);
 int mgpu_set_stream(mgpu_device* dev, void* cuda_stream);
 /* 0: dispatches return NULL (no event recorded, like passing no event in OpenCL);
@@ -361,7 +362,8 @@ mgpu_event* mgpu_kv_append(const mgpu_kv_cache* cache, const mgpu_paged_batch* b
  * at their tag's pitch; q_heads a multiple of kv_heads, at most 128 to a key head.  scale 0 means
  * 1 / sqrt(head_dim).  fp32 scores, softmax and sums.  The tensor cores take a weight in the cache's
  * type: in two parts, 16 to 22 bits, for single tokens and other few rows (a sequence's new tokens times the
- * query heads of a key head, up to 8 or 16), else rounded to it.  Uses the device's scratch (run once before a graph capture). */
+ * query heads of a key head, up to 8 or 16), else rounded to it.  Uses the device's scratch (run once
+ * before a graph capture). */
 mgpu_event* mgpu_paged_attention(const mgpu_kv_cache* cache, const mgpu_paged_batch* batch, mgpu_buf* q, mgpu_buf* out,
                                  int q_heads, float scale, int causal, int window);
 
@@ -393,8 +395,9 @@ typedef struct mgpu_logit_rules {
 } mgpu_logit_rules;
 /* out = rules(logits) for `rows` rows of n logits (f32 / f16 / bf16, each buffer's rows at its
  * tag's pitch, default n); out of logits' type, may be logits itself, or NULL.  best (>= 8 bytes a
- * row, or NULL) receives each row's {int32 index, fp32 value} as mgpu_argmax_rows(out) would.  Neither
- * out nor best may overlap anything else of the call. */
+ * row, or NULL) receives each row's {int32 index, fp32 value} as mgpu_argmax_rows(out) would, and uses
+ * the device's scratch (run once before a graph capture).  Neither out nor best may overlap anything
+ * else of the call. */
 mgpu_event* mgpu_logits_process(const mgpu_device* dev, mgpu_buf* logits, mgpu_buf* out, int rows, int n,
                                 const mgpu_logit_rules* rules, mgpu_buf* best);
 

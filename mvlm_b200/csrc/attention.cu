@@ -115,14 +115,16 @@ __device__ __forceinline__ bool named_barrier_or(int id, int threads, bool p) {
 // 15 clocks an instruction (it has left the instruction caches by then) 600 of them cost as much as
 // five blocks.
 // Measured (bf16, 8 key heads of 128, 4 rows): 64 sequences of 2150 tokens on average, 559 MB, in
-// 102 us, 5.46 TB/s, 83 % of a copy's; one of 131,002 tokens, 537 MB, in 91 us, 90 %.  256 sequences of
-// 540 reach 68 %: what an item costs is then seen.
+// 102 us, 5.48 TB/s, 84 % of a copy's; one of 131,002 tokens, 537 MB, in 91 us, 90 %.  256 sequences of
+// 540 reach 67 %: what an item costs is then seen.  16 rows: 128 us for the 64 sequences.
 constexpr int kRowsWarps = 8, kRowsThreads = 32 * (kRowsWarps + 3);  // then: keys, values, items
 constexpr int kRowsMax = 16;
 constexpr int kSeqCap = 1024;  // sequences whose block counts are kept in shared memory
 
 // Keys of a block: 32 KB whatever the head's dims, so that what a block costs beside its products
 // (waits, maxima) falls on as many bytes (64 sequences of 64 dims: 77 us with 64 keys, 60 with 128).
+// Heads of 72 to 96 dims take the stages of 128, filled to 56 to 75 %: 97 us for 64 sequences of 80 dims,
+// 349 MB, 55 % of a copy's.
 template <int DP> constexpr int rows_keys() { return DP == 64 ? 128 : 64; }
 template <int DP> constexpr int rows_stage_bytes() { return 2 * rows_keys<DP>() * DP * 2; }
 // 128 KB in flight, some three times what HBM's latency at full rate asks of an SM.  An even number,
@@ -782,14 +784,14 @@ cudaError_t launch_rows(const mgpu_k::LaunchCtx& c, const CUtensorMap& mk, const
 // +14 %), two threads to a row (453 us), the next scores in registers a half ahead (517 us).
 //
 // Which kernel: at most 16 rows go to the one above (64 sequences of 2150 tokens, 4 rows: 102 us there,
-// 150 here; 16 rows: 125 and 151; sequences of 250 tokens and 16 rows are the exception, 56 and 48).
-// A call with one sequence that may have more rows launches this kernel alone (761 tokens: 20.2 us, and
-// 22.6 with the other beside it).
+// 146 here; 16 rows: 128 and 147; 256 sequences of 250 tokens and 16 rows are the exception, 166 and 142), or
+// at most 8 of them (see paged_attention).  A call with one sequence that may have more rows launches this
+// kernel alone (761 tokens: 20.5 us, and 23.5 with the other beside it).
 constexpr int kTileKeys = 128, kTileRows = 128;
 constexpr int kTileThreads = 384;  // 8 softmax warps, then: products, loads, products, scheduling
 constexpr int kTileSeqs = 1024;    // sequences of one launch
 constexpr int kTileEntries = 2048; // entries of the table of items
-constexpr int kJoinBlocks = 6;     // what a join costs, in blocks (some 10 us)
+constexpr int kJoinBlocks = 6;     // what a join costs, in blocks (some 10 us for 64 dims, more for 128)
 
 template <int DP> constexpr int tile_stage_bytes() { return kTileKeys * DP * 2; }
 // K on even and V on odd stages: two blocks of 128 dims, four of 64
@@ -1024,8 +1026,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     for (int w = 0; w < kTileThreads / 32; ++w) most = max(most, warp_part[w]);
     const int head_blocks = cum[entries], total = head_blocks * a.hkv, items = pairs * a.hkv;
-    // Whole items, one to a CTA, unless cutting them saves more than a join costs (32 heads of 64 dims: 257
-    // new tokens 12.9 us whole and 20.6 cut, 761 tokens 20.3 and 22.2; 2000 tokens have too many items).
+    // Whole items, one to a CTA, unless cutting them saves more than a join costs.  32 heads of 64 dims: 257 new
+    // tokens 13.2 us whole and 21.0 cut, 761 tokens 20.5 and 22.7, 1024 tokens 24.8 and 27.8; of 128 dims: 16.3 and
+    // 30.2, 24.9 and 30.0, 29.4 and 36.5; 2000 tokens have too many items.
     const bool by_item = items <= (int)gridDim.x && most <= (total + (int)gridDim.x - 1) / (int)gridDim.x + kJoinBlocks;
     const int shares = by_item ? items : min((int)gridDim.x, total);
     if ((int)blockIdx.x >= shares) return;

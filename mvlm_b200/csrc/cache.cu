@@ -4,8 +4,9 @@
 // The reference rotates q and k in place and copies k and v into a contiguous cache
 // (dispatch_rope_apply and kv_cache_append, src/models/moondream2.cpp:406-420): three passes over
 // the activations.  Here each value is read once and written once: the bound is
-// T (Hq + 2 Hkv) D (source + cache bytes) at HBM rate.  Measured: 13,100 tokens of 32 + 16 heads of
-// 128, bf16, 322 MB, in 60 us, 5.4 TB/s, 82 % of a copy's; 761 tokens of 96 heads of 64 in 4.9 us.
+// T (Hq + 2 Hkv) D (source + cache bytes) and 4 T rot_dim of the rotation's table at HBM rate.  Measured: 12,814
+// tokens of 32 + 16 heads of 128, bf16, 322 MB, in 60 us, 5.4 TB/s, 82 % of a copy's; the same from fp32, 479 MB, in
+// 75 us, 98 %; 761 tokens of 96 heads of 64 in 4.9 us.
 #include <climits>
 #include <type_traits>
 
@@ -227,8 +228,8 @@ __device__ __forceinline__ void store1(void* p, int type, int64_t i, float v) {
     else reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
 }
 
-// The same for rows, pitches or rotations that do not fall on 16-byte boundaries: a thread to a pair,
-// or to a value that does not turn.
+// The same where rows, pitches or the halves of the rotation (rot_dim not a multiple of 16, of 8 for adjacent
+// pairs) do not fall on 16-byte boundaries: a thread to a pair, or to a value that does not turn.
 __global__ void __launch_bounds__(kAppendThreads) kv_append_single_kernel(const mgpu_k::AppendArgs a) {
     const int t = blockIdx.x, half = a.rot / 2, units = half + a.D - a.rot, heads = a.hq + 2 * a.hkv;
     Place place;
@@ -268,8 +269,9 @@ cudaError_t rope_table(const LaunchCtx& c, float* table, int max_pos, int rot, d
 }
 
 cudaError_t kv_append(const LaunchCtx& c, const AppendArgs& a) {
-    // 16-byte accesses need every row, and the two halves of a pair unit, on 16-byte boundaries; the kernel
-    // for the others takes 200 us where they take 59, and 18 us where they take 5
+    // 16-byte accesses need every row, and the two halves of a pair unit, on 16-byte boundaries: split halves of
+    // rot_dim 20, 24 or 40 do not have them, whatever the rows.  The kernel for the others takes 200 us where they
+    // take 60, and 18 us where they take 5; 12,814 tokens of heads of 80 take 209 us with rot_dim 40, 51 with 80.
     auto ok = [](const void* p, int type, int64_t ld) {
         return !p || (((uintptr_t)p & 15) == 0 && (ld * (type == MGPU_F32 ? 4 : 2)) % 16 == 0);
     };
@@ -284,7 +286,7 @@ cudaError_t kv_append(const LaunchCtx& c, const AppendArgs& a) {
     }
     // Few tokens: one pass of heads per CTA, so that a decode step's launch is one round of loads (64
     // tokens of 144 heads: 6.2 us cold, 9.4 with a CTA to a token).  Many: a CTA keeps its token's heads,
-    // so that the look-ups are paid once (5 prompts of 2620 tokens: 59 us, 126 with a pass per CTA).
+    // so that the look-ups are paid once (5 prompts, 12,814 tokens: 59 us, 126 with a pass per CTA).
     int gy = 1;
     while (gy < passes && gy < 65535 && (int64_t)a.batch.n_tokens * gy < 4 * c.sm_count) ++gy;
     cudaLaunchConfig_t cfg = {};
@@ -301,7 +303,7 @@ cudaError_t kv_append(const LaunchCtx& c, const AppendArgs& a) {
         constexpr int ST = decltype(st)::value, DT = decltype(dt)::value;
         return cudaLaunchKernelEx(&cfg, a.interleaved ? kv_append_kernel<true, ST, DT> : kv_append_kernel<false, ST, DT>, a);
     };
-    // The usual types are compiled in (5 prompts of 2620 tokens of 48 heads of 128 in 59 us, one of 761 in
+    // The usual types are compiled in (5 prompts, 12,814 tokens of 48 heads of 128, in 59 us, one of 761 in
     // 4.9); types that differ between q, k and v, or q_out's from the cache's, are looked at value by value
     // (75 and 8 us for the same).
     using F32 = std::integral_constant<int, MGPU_F32>;

@@ -23,7 +23,7 @@ using namespace mgpu_dev;
 namespace {
 
 constexpr int kRulesThreads = 256;
-constexpr int kPiece = 8192;  // tokens of a CTA's round: at most 32 KB of logits, 32 KB of words, 16 KB of places
+constexpr int kPiece = 8192;  // tokens of a CTA's round: at most 32 KB of logits, 32 KB of words, 2 KB of places
 constexpr int kIds = 8;        // entries of the history that a thread keeps
 constexpr int kListed = 1024;  // marked tokens that a round lists
 // A token's word: how often the history after the prompt holds it, whether the prompt does, and its
@@ -304,7 +304,10 @@ cudaError_t launch_rules(const mgpu_k::LaunchCtx& c, const mgpu_k::RulesArgs& a)
         configured.fetch_or(bit, std::memory_order_acq_rel);
     }
     // CTAs to a row: enough of them to fill the device, and short ranges (a range's waits come one after
-    // another).  One row of 51200: 20 us by one CTA, 13 by 2, 8.6 by 4, 8.0 by 8; 256 rows: 48, 48, 42, 37.
+    // another).  One row of 51200: 20 us by one CTA, 13 by 2, 8.6 by 4, 6.6 by 8; 256 rows: 48, 48, 42, 37.  More
+    // than 8 were measured in a copy whose join reads 32 results in place of 8, which alone costs 2 to 5 us: 256
+    // rows 58 us by 16 and 93 by 32, one row of 51200 9.0 and 9.2.  One row of 200,000 is the exception: 13.1 us
+    // by 8, 8.6 by 16 and 6.7 by 32.
     int ctas = 1;
     while (ctas < 8 && ((int64_t)a.rows * ctas < 4 * c.sm_count || (a.n + ctas - 1) / ctas > kPiece)) ctas *= 2;
     const int range = ((a.n + ctas - 1) / ctas + 31) / 32 * 32;

@@ -920,6 +920,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __shared__ Segment segs[kSegments];
     __shared__ uint32_t tmem_slot;
     __shared__ int warp_part[kTileThreads / 32];
+    __shared__ bool beyond;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = a.hq / a.hkv, per_tile = kTileRows / G;
 
@@ -943,6 +944,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             mbar_init(&seg_full[i], 1);
             mbar_init(&seg_empty[i], 11);  // all warps but the scheduling one
         }
+        beyond = false;
         fence_mbar_init();
         prefetch_tensormap(&tmK);
         prefetch_tensormap(&tmV);
@@ -959,8 +961,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if ((long long)s.n * G <= a.max_rows) s.n = 0;  // the rows kernel's
         return s;
     };
-    // exclusive prefix sums of v[0 .. n) in place, the total at v[n]
-    auto scan = [&](int* v, int n) {
+    // exclusive prefix sums of v[0 .. n) in place, the total at v[n]; `beyond` is set if one is more than `most`
+    auto scan = [&](int* v, int n, int most) {
         const int each = (n + kTileThreads - 1) / kTileThreads, i0 = min(n, tid * each), i1 = min(n, i0 + each);
         int sum = 0;
         for (int i = i0; i < i1; ++i) sum += v[i];
@@ -978,25 +980,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const int x = v[i];
             v[i] = before;
             before += x;
+            if ((unsigned)before > (unsigned)most) beyond = true;
         }
         if (tid == kTileThreads - 1) v[n] = before;
         __syncthreads();
     };
-    bool descends = false;
-    for (int b = tid; b < seqs; b += kTileThreads) {
-        descends |= a.batch.cu_q[seq0 + b + 1] < a.batch.cu_q[seq0 + b];
-        seq_first[b] = (view(b).n + 2 * per_tile - 1) / (2 * per_tile);
-    }
-    if (__syncthreads_or(descends)) {
-        // Sequences that share rows, between which cu_q descends, could have more items than the host's bound
-        // on the 32-bit counts below allows for.
-        long long rows = 0;
-        for (int b = 0; b < seqs; ++b) rows += view(b).n;
-        if (rows > a.batch.n_tokens) return;
-    }
-    scan(seq_first, seqs);
+    for (int b = tid; b < seqs; b += kTileThreads) seq_first[b] = (view(b).n + 2 * per_tile - 1) / (2 * per_tile);
+    __syncthreads();
+    // Sequences that share rows, between which cu_q descends, could have more pairs than the host's bound on the
+    // 32-bit counts below allows for.  (One has at most 2^23, so that the sums cannot pass over the bound.)
+    scan(seq_first, seqs, a.batch.n_tokens / (2 * per_tile) + a.batch.n_seqs);
     const int pairs = seq_first[seqs];
-    if (pairs == 0) return;
+    if (pairs == 0 || beyond) return;
     auto seq_of_pair = [&](int p) {  // the last b with seq_first[b] <= p
         int lo2 = 0, hi2 = seqs;
         while (hi2 - lo2 > 1) {
@@ -1021,7 +1016,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     most = __reduce_max_sync(0xffffffffu, most);
     __syncthreads();
-    scan(cum, entries);
+    scan(cum, entries, INT_MAX);
     if (lane == 0) warp_part[warp] = most;
     __syncthreads();
     for (int w = 0; w < kTileThreads / 32; ++w) most = max(most, warp_part[w]);
